@@ -321,6 +321,135 @@ int rec_set_option(rec_engine* e, const char* name, int64_t value);
  * which = 6 (not reset, no device call): the launch shape in effect - *total_ms = "user_batch", *launches = "global_window". */
 int rec_kernel_stats(rec_engine* e, int which, double* total_ms, int64_t* launches);
 
+/* ---- Device operators of sequence models: histories and losses over a catalogue's scores ------------------------------
+ * No counterpart in the reference, whose models weight a history's clicks with fixed taps (Fossil.cpp:286-296,
+ * REBUS.cpp:540-554) and score one item against one other.  A history is packed as in rec_corpus: the rows of sequence s
+ * are seq_off[s] .. seq_off[s+1]-1 (int64, not decreasing, within [0, rows]; empty sequences allowed).  Rows before
+ * seq_off[0] and from seq_off[n_seq] on belong to no sequence: outputs leave them as they were, or zero with "zero_rest" 1.
+ * Offsets, items and slots are read on the device and are not checked by the host; values that break the rules above give
+ * meaningless numbers, but nothing outside the arrays described here is read or written.
+ *
+ * All data pointers are memory of GPU `device`, aligned to their element type.  Strides count elements between rows; the
+ * channels (items) of a row are contiguous.  Parameters, recurrent states, sums and per-row results are f32; "type" is that of
+ * the activations and of the scores.  Calls only enqueue kernels on `stream` (a hipStream_t; NULL = the default stream), allocate
+ * nothing, wait for nothing and can be captured into a HIP graph.  A workspace needs no initial contents and holds nothing
+ * between calls; calls that may overlap in time, replays of two captured graphs among them, need one each.  The outputs of a
+ * call must not overlap its inputs or each other, except where an entry says so.  Results do not depend on timing: equal inputs
+ * give equal bits.  Entry points that need a workspace of rec_..._workspace() bytes take NULL where that is 0. */
+enum rec_type { REC_TYPE_F32 = 0, REC_TYPE_F16 = 1, REC_TYPE_BF16 = 2 };
+
+typedef struct {
+    int32_t device, type;     /* HIP device ordinal, enum rec_type */
+    int64_t rows;             /* packed rows (steps: clicks), at most 2^31 - 1 */
+    int32_t n_seq;            /* sequences (steps: slots of the state) */
+    int32_t channels;
+    int32_t taps;             /* 2 .. 8 */
+    int32_t silu;             /* 1: y = v / (1 + exp(-v)) of the sum v below, 0: y = v */
+    int32_t zero_rest;        /* 1: output rows outside all sequences are set to 0 */
+} rec_conv_desc;
+
+/* Short causal convolution over each history, one filter per channel:
+ *     v[t][d] = bias[d] + sum_{j < taps} weight[d][j] * x[t - (taps-1) + j][d],      y = silu(v) or v
+ * where rows before a history's first come from its window initial[s][taps-1][channels] (oldest first; NULL: zeros).
+ * weight [channels][taps], bias [channels] or NULL.  final_window (optional, [n_seq][taps-1][channels], of `type`): the last
+ * taps-1 rows of every history, its initial window included - what the next call, or a step, goes on from. */
+int rec_history_conv(const rec_conv_desc* d, const void* x, int64_t x_stride, const float* weight, const float* bias,
+                     const int64_t* seq_off, const void* initial, void* y, int64_t y_stride, void* final_window, void* stream);
+
+/* Its gradient for dy and (optional) dfinal [n_seq][taps-1][channels]: dx, and where not NULL dweight [channels][taps],
+ * dbias [channels] and dinitial [n_seq][taps-1][channels]. */
+int64_t rec_history_conv_backward_workspace(const rec_conv_desc* d);
+int rec_history_conv_backward(const rec_conv_desc* d, const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,
+                              const float* weight, const float* bias, const int64_t* seq_off, const void* initial,
+                              const void* dfinal, void* dx, int64_t dx_stride, float* dweight, float* dbias, void* dinitial,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+
+/* One click for each of `rows` histories kept in a pool of n_seq windows, window [n_seq][taps-1][channels]: row r appends to
+ * the window slots[r], in place, and y[r] is the convolution's value there.  Rows that name the same slot are taken in
+ * row order, as consecutive clicks; a row whose slot is outside [0, n_seq) moves nothing and gets zeros.  At most 65536 rows. */
+int rec_history_conv_step(const rec_conv_desc* d, const void* x, int64_t x_stride, const float* weight, const float* bias,
+                          const int32_t* slots, void* window, void* y, int64_t y_stride, void* stream);
+
+typedef struct {
+    int32_t device, type;
+    int64_t rows;             /* packed rows (steps: clicks), at most 2^31 - 1 */
+    int32_t n_seq;            /* sequences (steps: slots of the state) */
+    int32_t channels, groups; /* channel d takes B and C of group d / (channels / groups); groups divides channels */
+    int32_t states;           /* 1 .. 64 per channel */
+    int32_t softplus;         /* 1: delta = log(1 + exp(v)), 0: delta = v, of v = raw delta + delta_bias */
+    int32_t zero_rest;
+} rec_scan_desc;
+
+/* What a scan reads.  u, delta, z: [rows][channels] of `type` (z may be NULL: no gate); B, C: [rows][groups][states] of
+ * `type`, the groups of a row contiguous; A [channels][states], D [channels] and delta_bias [channels] f32 (the last two may be
+ * NULL); initial [n_seq][channels][states] f32 (NULL: zeros; not used by a step). */
+typedef struct {
+    const void *u, *delta, *z, *B, *C;
+    int64_t u_stride, delta_stride, z_stride, B_stride, C_stride;
+    const float *A, *D, *delta_bias, *initial;
+} rec_scan_inputs;
+
+/* Selective state space scan over each history, h[channels][states] starting at its initial state:
+ *     h = exp(delta_t A) h + delta_t u_t B_t        y_t = (sum_n C_t[n] h[n] + D u_t) * (z_t / (1 + exp(-z_t)))
+ * final_state (optional): [n_seq][channels][states] f32, initial of an empty history.  checkpoints (optional): the states in
+ * front of every REC_SCAN_CHECKPOINT-th packed row, [ceil(rows / REC_SCAN_CHECKPOINT)][channels][states] f32, which the
+ * gradient starts its recomputation from. */
+#define REC_SCAN_CHECKPOINT 16
+int64_t rec_history_scan_workspace(const rec_scan_desc* d);
+int rec_history_scan(const rec_scan_desc* d, const rec_scan_inputs* in, const int64_t* seq_off, void* y, int64_t y_stride,
+                     float* final_state, float* checkpoints, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Its gradient for dy and (optional) dfinal [n_seq][channels][states].  checkpoints: as rec_history_scan wrote them for the
+ * same inputs.  du, ddelta (of the raw delta) and dz (with z only) [rows][channels], contiguous rows; dB, dC [rows][groups][states],
+ * contiguous; dA, dD, ddelta_bias, dinitial f32, each may be NULL. */
+typedef struct {
+    void *du, *ddelta, *dz, *dB, *dC;
+    float *dA, *dD, *ddelta_bias, *dinitial;
+} rec_scan_gradients;
+int64_t rec_history_scan_backward_workspace(const rec_scan_desc* d);
+int rec_history_scan_backward(const rec_scan_desc* d, const void* dy, int64_t dy_stride, const rec_scan_inputs* in,
+                              const int64_t* seq_off, const float* checkpoints, const float* dfinal, const rec_scan_gradients* out,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+
+/* One click for each of `rows` histories whose states are kept in a pool, state [n_seq][channels][states] f32, updated in
+ * place; slots as for rec_history_conv_step. */
+int rec_history_scan_step(const rec_scan_desc* d, const rec_scan_inputs* in, const int32_t* slots, float* state, void* y,
+                          int64_t y_stride, void* stream);
+
+/* Losses of a policy that chooses item j of the catalogue with probability p[t][j] = softmax over j of scale * scores[t][j].
+ * items masked with -inf have probability 0.  A row takes no part - log-probability and gradient 0 - when its item is outside
+ * [0, n_items) or all its scores are -inf. */
+typedef struct {
+    int32_t device, type;
+    int64_t rows;             /* at most 2^22 - 1 */
+    int64_t n_items;          /* 1 .. 2^31 - 1 */
+    float scale;              /* > 0 (an inverse temperature) */
+    int32_t zero_rest;
+} rec_loss_desc;
+
+/* Preferences between two lists of choices: pair p prefers the rows of sequence 2p to those of sequence 2p+1 (seq_off:
+ * 2 n_pairs + 1 offsets), a list's log-ratio being sum over its rows of log p[t][item[t]] - ref_logp[t] (NULL: 0).
+ *     margin = beta * (log-ratio of 2p - log-ratio of 2p+1)
+ *     loss = -(1 - smoothing) log sigmoid(margin) - smoothing log sigmoid(-margin)
+ * logp[t] = log p[t][item[t]] of rows in a sequence.  With grad_weight [n_pairs], dscores [rows][n_items] is the gradient of
+ * sum_p grad_weight[p] loss[p] (both NULL: no gradient); dscores may be the scores themselves, with the same stride. */
+int64_t rec_preference_loss_workspace(const rec_loss_desc* d, int32_t n_pairs);
+int rec_preference_loss(const rec_loss_desc* d, const void* scores, int64_t scores_stride, const int32_t* item,
+                        const int64_t* seq_off, int32_t n_pairs, const float* ref_logp, float beta, float smoothing,
+                        const float* grad_weight, float* loss, float* margin, float* logp, void* dscores, int64_t dscores_stride,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Clipped policy loss of every row, for a choice made with log-probability old_logp and the given advantage:
+ *     r = exp(logp - old_logp)     kl = exp(ref_logp - logp) - (ref_logp - logp) - 1
+ *     loss = -min(r * advantage, clip(r, 1 - clip_low, 1 + clip_high) * advantage) + kl_coef * kl
+ * ref_logp NULL: no KL term (kl NULL or zeros, kl_coef 0).  With grad_weight [rows], dscores is the gradient of
+ * sum_t grad_weight[t] loss[t]; it may be the scores themselves, with the same stride. */
+int64_t rec_policy_loss_workspace(const rec_loss_desc* d);
+int rec_policy_loss(const rec_loss_desc* d, const void* scores, int64_t scores_stride, const int32_t* item,
+                    const float* old_logp, const float* advantage, const float* ref_logp, float clip_low, float clip_high,
+                    float kl_coef, const float* grad_weight, float* loss, float* kl, float* logp, void* dscores,
+                    int64_t dscores_stride, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

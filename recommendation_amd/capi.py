@@ -15,7 +15,10 @@ SEQUENTIAL, HOGWILD = 0, 1
 EXPORTS = ["rec_last_error", "rec_create", "rec_destroy", "rec_sync", "rec_nw", "rec_params_upload",
            "rec_params_download", "rec_params_read", "rec_params_init", "rec_snapshot_best", "rec_restore_best", "rec_sgd_replay", "rec_sgd_replay_static", "rec_partition_tuples", "rec_owner_slices",
            "rec_sgd_epoch", "rec_sample_tuples", "rec_sample_events", "rec_tuples_drawn", "rec_steps_per_epoch", "rec_eval", "rec_eval_sampled", "rec_eval_sampled_per_user", "rec_eval_topk", "rec_eval_user_count", "rec_eval_sums",
-           "rec_device_count", "rec_shards_begin_round", "rec_shards_combine", "rec_project_rows", "rec_rebus_build_paths", "rec_fsub_mine", "rec_num_tables", "rec_table_info", "rec_set_option", "rec_kernel_stats"]
+           "rec_device_count", "rec_shards_begin_round", "rec_shards_combine", "rec_project_rows", "rec_rebus_build_paths", "rec_fsub_mine", "rec_num_tables", "rec_table_info", "rec_set_option", "rec_kernel_stats",
+           "rec_history_conv", "rec_history_conv_backward_workspace", "rec_history_conv_backward", "rec_history_conv_step",
+           "rec_history_scan_workspace", "rec_history_scan", "rec_history_scan_backward_workspace", "rec_history_scan_backward", "rec_history_scan_step",
+           "rec_preference_loss_workspace", "rec_preference_loss", "rec_policy_loss_workspace", "rec_policy_loss"]
 
 
 class RecCorpus(C.Structure):

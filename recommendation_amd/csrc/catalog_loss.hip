@@ -1,0 +1,412 @@
+// Losses of a softmax policy over a catalogue's scores, with their gradient: preferences between lists, and the clipped policy
+// loss with a KL term.
+//
+//   log p[t][j] = scale (s[t][j] - m_t) - log l_t,   m_t = max_j s[t][j],   l_t = sum_j exp(scale (s[t][j] - m_t))
+//   dscores[t][j] = scale c_t (1[j = item_t] - p[t][j]),   c_t = d(weighted loss) / d(log p of row t's item)
+//
+// One exp and a few flop per score: bound by memory.  A block reads a row (or, where rows are few, a part of one) once, with
+// the running maximum and sum in registers; a row's parts are joined by whoever needs the row's loss.  Everything that is one number
+// per row is computed in 64 bits - a list's log-ratio is a small difference of sums of log-probabilities - and
+// rounded once when it is stored.
+#include "operators.h"
+#include <float.h>
+
+namespace {
+
+struct LossArgs {
+    const void* scores;
+    const int32_t* item;
+    const int64_t* off;                       // preference only
+    const float *ref_logp, *old_logp, *advantage, *grad_weight;
+    float *loss, *margin, *kl, *logp;
+    void* dscores;
+    float4* part;                             // [rows][splits] statistics of a row's parts
+    float2* stat;                             // [rows] (max, log2 of the sum) of a row
+    float* coef;                              // [rows] c_t, 0 where a row takes no part
+    int64_t rows, n_items, scores_stride, dscores_stride;
+    float scale, scale2;                      // scale2 = scale * log2(e), rounded
+    double scale_rest;                        // scale - scale2 / log2(e)
+    int n_seq, splits, zero_rest;
+    double beta, smoothing, clip_low, clip_high, kl_coef;
+};
+
+// What is known of a set of scores: its maximum m, l = sum of 2^(c (x - m)) and q = sum of (x - m) 2^(c (x - m)), c being scale *
+// log2(e) rounded to f32.  The rounding of c is the same for every score: it would move log l of all rows the same way (by 6e-8 for
+// scores of deviation 2), and the log-ratio of lists of different lengths by that times their difference.  q is the derivative of l by c
+// that takes it out again, to first order.  m is -inf for a set with nothing in it.
+struct Stat { float m, l, q; };
+
+__device__ __forceinline__ Stat join(Stat a, Stat b, float c)
+{
+    const float m = fmaxf(a.m, b.m), base = m == -INFINITY ? 0.0f : m;
+    // a set without a finite maximum has l = q = 0, or is NaN
+    const float da = a.m == -INFINITY ? 0.0f : a.m - base, db = b.m == -INFINITY ? 0.0f : b.m - base;
+    const float fa = fast_exp2(da * c), fb = fast_exp2(db * c);
+    return {m, a.l * fa + b.l * fb, (fa > 0.0f ? fmaf(da, a.l, a.q) * fa : 0.0f) + (fb > 0.0f ? fmaf(db, b.l, b.q) * fb : 0.0f)};
+}
+
+// the statistics of the scores [j0, j1) of a row, over the block; valid in every thread.  NaN scores give a NaN sum.
+template <class T>
+__device__ __forceinline__ Stat row_statistics(const T* __restrict__ row, int64_t j0, int64_t j1, float c, Stat* red)
+{
+    constexpr int V = 16 / sizeof(T);
+    Stat st = {-INFINITY, 0.0f, 0.0f};
+    auto add = [&](const float (&x)[V]) {
+        float m = x[0];
+#pragma unroll
+        for (int v = 1; v < V; v++) m = fmaxf(m, x[v]);
+        if (m > st.m) {   // rarely, after the first few
+            const float d = st.m == -INFINITY ? 0.0f : st.m - m, f = fast_exp2(d * c);
+            st.q = f > 0.0f ? fmaf(d, st.l, st.q) * f : 0.0f;
+            st.l *= f;
+            st.m = m;
+        }
+        const float base = st.m == -INFINITY ? 0.0f : st.m;
+        float l = 0.0f, q = 0.0f;
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            const float d = x[v] - base, e = fast_exp2(d * c);
+            l += e;
+            q = fmaf(fmaxf(d, -FLT_MAX), e, q);   // a masked score adds 0, not -inf * 0
+        }
+        st.l += l;
+        st.q += q;
+    };
+    // 16-byte loads from the first aligned element on; what is in front of it and behind the last whole vector singly
+    const int64_t a0 = j0 + (int64_t)(((16 - ((uintptr_t)(row + j0) & 15)) & 15) / sizeof(T));
+    const int64_t lead = a0 < j1 ? a0 : j1, vecs = (j1 - lead) / V, tail = lead + vecs * V;
+    const Pack<T, V>* p = reinterpret_cast<const Pack<T, V>*>(row + lead);
+    for (int64_t i = threadIdx.x; i < vecs; i += blockDim.x) {
+        const Pack<T, V> raw = p[i];
+        float x[V];
+#pragma unroll
+        for (int v = 0; v < V; v++) x[v] = to_f32(raw.v[v]);
+        add(x);
+    }
+    {
+        const int64_t n = (lead - j0) + (j1 - tail);   // at most 2 V - 2
+        if ((int64_t)threadIdx.x < n) {
+            const int64_t j = (int64_t)threadIdx.x < lead - j0 ? j0 + threadIdx.x : tail + (threadIdx.x - (lead - j0));
+            float x[V];
+#pragma unroll
+            for (int v = 0; v < V; v++) x[v] = v == 0 ? to_f32(row[j]) : -INFINITY;
+            add(x);
+        }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) st = join(st, {__shfl_xor(st.m, o, 64), __shfl_xor(st.l, o, 64), __shfl_xor(st.q, o, 64)}, c);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = st;
+    __syncthreads();
+    st = red[0];
+    for (int w = 1; w < (int)blockDim.x / 64; w++) st = join(st, red[w], c);
+    return st;
+}
+
+__device__ __forceinline__ bool row_counts(const LossArgs& a, int64_t row)
+{
+    return a.item[row] >= 0 && a.item[row] < a.n_items;
+}
+
+template <class T>
+__global__ __launch_bounds__(1024) void row_statistics_kernel(LossArgs a)
+{
+    __shared__ Stat red[16];
+    const int64_t row = blockIdx.x / a.splits;
+    const int split = blockIdx.x % a.splits;
+    if (!row_counts(a, row)) return;
+    if (a.off && (row < a.off[0] || row >= a.off[a.n_seq])) return;
+    const int64_t per = (a.n_items + a.splits - 1) / a.splits, j0 = split * per, j1 = j0 + per < a.n_items ? j0 + per : a.n_items;
+    const Stat st = row_statistics((const T*)a.scores + row * a.scores_stride, j0 < j1 ? j0 : j1, j1, a.scale2, red);
+    if (threadIdx.x == 0) a.part[blockIdx.x] = make_float4(st.m, st.l, st.q, 0.0f);
+}
+
+// log p of a row's item from its parts; false: the row takes no part
+template <class T>
+__device__ __forceinline__ bool row_log_probability(const LossArgs& a, int64_t row, double& logp)
+{
+    logp = 0.0;
+    if (!row_counts(a, row)) return false;
+    Stat st = {-INFINITY, 0.0f, 0.0f};
+    for (int k = 0; k < a.splits; k++) {
+        const float4 p = a.part[row * a.splits + k];
+        st = join(st, {p.x, p.y, p.z}, a.scale2);
+    }
+    if (st.m == -INFINITY && st.l == 0.0f) return false;
+    const double l = log((double)st.l);
+    a.stat[row] = make_float2(st.m, (float)(l * 1.4426950408889634));   // (base 2)
+    logp = (double)a.scale * ((double)to_f32(((const T*)a.scores)[row * a.scores_stride + a.item[row]]) - (double)st.m) - l - a.scale_rest * (double)st.q / (double)st.l;
+    return true;
+}
+
+__device__ __forceinline__ double softplus64(double v) { return fmax(v, 0.0) + log1p(exp(-fabs(v))); }
+
+// a block per pair; its threads take the rows of both lists, and add up in a fixed order
+template <class T>
+__global__ __launch_bounds__(256) void preference_kernel(LossArgs a)
+{
+    __shared__ double red[256];
+    const int64_t p = blockIdx.x;
+    double sum = 0.0;
+    int64_t begin[3];
+#pragma unroll
+    for (int k = 0; k < 3; k++) {   // offsets that break the rules stay within the rows
+        const int64_t o = a.off[2 * p + k];
+        begin[k] = o < 0 ? 0 : o > a.rows ? a.rows : o;
+    }
+#pragma unroll
+    for (int side = 0; side < 2; side++)
+        for (int64_t row = begin[side] + threadIdx.x; row < begin[side + 1]; row += 256) {
+            double logp;
+            const bool on = row_log_probability<T>(a, row, logp);
+            a.logp[row] = (float)logp;
+            if (on && a.ref_logp) logp -= (double)a.ref_logp[row];
+            sum += side ? -logp : logp;
+            a.coef[row] = on ? (side ? -1.0f : 1.0f) : 0.0f;
+        }
+    red[threadIdx.x] = sum;
+    __syncthreads();
+    for (int n = 128; n > 0; n >>= 1) {
+        if ((int)threadIdx.x < n) red[threadIdx.x] += red[threadIdx.x + n];
+        __syncthreads();
+    }
+    const double m = a.beta * red[0];
+    if (threadIdx.x == 0) {
+        a.margin[p] = (float)m;
+        double loss = 0.0;   // a term with weight 0 adds nothing, be it infinite
+        if (a.smoothing < 1.0) loss += (1.0 - a.smoothing) * softplus64(-m);
+        if (a.smoothing > 0.0) loss += a.smoothing * softplus64(m);
+        a.loss[p] = (float)loss;
+    }
+    if (!a.grad_weight) return;
+    const float c = (float)(a.beta * (a.smoothing - 1.0 / (1.0 + exp(m))) * (double)a.grad_weight[p]);
+    for (int64_t row = begin[0] + threadIdx.x; row < begin[2]; row += 256) a.coef[row] = a.coef[row] == 0.0f ? 0.0f : a.coef[row] * c;
+}
+
+// loss, KL and c_t of one row
+__device__ __forceinline__ void policy_row(const LossArgs& a, int64_t row, double logp, bool on, float& coef)
+{
+    double loss = 0.0, kl = 0.0, c = 0.0;
+    if (on) {
+        const double adv = a.advantage[row], r = exp(logp - (double)a.old_logp[row]);
+        // an advantage of 0 asks for nothing, however far the ratio went
+        const double open = adv == 0.0 ? 0.0 : r * adv, held = adv == 0.0 ? 0.0 : fmin(fmax(r, 1.0 - a.clip_low), 1.0 + a.clip_high) * adv;
+        const bool nan = r != r || adv != adv;
+        loss = nan ? r * adv : -fmin(open, held);
+        c = nan ? r * adv : open <= held ? -open : 0.0;
+        if (a.ref_logp) {
+            const double x = (double)a.ref_logp[row] - logp, e = expm1(x);
+            kl = x == (double)INFINITY ? x : e - x;
+            if (a.kl_coef != 0.0) { loss += a.kl_coef * kl; c -= a.kl_coef * e; }
+        }
+    }
+    a.loss[row] = (float)loss;
+    if (a.kl) a.kl[row] = (float)kl;
+    a.logp[row] = (float)logp;
+    coef = a.grad_weight ? (float)(c * (double)a.grad_weight[row]) : 0.0f;
+    if (!on) coef = 0.0f;
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void policy_kernel(LossArgs a)
+{
+    const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (row >= a.rows) return;
+    double logp;
+    const bool on = row_log_probability<T>(a, row, logp);
+    policy_row(a, row, logp, on, a.coef[row]);
+}
+
+// the gradient's elements [j0, j1) of a row
+template <class T>
+__device__ __forceinline__ void write_gradient(const LossArgs& a, int64_t row, int64_t j0, int64_t j1, float coef, float2 st)
+{
+    constexpr int V = 16 / sizeof(T);
+    const T* in = (const T*)a.scores + row * a.scores_stride;
+    T* out = (T*)a.dscores + row * a.dscores_stride;
+    const float c = coef * a.scale;
+    const int item = a.item[row];
+    auto of = [&](float x, int64_t j) {
+        const float p = fast_exp2((x - st.x) * a.scale2 - st.y);
+        return from_f32<T>(c * ((j == item ? 1.0f : 0.0f) - p));
+    };
+    const int64_t a0 = j0 + (int64_t)(((16 - ((uintptr_t)(out + j0) & 15)) & 15) / sizeof(T));
+    const bool same = (((uintptr_t)(in + j0) ^ (uintptr_t)(out + j0)) & 15) == 0;   // rows of equal alignment move in 16-byte pieces
+    const int64_t lead = !same ? j1 : a0 < j1 ? a0 : j1, vecs = (j1 - lead) / V;
+    for (int64_t i = threadIdx.x; i < vecs; i += blockDim.x) {
+        const int64_t j = lead + i * V;
+        const Pack<T, V> q = *reinterpret_cast<const Pack<T, V>*>(in + j);
+        Pack<T, V> o;
+#pragma unroll
+        for (int v = 0; v < V; v++) o.v[v] = of(to_f32(q.v[v]), j + v);
+        *reinterpret_cast<Pack<T, V>*>(out + j) = o;
+    }
+    for (int64_t j = j0 + threadIdx.x; j < lead; j += blockDim.x) out[j] = of(to_f32(in[j]), j);
+    for (int64_t j = lead + vecs * V + threadIdx.x; j < j1; j += blockDim.x) out[j] = of(to_f32(in[j]), j);
+}
+
+template <class T>
+__device__ __forceinline__ void write_zeros(const LossArgs& a, int64_t row, int64_t j0, int64_t j1)
+{
+    T* out = (T*)a.dscores + row * a.dscores_stride;
+    for (int64_t j = j0 + threadIdx.x; j < j1; j += blockDim.x) out[j] = from_f32<T>(0.0f);
+}
+
+template <class T>
+__global__ __launch_bounds__(1024) void gradient_kernel(LossArgs a)
+{
+    const int64_t row = blockIdx.x / a.splits;
+    const int split = blockIdx.x % a.splits;
+    const int64_t per = (a.n_items + a.splits - 1) / a.splits, j0 = split * per, j1 = j0 + per < a.n_items ? j0 + per : a.n_items;
+    if (a.off && (row < a.off[0] || row >= a.off[a.n_seq])) {
+        if (!a.zero_rest) return;
+        write_zeros<T>(a, row, j0, j1);
+        if (split == 0 && threadIdx.x == 0) a.logp[row] = 0.0f;
+        return;
+    }
+    const float coef = a.coef[row];
+    if (coef == 0.0f) write_zeros<T>(a, row, j0, j1);   // p is finite or the row's coefficient is NaN: nothing to read
+    else write_gradient<T>(a, row, j0, j1, coef, a.stat[row]);
+}
+
+// rows of no list, where no gradient pass comes by
+__global__ __launch_bounds__(256) void rest_kernel(LossArgs a)
+{
+    const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (row < a.rows && (row < a.off[0] || row >= a.off[a.n_seq])) a.logp[row] = 0.0f;
+}
+
+int check_desc(const rec_loss_desc* d)
+{
+    REC_REFUSE(!d, "null argument");
+    REC_REFUSE(d->type < REC_TYPE_F32 || d->type > REC_TYPE_BF16, "unknown type");
+    REC_REFUSE(d->rows < 0 || d->rows > (1 << 22) - 1, "rows must be in 0..2^22-1");   // a launch holds fewer than 2^32 threads
+    REC_REFUSE(d->n_items < 1 || d->n_items > INT32_MAX, "n_items must be in 1..2^31-1");
+    REC_REFUSE(!(d->scale > 0.0f) || !isfinite(d->scale), "scale must be positive and finite");
+    return 0;
+}
+
+// Parts a row is cut into: one where the rows alone fill the chip (4 blocks of 512 threads per compute unit), else as many as
+// that takes, of at least 8192 items each.
+constexpr int kThreads = 512;
+int splits_of(const rec_loss_desc* d)
+{
+    const int64_t want = d->rows > 0 ? (1024 + d->rows - 1) / d->rows : 1, most = (d->n_items + 8191) / 8192;
+    const int64_t s = want < most ? want : most;
+    return (int)(s < 1 ? 1 : s > 256 ? 256 : s);
+}
+
+int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
+int64_t workspace_of(const rec_loss_desc* d) { return d->rows * splits_of(d) * 16 + round16(d->rows * 8) + round16(d->rows * 4); }
+
+int check_call(const rec_loss_desc* d, const void* scores, int64_t scores_stride, const float* grad_weight, int64_t weights, const void* dscores,
+               int64_t dscores_stride, const void* workspace, int64_t workspace_bytes, int64_t needs)
+{
+    const int64_t size = rec_type_size(d->type);
+    REC_REFUSE(scores_stride < d->n_items || scores_stride > INT32_MAX, "the scores' row stride is smaller than n_items, or beyond 2^31-1");
+    REC_REFUSE(weights > 0 && d->rows > 0 && !grad_weight != !dscores, "grad_weight and dscores come together");   // an empty array may be null
+    if (dscores) {
+        REC_REFUSE(dscores_stride < d->n_items || dscores_stride > INT32_MAX, "the gradient's row stride is smaller than n_items, or beyond 2^31-1");
+        const bool in_place = dscores == scores && dscores_stride == scores_stride;
+        REC_REFUSE(!in_place && rec_overlap(RowsOf{scores, d->rows, scores_stride * size, d->n_items * size}, RowsOf{dscores, d->rows, dscores_stride * size, d->n_items * size}), "dscores overlaps the scores");
+    }
+    REC_REFUSE(workspace_bytes < needs, "the workspace is too small");
+    REC_REFUSE(needs > 0 && (!workspace || !rec_aligned(workspace, 16)), "the workspace is null or not aligned to 16 bytes");
+    return rec_check_device(d->device);
+}
+
+void fill(LossArgs& a, const rec_loss_desc* d, const void* scores, int64_t scores_stride, const int32_t* item, const float* ref_logp, const float* grad_weight,
+          float* loss, float* logp, void* dscores, int64_t dscores_stride, void* workspace)
+{
+    a.scores = scores; a.scores_stride = scores_stride; a.item = item; a.ref_logp = ref_logp; a.grad_weight = grad_weight;
+    a.loss = loss; a.logp = logp; a.dscores = dscores; a.dscores_stride = dscores_stride;
+    a.rows = d->rows; a.n_items = d->n_items; a.scale = d->scale; a.scale2 = (float)((double)d->scale * 1.4426950408889634);
+    a.scale_rest = (double)d->scale - (double)a.scale2 * 0.6931471805599453;
+    a.zero_rest = d->zero_rest; a.splits = splits_of(d);
+    char* ws = (char*)workspace;
+    a.part = (float4*)ws;
+    a.stat = (float2*)(ws + d->rows * a.splits * 16);
+    a.coef = (float*)(ws + d->rows * a.splits * 16 + round16(d->rows * 8));
+}
+
+#define LOSS_DISPATCH(CALL)                                                                         \
+    if (d->type == REC_TYPE_F32) { CALL(float); }                                                   \
+    else if (d->type == REC_TYPE_F16) { CALL(_Float16); }                                           \
+    else { CALL(__bf16); }
+
+}  // namespace
+
+extern "C" int64_t rec_preference_loss_workspace(const rec_loss_desc* d, int32_t n_pairs)
+{
+    if (check_desc(d)) return -1;
+    if (n_pairs < 0) { rec_set_error("n_pairs must be in 0..2^22-1"); return -1; }
+    return workspace_of(d);
+}
+
+extern "C" int rec_preference_loss(const rec_loss_desc* d, const void* scores, int64_t scores_stride, const int32_t* item,
+                                   const int64_t* seq_off, int32_t n_pairs, const float* ref_logp, float beta, float smoothing,
+                                   const float* grad_weight, float* loss, float* margin, float* logp, void* dscores, int64_t dscores_stride,
+                                   void* workspace, int64_t workspace_bytes, void* stream)
+{
+    return rec_guarded([&]() -> int {
+        if (int rc = check_desc(d)) return rc;
+        REC_REFUSE(n_pairs < 0 || n_pairs > (1 << 22) - 1, "n_pairs must be in 0..2^22-1");
+        REC_REFUSE(!seq_off || (d->rows > 0 && (!scores || !item || !logp)) || (n_pairs > 0 && (!loss || !margin)), "null argument");
+        REC_REFUSE(!isfinite(beta), "beta must be finite");
+        REC_REFUSE(!(smoothing >= 0.0f && smoothing <= 1.0f), "smoothing must be in 0..1");
+        if (int rc = check_call(d, scores, scores_stride, grad_weight, n_pairs, dscores, dscores_stride, workspace, workspace_bytes, workspace_of(d))) return rc;
+        LossArgs a = {};
+        fill(a, d, scores, scores_stride, item, ref_logp, grad_weight, loss, logp, dscores, dscores_stride, workspace);
+        a.off = seq_off; a.n_seq = 2 * n_pairs; a.margin = margin; a.beta = beta; a.smoothing = smoothing;
+        DeviceScope scope;
+        HIP_TRY(scope.enter(d->device));
+        hipStream_t st = (hipStream_t)stream;
+        const unsigned blocks = (unsigned)(d->rows * a.splits);
+#define CALL(T)                                                                                     \
+        if (blocks) row_statistics_kernel<T><<<blocks, kThreads, 0, st>>>(a);                       \
+        if (n_pairs) preference_kernel<T><<<(unsigned)n_pairs, 256, 0, st>>>(a);                    \
+        if (blocks && dscores) gradient_kernel<T><<<blocks, kThreads, 0, st>>>(a)
+        LOSS_DISPATCH(CALL)
+#undef CALL
+        if (d->zero_rest && !dscores && d->rows > 0) rest_kernel<<<(unsigned)((d->rows + 255) / 256), 256, 0, st>>>(a);
+        HIP_TRY(hipGetLastError());
+        return 0;
+    });
+}
+
+extern "C" int64_t rec_policy_loss_workspace(const rec_loss_desc* d)
+{
+    if (check_desc(d)) return -1;
+    return workspace_of(d);
+}
+
+extern "C" int rec_policy_loss(const rec_loss_desc* d, const void* scores, int64_t scores_stride, const int32_t* item,
+                               const float* old_logp, const float* advantage, const float* ref_logp, float clip_low, float clip_high,
+                               float kl_coef, const float* grad_weight, float* loss, float* kl, float* logp, void* dscores,
+                               int64_t dscores_stride, void* workspace, int64_t workspace_bytes, void* stream)
+{
+    return rec_guarded([&]() -> int {
+        if (int rc = check_desc(d)) return rc;
+        REC_REFUSE(d->rows > 0 && (!scores || !item || !old_logp || !advantage || !loss || !logp), "null argument");
+        REC_REFUSE(!(clip_low >= 0.0f && clip_low <= 1.0f) || !(clip_high >= 0.0f) || !isfinite(clip_high), "clip_low must be in 0..1 and clip_high at least 0");
+        REC_REFUSE(!isfinite(kl_coef) || (!ref_logp && kl_coef != 0.0f), "kl_coef must be finite, and 0 without ref_logp");
+        if (int rc = check_call(d, scores, scores_stride, grad_weight, d->rows, dscores, dscores_stride, workspace, workspace_bytes, workspace_of(d))) return rc;
+        LossArgs a = {};
+        fill(a, d, scores, scores_stride, item, ref_logp, grad_weight, loss, logp, dscores, dscores_stride, workspace);
+        a.old_logp = old_logp; a.advantage = advantage; a.kl = kl;
+        a.clip_low = clip_low; a.clip_high = clip_high; a.kl_coef = kl_coef;
+        if (d->rows == 0) return 0;
+        DeviceScope scope;
+        HIP_TRY(scope.enter(d->device));
+        hipStream_t st = (hipStream_t)stream;
+        const unsigned blocks = (unsigned)(d->rows * a.splits);
+#define CALL(T)                                                                                     \
+        row_statistics_kernel<T><<<blocks, kThreads, 0, st>>>(a);                                   \
+        policy_kernel<T><<<(unsigned)((d->rows + 255) / 256), 256, 0, st>>>(a);                     \
+        if (dscores) gradient_kernel<T><<<blocks, kThreads, 0, st>>>(a)
+        LOSS_DISPATCH(CALL)
+#undef CALL
+        HIP_TRY(hipGetLastError());
+        return 0;
+    });
+}

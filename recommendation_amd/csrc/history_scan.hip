@@ -1,0 +1,783 @@
+// Selective state space scan over packed histories: y, its gradient, and the form for single clicks.
+//
+//   delta = softplus(raw + bias)    h_t[n] = exp(delta_t A[n]) h_{t-1}[n] + delta_t u_t B_t[n]    y_t = (sum_n C_t[n] h_t[n] + D u_t) silu(z_t)
+//
+// per channel; h starts at each history's initial state.  A lane holds four states of one channel, LN neighbouring lanes all of
+// them, so a block of 256 lanes walks 256 / LN channels of one group through time; what a step needs per channel (delta and
+// delta * u) and per group (B, C) is staged in LDS 16 rows at a time, in f32.
+//
+// The packed rows are cut into chunks that ignore where histories begin, so ragged lengths leave no block idle.  A history that
+// crosses from one chunk into the next hands its state over: the first pass computes what each chunk adds on its own
+// (only from the last history's beginning on, and only if it goes on), the second links the chunks of each history, the third
+// walks again from the linked states and writes y.  With one chunk the first two are not launched.
+#include "operators.h"
+
+namespace {
+
+constexpr int TT = REC_SCAN_CHECKPOINT;   // rows staged at a time
+
+struct ScanArgs {
+    const void *u, *delta, *z, *B, *C, *dy;
+    const float *A, *D, *delta_bias, *initial, *dfinal, *checkpoints_in;
+    const int64_t* off;
+    void *y, *du, *ddelta, *dz, *dB, *dC;
+    float *final_state, *checkpoints, *dinitial;
+    float *link, *span;          // [chunks + 1][channels][states] state handed into a chunk (backward: gradient handed out of it), [chunks][channels] sum of delta
+    float *part_bc;              // backward: [channel tiles of a group][rows][groups][2][states]
+    float *part_a;               // backward: [chunks][channels * states + 2 * channels]: dA, dD, ddelta_bias
+    int64_t u_stride, delta_stride, z_stride, B_stride, C_stride, y_stride, dy_stride;
+    int64_t rows;
+    int n_seq, channels, groups, per, states, chunk, chunks, tiles, tiles_per_group, softplus, zero_rest;
+};
+
+__device__ __forceinline__ float softplus_f32(float v) { return v > 20.0f ? v : log1pf(fast_exp(v)); }   // beyond 20, log(1 + e^v) - v < 2^-28 v
+
+// the block's place: a chunk of rows, a run of channels of one group
+template <int LN> struct Place {
+    static constexpr int CH = 256 / LN;
+    int64_t r0, r1;
+    int chunk, g, part, ch0, nch, ch, lane_n, d;
+    bool on;
+    __device__ __forceinline__ Place(const ScanArgs& a)
+    {
+        const int tile = blockIdx.x % a.tiles;
+        chunk = blockIdx.x / a.tiles;
+        r0 = (int64_t)chunk * a.chunk;
+        r1 = r0 + a.chunk < a.rows ? r0 + a.chunk : a.rows;
+        g = tile / a.tiles_per_group;
+        part = tile % a.tiles_per_group;
+        ch0 = g * a.per + part * CH;
+        nch = min(CH, (g + 1) * a.per - ch0);
+        ch = threadIdx.x / LN;
+        lane_n = threadIdx.x % LN * 4;
+        on = ch < nch;
+        d = ch0 + (on ? ch : 0);
+    }
+};
+
+// four of a channel's states, of an f32 array [...][channels][states]
+__device__ __forceinline__ void load_states(const float* __restrict__ p, int64_t lead, const ScanArgs& a, int d, int n0, bool on, float (&h)[4])
+{
+#pragma unroll
+    for (int e = 0; e < 4; e++) h[e] = on && p && n0 + e < a.states ? p[(lead * a.channels + d) * a.states + n0 + e] : 0.0f;
+}
+__device__ __forceinline__ void store_states(float* __restrict__ p, int64_t lead, const ScanArgs& a, int d, int n0, bool on, const float (&h)[4])
+{
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (on && n0 + e < a.states) p[(lead * a.channels + d) * a.states + n0 + e] = h[e];
+}
+
+template <class T>
+__device__ __forceinline__ float delta_of(const ScanArgs& a, int64_t row, int d, float& raw)
+{
+    raw = to_f32(((const T*)a.delta)[row * a.delta_stride + d]) + (a.delta_bias ? a.delta_bias[d] : 0.0f);
+    return a.softplus ? softplus_f32(raw) : raw;
+}
+
+// B or C of the tile's rows, zero where the row is not one of [lo, hi)
+template <class T, int NP>
+__device__ __forceinline__ void stage_group(const void* p, int64_t stride, const ScanArgs& a, int g, int64_t t0, int64_t lo, int64_t hi, float (&s)[TT][NP])
+{
+    for (int i = threadIdx.x; i < TT * NP; i += 256) {
+        const int r = i / NP, n = i % NP;
+        const int64_t row = t0 + r;
+        s[r][n] = n < a.states && row >= lo && row < hi ? to_f32(((const T*)p)[row * stride + (int64_t)g * a.states + n]) : 0.0f;
+    }
+}
+
+// first pass: the state a chunk's last history has at the chunk's end, for a state of zero in front of the chunk
+template <class T, int LN>
+__global__ __launch_bounds__(256) void scan_local_kernel(ScanArgs a)
+{
+    using P = Place<LN>;
+    constexpr int CH = P::CH, NP = 4 * LN;
+    __shared__ float2 sd[TT][CH];
+    __shared__ float sB[TT][NP];
+    const P p(a);
+    if (p.chunk + 1 >= a.chunks) return;
+    const int s = sequence_of(a.off, a.n_seq, p.r1 - 1);
+    if (s < 0 || s >= a.n_seq || a.off[s + 1] <= p.r1) return;
+    const int64_t begin = a.off[s];
+    const int64_t from = begin > p.r0 ? begin : p.r0;
+    float A2[4], h[4], span = 0.0f;
+    load_states(a.A, 0, a, p.d, p.lane_n, p.on, A2);
+#pragma unroll
+    for (int e = 0; e < 4; e++) A2[e] *= REC_LOG2E;
+    load_states(begin >= p.r0 ? a.initial : nullptr, s, a, p.d, p.lane_n, p.on, h);
+    for (int64_t t0 = from; t0 < p.r1; t0 += TT) {
+        const int nt = (int)(p.r1 - t0 < TT ? p.r1 - t0 : TT);
+        __syncthreads();
+        for (int i = threadIdx.x; i < TT * CH; i += 256) {
+            const int r = i / CH, c = i % CH;
+            float2 v = make_float2(0.0f, 0.0f);
+            if (r < nt && c < p.nch) {
+                float raw;
+                v.x = delta_of<T>(a, t0 + r, p.ch0 + c, raw);
+                v.y = v.x * to_f32(((const T*)a.u)[(t0 + r) * a.u_stride + p.ch0 + c]);
+            }
+            sd[r][c] = v;
+        }
+        stage_group<T, NP>(a.B, a.B_stride, a, p.g, t0, t0, t0 + nt, sB);
+        __syncthreads();
+        for (int r = 0; r < nt; r++) {
+            const float2 v = sd[r][p.ch];
+            span += v.x;
+#pragma unroll
+            for (int e = 0; e < 4; e++) h[e] = fmaf(fast_exp2(v.x * A2[e]), h[e], v.y * sB[r][p.lane_n + e]);
+        }
+    }
+    store_states(a.link, p.chunk + 1, a, p.d, p.lane_n, p.on, h);
+    if (p.on && p.lane_n == 0) a.span[(int64_t)p.chunk * a.channels + p.d] = span;
+}
+
+// second pass: along each history that crosses chunks, the state handed into chunk c becomes exp(A span) of what was handed
+// into c - 1, plus what c - 1 added.  A thread per channel and state; the blocks of a history's first crossing walk it.
+__global__ __launch_bounds__(256) void scan_link_kernel(ScanArgs a, int blocks)
+{
+    int c = blockIdx.x / blocks + 1;
+    const int64_t row = (int64_t)c * a.chunk;
+    const int s = sequence_of(a.off, a.n_seq, row);
+    if (s < 0 || s >= a.n_seq) return;
+    const int64_t begin = a.off[s], end = a.off[s + 1];
+    if (begin >= row || begin < row - a.chunk) return;
+    const int64_t i = (int64_t)(blockIdx.x % blocks) * 256 + threadIdx.x, n = (int64_t)a.channels * a.states;
+    if (i >= n) return;
+    const float A2 = a.A[i] * REC_LOG2E;
+    const int d = (int)(i / a.states);
+    float h = a.link[c * n + i];
+    for (; c + 1 < a.chunks && end > (int64_t)(c + 1) * a.chunk; c++) {
+        h = fmaf(fast_exp2(A2 * a.span[(int64_t)c * a.channels + d]), h, a.link[(c + 1) * n + i]);
+        a.link[(c + 1) * n + i] = h;
+    }
+}
+
+// third pass
+template <class T, int LN>
+__global__ __launch_bounds__(256) void scan_forward_kernel(ScanArgs a)
+{
+    using P = Place<LN>;
+    constexpr int CH = P::CH, NP = 4 * LN;
+    __shared__ float2 sd[TT][CH];
+    __shared__ float sB[TT][NP], sC[TT][NP], sy[TT][CH];
+    const P p(a);
+    const int64_t lo = a.off[0], hi = a.off[a.n_seq];
+    SeqCursor c;
+    c.begin(a.off, a.n_seq, p.r0);
+    float A2[4], h[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    load_states(a.A, 0, a, p.d, p.lane_n, p.on, A2);
+#pragma unroll
+    for (int e = 0; e < 4; e++) A2[e] *= REC_LOG2E;
+    if (c.inside(a.n_seq)) {
+        if (a.off[c.s] >= p.r0) load_states(a.initial, c.s, a, p.d, p.lane_n, p.on, h);
+        else if (p.chunk > 0) load_states(a.link, p.chunk, a, p.d, p.lane_n, p.on, h);
+    }
+    for (int64_t t0 = p.r0; t0 < p.r1; t0 += TT) {
+        const int nt = (int)(p.r1 - t0 < TT ? p.r1 - t0 : TT);
+        for (int i = threadIdx.x; i < TT * CH; i += 256) {
+            const int r = i / CH, ch = i % CH;
+            float2 v = make_float2(0.0f, 0.0f);
+            if (r < nt && ch < p.nch && t0 + r >= lo && t0 + r < hi) {   // a row of no history moves nothing
+                float raw;
+                v.x = delta_of<T>(a, t0 + r, p.ch0 + ch, raw);
+                v.y = v.x * to_f32(((const T*)a.u)[(t0 + r) * a.u_stride + p.ch0 + ch]);
+            }
+            sd[r][ch] = v;
+        }
+        const int64_t blo = lo > t0 ? lo : t0, bhi = hi < t0 + nt ? hi : t0 + nt;
+        stage_group<T, NP>(a.B, a.B_stride, a, p.g, t0, blo, bhi, sB);
+        stage_group<T, NP>(a.C, a.C_stride, a, p.g, t0, blo, bhi, sC);
+        __syncthreads();
+        if (a.checkpoints) store_states(a.checkpoints, t0 / TT, a, p.d, p.lane_n, p.on, h);
+        for (int r = 0; r < nt; r++) {
+            const int64_t row = t0 + r;
+            if (row >= c.next) {
+                c.advance(a.off, a.n_seq, row);
+                load_states(c.inside(a.n_seq) ? a.initial : nullptr, c.s, a, p.d, p.lane_n, p.on, h);
+            }
+            const float2 v = sd[r][p.ch];
+            float y = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                h[e] = fmaf(fast_exp2(v.x * A2[e]), h[e], v.y * sB[r][p.lane_n + e]);
+                y = fmaf(h[e], sC[r][p.lane_n + e], y);
+            }
+            y = group_sum_dpp<LN>(y);
+            if (p.lane_n == 0) sy[r][p.ch] = y;
+            if (a.final_state && row + 1 == c.next && c.inside(a.n_seq)) store_states(a.final_state, c.s, a, p.d, p.lane_n, p.on, h);
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < TT * CH; i += 256) {
+            const int r = i / CH, ch = i % CH, d = p.ch0 + ch;
+            const int64_t row = t0 + r;
+            if (r >= nt || ch >= p.nch) continue;
+            T* y = (T*)a.y + row * a.y_stride + d;
+            if (row < lo || row >= hi) {
+                if (a.zero_rest) *y = from_f32<T>(0.0f);
+                continue;
+            }
+            float v = sy[r][ch];
+            if (a.D) v = fmaf(a.D[d], to_f32(((const T*)a.u)[row * a.u_stride + d]), v);
+            if (a.z) v *= silu_f32(to_f32(((const T*)a.z)[row * a.z_stride + d]));
+            *y = from_f32<T>(v);
+        }
+    }
+}
+
+// empty histories: their state passes through (forward: initial -> final_state, backward: dfinal -> dinitial)
+__global__ __launch_bounds__(256) void scan_empty_kernel(ScanArgs a, const float* from, float* to)
+{
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = (int64_t)a.channels * a.states;
+    if (i >= n * a.n_seq) return;
+    const int64_t s = i / n;
+    if (a.off[s + 1] <= a.off[s]) to[i] = from ? from[i] : 0.0f;
+}
+
+// ---- gradient.  With G_t = dL/dh_t:   G_t = C_t dys_t + exp(delta_{t+1} A) G_{t+1}   (dfinal in place of the second term at a
+// history's last row), dys = dy silu(z).  The chunks are linked as above, from the back.
+
+// first pass: what a chunk hands to the rows in front of it, exp(delta A) G at its first row, for nothing handed in from behind
+template <class T, int LN>
+__global__ __launch_bounds__(256) void scan_local_backward_kernel(ScanArgs a)
+{
+    using P = Place<LN>;
+    constexpr int CH = P::CH, NP = 4 * LN;
+    __shared__ float2 sd[TT][CH];
+    __shared__ float sC[TT][NP];
+    const P p(a);
+    if (p.chunk == 0) return;
+    const int s = sequence_of(a.off, a.n_seq, p.r0);
+    if (s < 0 || s >= a.n_seq || a.off[s] >= p.r0) return;
+    const int64_t end = a.off[s + 1];
+    const int64_t to = end < p.r1 ? end : p.r1;
+    float A2[4], g[4], span = 0.0f;
+    load_states(a.A, 0, a, p.d, p.lane_n, p.on, A2);
+#pragma unroll
+    for (int e = 0; e < 4; e++) A2[e] *= REC_LOG2E;
+    load_states(end <= p.r1 ? a.dfinal : nullptr, s, a, p.d, p.lane_n, p.on, g);
+    for (int64_t t1 = to; t1 > p.r0; t1 -= TT) {
+        const int64_t t0 = t1 - TT > p.r0 ? t1 - TT : p.r0;
+        const int nt = (int)(t1 - t0);
+        __syncthreads();
+        for (int i = threadIdx.x; i < TT * CH; i += 256) {
+            const int r = i / CH, c = i % CH;
+            float2 v = make_float2(0.0f, 0.0f);
+            if (r < nt && c < p.nch) {
+                float raw;
+                v.x = delta_of<T>(a, t0 + r, p.ch0 + c, raw);
+                v.y = to_f32(((const T*)a.dy)[(t0 + r) * a.dy_stride + p.ch0 + c]);
+                if (a.z) v.y *= silu_f32(to_f32(((const T*)a.z)[(t0 + r) * a.z_stride + p.ch0 + c]));
+            }
+            sd[r][c] = v;
+        }
+        stage_group<T, NP>(a.C, a.C_stride, a, p.g, t0, t0, t0 + nt, sC);
+        __syncthreads();
+        for (int r = nt - 1; r >= 0; r--) {
+            const float2 v = sd[r][p.ch];
+            span += v.x;
+#pragma unroll
+            for (int e = 0; e < 4; e++) g[e] = fast_exp2(v.x * A2[e]) * fmaf(sC[r][p.lane_n + e], v.y, g[e]);
+        }
+    }
+    store_states(a.link, p.chunk, a, p.d, p.lane_n, p.on, g);
+    if (p.on && p.lane_n == 0) a.span[(int64_t)p.chunk * a.channels + p.d] = span;
+}
+
+// second pass: the blocks of a history's last crossing walk it towards its first
+__global__ __launch_bounds__(256) void scan_link_backward_kernel(ScanArgs a, int blocks)
+{
+    int c = blockIdx.x / blocks + 1;
+    const int64_t row = (int64_t)c * a.chunk;
+    const int s = sequence_of(a.off, a.n_seq, row);
+    if (s < 0 || s >= a.n_seq) return;
+    const int64_t begin = a.off[s], end = a.off[s + 1];
+    if (begin >= row || (end > row + a.chunk && c + 1 < a.chunks)) return;
+    const int64_t i = (int64_t)(blockIdx.x % blocks) * 256 + threadIdx.x, n = (int64_t)a.channels * a.states;
+    if (i >= n) return;
+    const float A2 = a.A[i] * REC_LOG2E;
+    const int d = (int)(i / a.states);
+    float g = a.link[c * n + i];
+    for (c--; c >= 1 && begin < (int64_t)c * a.chunk; c--) {
+        g = fmaf(fast_exp2(A2 * a.span[(int64_t)c * a.channels + d]), g, a.link[c * n + i]);
+        a.link[c * n + i] = g;
+    }
+}
+
+// third pass: per 16 rows, the states again from the checkpoint in front of them, then the gradient backwards
+template <class T, int LN>
+__global__ __launch_bounds__(256) void scan_backward_kernel(ScanArgs a)
+{
+    using P = Place<LN>;
+    constexpr int CH = P::CH, NP = 4 * LN, PT = TT * CH / 256;   // PT: (row, channel) pairs per thread in the element-wise parts
+    __shared__ float2 sd[TT][CH];                  // delta, delta * u
+    __shared__ float sg[TT][CH];                   // dys
+    __shared__ float sB[TT][NP], sC[TT][NP];
+    __shared__ float s_in[TT][CH], s_gB[TT][CH], s_qA[TT][CH];
+    __shared__ float s_bc[4][TT][2][NP];
+    __shared__ unsigned starts_s;
+    const P p(a);
+    const int64_t lo = a.off[0], hi = a.off[a.n_seq];
+    float A[4], A2[4], G[4] = {0.0f, 0.0f, 0.0f, 0.0f}, dA[4] = {0.0f, 0.0f, 0.0f, 0.0f}, dD = 0.0f, dbias = 0.0f;
+    load_states(a.A, 0, a, p.d, p.lane_n, p.on, A);
+#pragma unroll
+    for (int e = 0; e < 4; e++) A2[e] = A[e] * REC_LOG2E;
+    int s = sequence_of(a.off, a.n_seq, p.r1 - 1);   // of the row at hand, walking backwards
+    if (s >= 0 && s < a.n_seq && a.off[s + 1] > p.r1 && p.chunk + 1 < a.chunks) load_states(a.link, p.chunk + 1, a, p.d, p.lane_n, p.on, G);
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    for (int64_t t0 = (p.r1 - 1) / TT * TT; t0 >= p.r0; t0 -= TT) {
+        const int nt = (int)(p.r1 - t0 < TT ? p.r1 - t0 : TT);
+        __syncthreads();
+        if (threadIdx.x == 0) {   // which of the tile's rows begin a history
+            unsigned m = 0;
+            SeqCursor c;
+            c.begin(a.off, a.n_seq, t0);
+            if (c.inside(a.n_seq) && a.off[c.s] == t0) m = 1;
+            for (int r = 1; r < nt; r++)
+                if (t0 + r >= c.next) { c.advance(a.off, a.n_seq, t0 + r); if (c.inside(a.n_seq)) m |= 1u << r; }
+            starts_s = m;
+        }
+        float raw[PT], u[PT], zz[PT], gy[PT];
+#pragma unroll
+        for (int k = 0; k < PT; k++) {
+            const int i = threadIdx.x + 256 * k, r = i / CH, ch = i % CH, d = p.ch0 + ch;
+            const int64_t row = t0 + r;
+            float2 v = make_float2(0.0f, 0.0f);
+            raw[k] = u[k] = zz[k] = gy[k] = 0.0f;
+            float ys = 0.0f;
+            if (r < nt && ch < p.nch && row >= lo && row < hi) {
+                v.x = delta_of<T>(a, row, d, raw[k]);
+                u[k] = to_f32(((const T*)a.u)[row * a.u_stride + d]);
+                v.y = v.x * u[k];
+                gy[k] = to_f32(((const T*)a.dy)[row * a.dy_stride + d]);
+                ys = gy[k];
+                if (a.z) { zz[k] = to_f32(((const T*)a.z)[row * a.z_stride + d]); ys *= silu_f32(zz[k]); }
+            }
+            sd[r][ch] = v;
+            sg[r][ch] = ys;
+        }
+        const int64_t blo = lo > t0 ? lo : t0, bhi = hi < t0 + nt ? hi : t0 + nt;
+        stage_group<T, NP>(a.B, a.B_stride, a, p.g, t0, blo, bhi, sB);
+        stage_group<T, NP>(a.C, a.C_stride, a, p.g, t0, blo, bhi, sC);
+        __syncthreads();
+        const unsigned starts = starts_s;
+        float hb[TT][4], h[4];   // the state in front of each row
+        load_states(a.checkpoints_in, t0 / TT, a, p.d, p.lane_n, p.on, h);
+#pragma unroll
+        for (int r = 0; r < TT; r++) {
+            if ((starts >> r) & 1) load_states(a.initial, sequence_of(a.off, a.n_seq, t0 + r), a, p.d, p.lane_n, p.on, h);
+            const float2 v = sd[r][p.ch];
+            float y = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                hb[r][e] = h[e];
+                h[e] = fmaf(fast_exp2(v.x * A2[e]), h[e], v.y * sB[r][p.lane_n + e]);
+                y = fmaf(h[e], sC[r][p.lane_n + e], y);
+            }
+            y = group_sum_dpp<LN>(y);
+            if (p.lane_n == 0) s_in[r][p.ch] = y;
+        }
+#pragma unroll
+        for (int r = TT - 1; r >= 0; r--) {
+            if (r >= nt) continue;
+            const int64_t row = t0 + r;
+            // a row with the next history (or none) behind it is the last of its own: dfinal instead of what came from behind
+            const bool last = row + 1 == hi || (r + 1 < nt && ((starts >> (r + 1)) & 1)) || (r + 1 == nt && s >= 0 && s < a.n_seq && a.off[s + 1] == row + 1);
+            if (last) {
+                s = sequence_of(a.off, a.n_seq, row);
+                load_states(s >= 0 && s < a.n_seq ? a.dfinal : nullptr, s, a, p.d, p.lane_n, p.on, G);
+            }
+            const float2 v = sd[r][p.ch];
+            const float ys = sg[r][p.ch];
+            float gB = 0.0f, qA = 0.0f, vB[4], vC[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float ea = fast_exp2(v.x * A2[e]);
+                const float h1 = fmaf(ea, hb[r][e], v.y * sB[r][p.lane_n + e]);
+                const float g = fmaf(sC[r][p.lane_n + e], ys, G[e]);
+                vB[e] = g * v.y;
+                vC[e] = h1 * ys;
+                gB = fmaf(g, sB[r][p.lane_n + e], gB);
+                G[e] = ea * g;
+                const float q = G[e] * hb[r][e];
+                qA = fmaf(q, A[e], qA);
+                dA[e] = fmaf(q, v.x, dA[e]);
+            }
+            gB = group_sum_dpp<LN>(gB);
+            qA = group_sum_dpp<LN>(qA);
+            if (p.lane_n == 0) { s_gB[r][p.ch] = gB; s_qA[r][p.ch] = qA; }
+#pragma unroll
+            for (int e = 0; e < 4; e++) {   // over the wavefront's channels
+#pragma unroll
+                for (int m = LN; m < 64; m <<= 1) { vB[e] += __shfl_xor(vB[e], m, 64); vC[e] += __shfl_xor(vC[e], m, 64); }
+                if (lane < LN) { s_bc[wave][r][0][p.lane_n + e] = vB[e]; s_bc[wave][r][1][p.lane_n + e] = vC[e]; }
+            }
+            if ((starts >> r) & 1) {
+                if (a.dinitial) {
+                    const int si = sequence_of(a.off, a.n_seq, row);
+                    if (si >= 0 && si < a.n_seq) store_states(a.dinitial, si, a, p.d, p.lane_n, p.on, G);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) G[e] = 0.0f;
+            }
+        }
+        s = sequence_of(a.off, a.n_seq, t0 - 1);
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < PT; k++) {
+            const int i = threadIdx.x + 256 * k, r = i / CH, ch = i % CH, d = p.ch0 + ch;
+            const int64_t row = t0 + r, at = row * a.channels + d;
+            if (r >= nt || ch >= p.nch) continue;
+            if (row < lo || row >= hi) {
+                if (a.zero_rest) {
+                    ((T*)a.du)[at] = ((T*)a.ddelta)[at] = from_f32<T>(0.0f);
+                    if (a.z) ((T*)a.dz)[at] = from_f32<T>(0.0f);
+                }
+                continue;
+            }
+            const float2 v = sd[r][ch];
+            const float ys = sg[r][ch], gB = s_gB[r][ch], Dd = a.D ? a.D[d] : 0.0f;
+            float dd = fmaf(u[k], gB, s_qA[r][ch]);
+            if (a.softplus) dd *= sigmoid_f32(raw[k]);
+            ((T*)a.du)[at] = from_f32<T>(fmaf(v.x, gB, Dd * ys));
+            ((T*)a.ddelta)[at] = from_f32<T>(dd);
+            if (a.z) ((T*)a.dz)[at] = from_f32<T>(gy[k] * fmaf(Dd, u[k], s_in[r][ch]) * dsilu_f32(zz[k]));
+            dD = fmaf(ys, u[k], dD);
+            dbias += dd;
+        }
+        // dB and dC of the block's channels: the four wavefronts in order
+        for (int i = threadIdx.x; i < TT * 2 * NP; i += 256) {
+            const int r = i / (2 * NP), w = i / NP % 2, n = i % NP;
+            const int64_t row = t0 + r;
+            if (r >= nt || n >= a.states) continue;
+            const float v = (s_bc[0][r][w][n] + s_bc[1][r][w][n]) + (s_bc[2][r][w][n] + s_bc[3][r][w][n]);
+            if (a.tiles_per_group > 1) {
+                a.part_bc[((((int64_t)p.part * a.rows + row) * a.groups + p.g) * 2 + w) * a.states + n] = v;
+            } else if ((row >= lo && row < hi) || a.zero_rest) {
+                ((T*)(w ? a.dC : a.dB))[(row * a.groups + p.g) * a.states + n] = from_f32<T>(v);
+            }
+        }
+    }
+    if (!a.part_a) return;
+    float* part = a.part_a + (int64_t)p.chunk * (a.channels * a.states + 2 * a.channels);
+    store_states(part, 0, a, p.d, p.lane_n, p.on, dA);
+    // a thread's pairs are of one channel: the threads of a channel in order
+    __syncthreads();
+    float *red_D = &s_in[0][0], *red_b = &s_gB[0][0];   // 16 * CH >= 256 each
+    red_D[threadIdx.x] = dD;
+    red_b[threadIdx.x] = dbias;
+    __syncthreads();
+    if ((int)threadIdx.x < p.nch) {
+        float x = 0.0f, y = 0.0f;
+        for (int k = threadIdx.x; k < 256; k += CH) { x += red_D[k]; y += red_b[k]; }
+        part[a.channels * a.states + p.ch0 + threadIdx.x] = x;
+        part[a.channels * a.states + a.channels + p.ch0 + threadIdx.x] = y;
+    }
+}
+
+// dB and dC where a group's channels are spread over blocks
+template <class T>
+__global__ __launch_bounds__(256) void scan_sum_groups_kernel(ScanArgs a)
+{
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per_row = (int64_t)a.groups * 2 * a.states, n = a.rows * per_row;
+    if (i >= n) return;
+    const int64_t row = i / per_row;
+    if ((row < a.off[0] || row >= a.off[a.n_seq]) && !a.zero_rest) return;
+    float v = 0.0f;
+    for (int k = 0; k < a.tiles_per_group; k++) v += a.part_bc[k * n + i];
+    const int64_t at = (i / (2 * a.states)) * a.states + i % a.states;
+    ((T*)(i / a.states % 2 ? a.dC : a.dB))[at] = from_f32<T>(v);
+}
+
+// ---- single clicks: a block per row and up to 256 / LN of its channels; the state moves through registers once
+template <class T, int LN>
+__global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a, const int32_t* __restrict__ slots, float* __restrict__ state)
+{
+    constexpr int CH = 256 / LN;
+    const int64_t row = blockIdx.x / a.tiles;
+    const int tile = blockIdx.x % a.tiles, g = tile / a.tiles_per_group, ch0 = g * a.per + tile % a.tiles_per_group * CH;
+    const int ch = threadIdx.x / LN, n0 = threadIdx.x % LN * 4, d = ch0 + ch;
+    const int slot = slots[row];
+    bool earlier, later;
+    slot_is_shared(slots, a.rows, row, slot, earlier, later);
+    if (d >= (g + 1) * a.per) return;
+    if (slot < 0 || slot >= a.n_seq) {
+        if (n0 == 0) ((T*)a.y)[row * a.y_stride + d] = from_f32<T>(0.0f);
+        return;
+    }
+    if (earlier) return;
+    float A2[4], h[4];
+    load_states(state, slot, a, d, n0, true, h);
+    load_states(a.A, 0, a, d, n0, true, A2);
+#pragma unroll
+    for (int e = 0; e < 4; e++) A2[e] *= REC_LOG2E;
+    for (int64_t r = row; r < a.rows; r++) {
+        if (r > row) {
+            if (!later) break;
+            if (slots[r] != slot) continue;
+        }
+        float raw, y = 0.0f;
+        const float delta = delta_of<T>(a, r, d, raw), u = to_f32(((const T*)a.u)[r * a.u_stride + d]);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (n0 + e >= a.states) continue;
+            const float b = to_f32(((const T*)a.B)[r * a.B_stride + (int64_t)g * a.states + n0 + e]);
+            const float c = to_f32(((const T*)a.C)[r * a.C_stride + (int64_t)g * a.states + n0 + e]);
+            h[e] = fmaf(fast_exp2(delta * A2[e]), h[e], delta * u * b);
+            y = fmaf(h[e], c, y);
+        }
+        y = group_sum_dpp<LN>(y);
+        if (n0 == 0) {
+            if (a.D) y = fmaf(a.D[d], u, y);
+            if (a.z) y *= silu_f32(to_f32(((const T*)a.z)[r * a.z_stride + d]));
+            ((T*)a.y)[r * a.y_stride + d] = from_f32<T>(y);
+        }
+    }
+    store_states(state, slot, a, d, n0, true, h);
+}
+
+// ---- host
+int check_desc(const rec_scan_desc* d)
+{
+    REC_REFUSE(!d, "null argument");
+    REC_REFUSE(d->type < REC_TYPE_F32 || d->type > REC_TYPE_BF16, "unknown type");
+    REC_REFUSE(d->rows < 0 || d->rows > INT32_MAX, "rows must be in 0..2^31-1");
+    REC_REFUSE(d->n_seq < 0, "n_seq must not be negative");
+    REC_REFUSE(d->channels < 1 || d->channels > 1 << 20, "channels must be in 1..2^20");
+    REC_REFUSE(d->groups < 1 || d->channels % d->groups, "groups must divide the channels");
+    REC_REFUSE(d->states < 1 || d->states > 64, "states must be in 1..64");
+    return 0;
+}
+
+int check_inputs(const rec_scan_desc* d, const rec_scan_inputs* in)
+{
+    REC_REFUSE(!in || !in->A || (d->rows > 0 && (!in->u || !in->delta || !in->B || !in->C)), "null argument");
+    const int64_t n = (int64_t)d->groups * d->states;
+    REC_REFUSE(in->u_stride < d->channels || in->delta_stride < d->channels || (in->z && in->z_stride < d->channels), "a row stride is smaller than the channels");
+    REC_REFUSE(in->B_stride < n || in->C_stride < n, "a row stride is smaller than groups x states");
+    REC_REFUSE(in->u_stride > INT32_MAX || in->delta_stride > INT32_MAX || in->z_stride > INT32_MAX || in->B_stride > INT32_MAX || in->C_stride > INT32_MAX,
+               "a row stride is beyond 2^31-1");
+    return 0;
+}
+
+bool overlaps_inputs(const rec_scan_desc* d, const rec_scan_inputs* in, const RowsOf& out)
+{
+    const int64_t e = rec_type_size(d->type), w = d->channels * e, n = (int64_t)d->groups * d->states * e;
+    const RowsOf ins[5] = {{in->u, d->rows, in->u_stride * e, w}, {in->delta, d->rows, in->delta_stride * e, w}, {in->z, d->rows, in->z_stride * e, w},
+                           {in->B, d->rows, in->B_stride * e, n}, {in->C, d->rows, in->C_stride * e, n}};
+    for (const RowsOf& i : ins)
+        if (rec_overlap(i, out)) return true;
+    return false;
+}
+
+RowsOf channel_rows(const rec_scan_desc* d, const void* p, int64_t stride)
+{
+    const int64_t e = rec_type_size(d->type);
+    return {p, d->rows, stride * e, d->channels * e};
+}
+
+int lanes_of(int states) { return states <= 4 ? 1 : states <= 8 ? 2 : states <= 16 ? 4 : states <= 32 ? 8 : 16; }
+
+// How the rows are cut.  A walk of one row takes a block about 0.1 us whatever else runs, a chunk more costs its first pass (two
+// thirds of the third) and a state handed over; so chunks are as long as they can be while the launch still has about
+// eight blocks per compute unit, between 32 and 512 rows.
+struct Cut { int tiles_per_group, tiles, chunk, chunks; };
+Cut cut_of(const rec_scan_desc* d)
+{
+    Cut c;
+    const int ch = 256 / lanes_of(d->states), per = d->channels / d->groups;
+    c.tiles_per_group = (per + ch - 1) / ch;
+    c.tiles = c.tiles_per_group * d->groups;
+    int64_t rows = d->rows * c.tiles / 2048 / TT * TT;
+    if (rows < 32) rows = 32;
+    if (rows > 512) rows = 512;
+    c.chunk = (int)rows;
+    c.chunks = (int)((d->rows + rows - 1) / rows);
+    return c;
+}
+
+int64_t link_bytes(const rec_scan_desc* d, const Cut& c)
+{
+    return c.chunks > 1 ? ((int64_t)(c.chunks + 1) * d->channels * d->states + (int64_t)c.chunks * d->channels) * 4 : 0;
+}
+
+void fill(ScanArgs& a, const rec_scan_desc* d, const rec_scan_inputs* in, const Cut& c)
+{
+    a.u = in->u; a.delta = in->delta; a.z = in->z; a.B = in->B; a.C = in->C; a.A = in->A; a.D = in->D; a.delta_bias = in->delta_bias; a.initial = in->initial;
+    a.u_stride = in->u_stride; a.delta_stride = in->delta_stride; a.z_stride = in->z_stride; a.B_stride = in->B_stride; a.C_stride = in->C_stride;
+    a.rows = d->rows; a.n_seq = d->n_seq; a.channels = d->channels; a.groups = d->groups; a.per = d->channels / d->groups; a.states = d->states;
+    a.chunk = c.chunk; a.chunks = c.chunks; a.tiles = c.tiles; a.tiles_per_group = c.tiles_per_group; a.softplus = d->softplus; a.zero_rest = d->zero_rest;
+}
+
+int check_blocks(int64_t blocks)
+{
+    REC_REFUSE(blocks > (1ll << 24) - 1, "too many rows, channels or sequences for one call");   // a launch holds fewer than 2^32 threads
+    return 0;
+}
+
+int check_workspace(const void* p, int64_t has, int64_t needs)
+{
+    REC_REFUSE(has < needs, "the workspace is too small");
+    REC_REFUSE(needs > 0 && (!p || !rec_aligned(p, 16)), "the workspace is null or not aligned to 16 bytes");
+    return 0;
+}
+
+#define SCAN_LANES(T, CALL)                                                                                 \
+    switch (lanes_of(d->states)) {                                                                          \
+    case 1: CALL(T, 1); break; case 2: CALL(T, 2); break; case 4: CALL(T, 4); break;                        \
+    case 8: CALL(T, 8); break; default: CALL(T, 16); break;                                                 \
+    }
+#define SCAN_DISPATCH(CALL)                                                                                 \
+    if (d->type == REC_TYPE_F32) { SCAN_LANES(float, CALL) }                                                \
+    else if (d->type == REC_TYPE_F16) { SCAN_LANES(_Float16, CALL) }                                        \
+    else { SCAN_LANES(__bf16, CALL) }
+
+}  // namespace
+
+extern "C" int64_t rec_history_scan_workspace(const rec_scan_desc* d)
+{
+    if (check_desc(d)) return -1;
+    return link_bytes(d, cut_of(d));
+}
+
+extern "C" int rec_history_scan(const rec_scan_desc* d, const rec_scan_inputs* in, const int64_t* seq_off, void* y, int64_t y_stride,
+                                float* final_state, float* checkpoints, void* workspace, int64_t workspace_bytes, void* stream)
+{
+    return rec_guarded([&]() -> int {
+        if (int rc = check_desc(d)) return rc;
+        if (int rc = check_inputs(d, in)) return rc;
+        REC_REFUSE(!seq_off || (d->rows > 0 && !y), "null argument");
+        REC_REFUSE(y_stride < d->channels || y_stride > INT32_MAX, "a row stride is smaller than the channels, or beyond 2^31-1");
+        REC_REFUSE(overlaps_inputs(d, in, channel_rows(d, y, y_stride)), "the output overlaps an input");
+        const Cut c = cut_of(d);
+        if (int rc = check_workspace(workspace, workspace_bytes, link_bytes(d, c))) return rc;
+        if (int rc = rec_check_device(d->device)) return rc;
+        const int64_t blocks = (int64_t)c.chunks * c.tiles, n = (int64_t)d->channels * d->states, per_chunk = (n + 255) / 256;
+        if (int rc = check_blocks(blocks > per_chunk * c.chunks ? blocks : per_chunk * c.chunks)) return rc;
+        const int64_t empty_blocks = final_state ? (n * d->n_seq + 255) / 256 : 0;
+        if (int rc = check_blocks(empty_blocks)) return rc;
+        ScanArgs a = {};
+        fill(a, d, in, c);
+        a.off = seq_off; a.y = y; a.y_stride = y_stride; a.final_state = final_state; a.checkpoints = checkpoints;
+        a.link = (float*)workspace;
+        a.span = a.link + (int64_t)(c.chunks + 1) * n;
+        DeviceScope scope;
+        HIP_TRY(scope.enter(d->device));
+        hipStream_t st = (hipStream_t)stream;
+        if (c.chunks > 1) {
+#define CALL(T, LN) scan_local_kernel<T, LN><<<(unsigned)blocks, 256, 0, st>>>(a)
+            SCAN_DISPATCH(CALL)
+#undef CALL
+            scan_link_kernel<<<(unsigned)(per_chunk * (c.chunks - 1)), 256, 0, st>>>(a, (int)per_chunk);
+        }
+        if (blocks > 0) {
+#define CALL(T, LN) scan_forward_kernel<T, LN><<<(unsigned)blocks, 256, 0, st>>>(a)
+            SCAN_DISPATCH(CALL)
+#undef CALL
+        }
+        if (empty_blocks > 0) scan_empty_kernel<<<(unsigned)empty_blocks, 256, 0, st>>>(a, in->initial, final_state);
+        HIP_TRY(hipGetLastError());
+        return 0;
+    });
+}
+
+static int64_t backward_part_a(const rec_scan_desc* d, const Cut& c) { return (int64_t)c.chunks * ((int64_t)d->channels * d->states + 2 * d->channels) * 4; }
+static int64_t backward_part_bc(const rec_scan_desc* d, const Cut& c) { return c.tiles_per_group > 1 ? (int64_t)c.tiles_per_group * d->rows * d->groups * 2 * d->states * 4 : 0; }
+static int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
+
+extern "C" int64_t rec_history_scan_backward_workspace(const rec_scan_desc* d)
+{
+    if (check_desc(d)) return -1;
+    const Cut c = cut_of(d);
+    return round16(link_bytes(d, c)) + round16(backward_part_a(d, c)) + backward_part_bc(d, c);
+}
+
+extern "C" int rec_history_scan_backward(const rec_scan_desc* d, const void* dy, int64_t dy_stride, const rec_scan_inputs* in,
+                                         const int64_t* seq_off, const float* checkpoints, const float* dfinal, const rec_scan_gradients* out,
+                                         void* workspace, int64_t workspace_bytes, void* stream)
+{
+    return rec_guarded([&]() -> int {
+        if (int rc = check_desc(d)) return rc;
+        if (int rc = check_inputs(d, in)) return rc;
+        REC_REFUSE(!seq_off || !out || (d->rows > 0 && (!dy || !checkpoints || !out->du || !out->ddelta || !out->dB || !out->dC || (in->z && !out->dz))), "null argument");
+        REC_REFUSE(dy_stride < d->channels || dy_stride > INT32_MAX, "a row stride is smaller than the channels, or beyond 2^31-1");
+        const int64_t group = (int64_t)rec_type_size(d->type) * d->groups * d->states;
+        const RowsOf outs[5] = {channel_rows(d, out->du, d->channels), channel_rows(d, out->ddelta, d->channels), channel_rows(d, in->z ? out->dz : nullptr, d->channels),
+                                {out->dB, d->rows, group, group}, {out->dC, d->rows, group, group}};
+        for (int k = 0; k < 5; k++) {
+            REC_REFUSE(overlaps_inputs(d, in, outs[k]) || rec_overlap(channel_rows(d, dy, dy_stride), outs[k]), "an output overlaps an input");
+            for (int j = 0; j < k; j++) REC_REFUSE(rec_overlap(outs[j], outs[k]), "two outputs overlap");
+        }
+        if (int rc = check_workspace(workspace, workspace_bytes, rec_history_scan_backward_workspace(d))) return rc;
+        if (int rc = rec_check_device(d->device)) return rc;
+        const Cut c = cut_of(d);
+        const int64_t blocks = (int64_t)c.chunks * c.tiles, n = (int64_t)d->channels * d->states, per_chunk = (n + 255) / 256;
+        if (int rc = check_blocks(blocks > per_chunk * c.chunks ? blocks : per_chunk * c.chunks)) return rc;
+        const int64_t empty_blocks = out->dinitial ? (n * d->n_seq + 255) / 256 : 0;
+        const int64_t sum_blocks = c.tiles_per_group > 1 ? (d->rows * d->groups * 2 * d->states + 255) / 256 : 0;
+        if (int rc = check_blocks(empty_blocks > sum_blocks ? empty_blocks : sum_blocks)) return rc;
+        const bool params = out->dA || out->dD || out->ddelta_bias;
+        ScanArgs a = {};
+        fill(a, d, in, c);
+        a.off = seq_off; a.dy = dy; a.dy_stride = dy_stride; a.checkpoints_in = checkpoints; a.dfinal = dfinal;
+        a.du = out->du; a.ddelta = out->ddelta; a.dz = out->dz; a.dB = out->dB; a.dC = out->dC; a.dinitial = out->dinitial;
+        char* ws = (char*)workspace;
+        a.link = (float*)ws;
+        a.span = a.link + (int64_t)(c.chunks + 1) * n;
+        float* part_a = (float*)(ws + round16(link_bytes(d, c)));
+        a.part_a = params ? part_a : nullptr;
+        a.part_bc = (float*)(ws + round16(link_bytes(d, c)) + round16(backward_part_a(d, c)));
+        DeviceScope scope;
+        HIP_TRY(scope.enter(d->device));
+        hipStream_t st = (hipStream_t)stream;
+        if (c.chunks > 1) {
+#define CALL(T, LN) scan_local_backward_kernel<T, LN><<<(unsigned)blocks, 256, 0, st>>>(a)
+            SCAN_DISPATCH(CALL)
+#undef CALL
+            scan_link_backward_kernel<<<(unsigned)(per_chunk * (c.chunks - 1)), 256, 0, st>>>(a, (int)per_chunk);
+        }
+        if (blocks > 0) {
+#define CALL(T, LN) scan_backward_kernel<T, LN><<<(unsigned)blocks, 256, 0, st>>>(a)
+            SCAN_DISPATCH(CALL)
+#undef CALL
+        }
+        if (sum_blocks > 0) {
+            if (d->type == REC_TYPE_F32) scan_sum_groups_kernel<float><<<(unsigned)sum_blocks, 256, 0, st>>>(a);
+            else if (d->type == REC_TYPE_F16) scan_sum_groups_kernel<_Float16><<<(unsigned)sum_blocks, 256, 0, st>>>(a);
+            else scan_sum_groups_kernel<__bf16><<<(unsigned)sum_blocks, 256, 0, st>>>(a);
+        }
+        if (empty_blocks > 0) scan_empty_kernel<<<(unsigned)empty_blocks, 256, 0, st>>>(a, dfinal, out->dinitial);
+        HIP_TRY(hipGetLastError());
+        if (!params) return 0;
+        return launch_sum_partials(part_a, c.chunks, n + 2 * d->channels, out->dA, n, out->dD, d->channels, out->ddelta_bias, st);
+    });
+}
+
+extern "C" int rec_history_scan_step(const rec_scan_desc* d, const rec_scan_inputs* in, const int32_t* slots, float* state, void* y,
+                                     int64_t y_stride, void* stream)
+{
+    return rec_guarded([&]() -> int {
+        if (int rc = check_desc(d)) return rc;
+        if (int rc = check_inputs(d, in)) return rc;
+        REC_REFUSE(d->rows > 65536, "a step takes at most 65536 rows");
+        REC_REFUSE((d->rows > 0 && (!y || !slots)) || (d->n_seq > 0 && !state), "null argument");
+        REC_REFUSE(y_stride < d->channels || y_stride > INT32_MAX, "a row stride is smaller than the channels, or beyond 2^31-1");
+        const RowsOf yr = channel_rows(d, y, y_stride), pool = {state, 1, INT64_MAX, (int64_t)d->n_seq * d->channels * d->states * 4};
+        REC_REFUSE(overlaps_inputs(d, in, yr) || overlaps_inputs(d, in, pool) || rec_overlap(pool, yr), "the inputs, y and the state must not overlap");
+        if (int rc = rec_check_device(d->device)) return rc;
+        if (d->rows == 0) return 0;
+        Cut c = cut_of(d);
+        c.chunk = 0; c.chunks = 0;
+        ScanArgs a = {};
+        fill(a, d, in, c);
+        a.y = y; a.y_stride = y_stride;
+        const int64_t blocks = d->rows * c.tiles;
+        if (int rc = check_blocks(blocks)) return rc;
+        DeviceScope scope;
+        HIP_TRY(scope.enter(d->device));
+#define CALL(T, LN) scan_step_kernel<T, LN><<<(unsigned)blocks, 256, 0, (hipStream_t)stream>>>(a, slots, state)
+        SCAN_DISPATCH(CALL)
+#undef CALL
+        HIP_TRY(hipGetLastError());
+        return 0;
+    });
+}

@@ -1,0 +1,122 @@
+// What the device operators (history_conv, history_scan, catalog_loss) share.
+#pragma once
+#include "common.h"
+#include <limits.h>
+#include <math.h>
+
+// ---- host side: an entry point works on the caller's device and stream, and nothing is thrown across the C boundary
+struct DeviceScope {
+    int before = -1;
+    bool moved = false;
+    hipError_t enter(int device)
+    {
+        hipError_t rc = hipGetDevice(&before);
+        if (rc == hipSuccess && before != device) { rc = hipSetDevice(device); moved = rc == hipSuccess; }
+        return rc;
+    }
+    ~DeviceScope() { if (moved) (void)hipSetDevice(before); }
+};
+
+#define REC_REFUSE(cond, msg)                       \
+    do {                                            \
+        if (cond) { rec_set_error(msg); return -1; } \
+    } while (0)
+
+template <class F> int rec_guarded(F&& f)
+{
+    try { return f(); } catch (...) { return -3; }   // only the message's own allocation can throw
+}
+
+inline int rec_check_device(int device)
+{
+    int n = 0;
+    if (hipGetDeviceCount(&n) != hipSuccess) n = 0;
+    REC_REFUSE(device < 0 || device >= n, "no such HIP device");
+    return 0;
+}
+
+inline bool rec_overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes)
+{
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return a && b && a_bytes > 0 && b_bytes > 0 && x < y + (uintptr_t)b_bytes && y < x + (uintptr_t)a_bytes;
+}
+
+// Rows of an array, in bytes: `width` of them every `stride`.  Two such arrays share a byte if their extents do, unless they are
+// different columns of one wider array.
+struct RowsOf { const void* p; int64_t rows, stride, width; };
+inline bool rec_overlap(const RowsOf& a, const RowsOf& b)
+{
+    if (a.rows < 1 || b.rows < 1 || !rec_overlap(a.p, (a.rows - 1) * a.stride + a.width, b.p, (b.rows - 1) * b.stride + b.width)) return false;
+    if (a.stride != b.stride) return true;
+    const int64_t off = (int64_t)((uintptr_t)b.p - (uintptr_t)a.p) % a.stride, ahead = off < 0 ? off + a.stride : off;
+    return ahead < a.width || a.stride - ahead < b.width;
+}
+
+inline int rec_type_size(int type) { return type == REC_TYPE_F32 ? 4 : 2; }
+inline bool rec_aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+// sums over the rows of a partial matrix [n_rows][n_cols], in row order, in 64 bits: columns [0, n0) to out0, [n0, n0 + n1) to
+// out1, the rest to out2 (each may be null)
+int launch_sum_partials(const float* part, int64_t n_rows, int64_t n_cols, float* out0, int64_t n0, float* out1, int64_t n1, float* out2, hipStream_t st);
+
+#ifdef __HIPCC__
+// ---- device side
+template <class T> __device__ __forceinline__ float to_f32(T v) { return (float)v; }
+template <class T> __device__ __forceinline__ T from_f32(float v) { return (T)v; }   // rounds to nearest even, once, at the store
+
+template <class T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
+
+// The sequence a packed row lies in: the largest s with off[s] <= row; -1 in front of the first, n_seq behind the last.
+// Only compares what it reads: offsets that are out of order lead to some s in [-1, n_seq], never out of the arrays.
+__device__ __forceinline__ int sequence_of(const int64_t* __restrict__ off, int n_seq, int64_t row)
+{
+    int lo = 0, hi = n_seq + 1;   // first index whose offset is beyond the row
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (off[mid] <= row) lo = mid + 1; else hi = mid;
+    }
+    return lo - 1;
+}
+
+// Walks packed rows forwards: the current sequence, and the first row that is not in it any more.
+struct SeqCursor {
+    int s;
+    int64_t next;
+    __device__ __forceinline__ void begin(const int64_t* __restrict__ off, int n_seq, int64_t row)
+    {
+        s = sequence_of(off, n_seq, row);
+        next = s < n_seq ? off[s + 1] : INT64_MAX;
+    }
+    __device__ __forceinline__ void advance(const int64_t* __restrict__ off, int n_seq, int64_t row)   // row >= next
+    {
+        do s++; while (s < n_seq && off[s + 1] <= row);
+        next = s < n_seq ? off[s + 1] : INT64_MAX;
+    }
+    __device__ __forceinline__ bool inside(int n_seq) const { return s >= 0 && s < n_seq; }
+};
+
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }   // v_exp_f32: 1 ulp, results below 2^-126 are 0
+#define REC_LOG2E 1.44269504088896340736f
+__device__ __forceinline__ float fast_exp(float x) { return fast_exp2(x * REC_LOG2E); }
+__device__ __forceinline__ float sigmoid_f32(float v) { return 1.0f / (1.0f + fast_exp(-v)); }
+__device__ __forceinline__ float silu_f32(float v) { return v * sigmoid_f32(v); }
+__device__ __forceinline__ float dsilu_f32(float v)
+{
+    const float g = sigmoid_f32(v);
+    return g * (1.0f + v * (1.0f - g));
+}
+
+// Rows of a step that name the same slot: `earlier`, whether a row in front of `row` names `slot`, `later`, whether one behind
+// it does.  The block's threads share the reading of the slots; every thread of the block calls it with the block's row.
+__device__ __forceinline__ void slot_is_shared(const int32_t* __restrict__ slots, int64_t rows, int64_t row, int slot, bool& earlier, bool& later)
+{
+    bool e = false, l = false;
+    for (int64_t i = threadIdx.x; i < rows; i += blockDim.x) {
+        const bool same = slots[i] == slot;
+        e |= same && i < row;
+        l |= same && i > row;
+    }
+    earlier = __syncthreads_or(e);
+    later = __syncthreads_or(l);
+}
+#endif
