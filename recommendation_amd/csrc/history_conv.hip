@@ -272,7 +272,7 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs a)
 
 // A block takes one row and up to 256 V of its channels.  The first row that names a slot takes the later ones along.
 template <class T, int W, int V>
-__global__ __launch_bounds__(256) void conv_step_kernel(ConvArgs a, const int32_t* __restrict__ slots, T* __restrict__ window)
+__global__ __launch_bounds__(256) void conv_step_kernel(ConvArgs a, const int32_t* __restrict__ slots, T* window)
 {
     const int64_t row = blockIdx.x / a.tiles;
     const int cv = (int)(blockIdx.x % a.tiles) * (int)blockDim.x + threadIdx.x, d = cv * V;
@@ -288,33 +288,29 @@ __global__ __launch_bounds__(256) void conv_step_kernel(ConvArgs a, const int32_
         return;
     }
     if (earlier) return;
-    float w[W][V], b[V], win[W - 1][V];
+    float w[W][V], b[V];
     load_filter<W, V>(a, d, w, b);
     const int64_t at = (int64_t)slot * (W - 1) * a.channels + d;
+    auto click = [&](int64_t r) {   // the window goes through memory, so that rows of a shared slot are steps like any other
+        float win[W][V];
 #pragma unroll
-    for (int j = 0; j < W - 1; j++) load_row<T, V>(window, at + (int64_t)j * a.channels, win[j]);
-    for (int64_t r = row; r < a.rows; r++) {
-        if (r > row) {
-            if (!later) break;
-            if (slots[r] != slot) continue;
-        }
-        float x[V];
-        load_row<T, V>(a.x, r * a.x_stride + d, x);
+        for (int j = 0; j < W - 1; j++) load_row<T, V>(window, at + (int64_t)j * a.channels, win[j]);
+        load_row<T, V>(a.x, r * a.x_stride + d, win[W - 1]);
 #pragma unroll
         for (int v = 0; v < V; v++) {
             float s = b[v];
 #pragma unroll
-            for (int j = 0; j < W - 1; j++) s = fmaf(w[j][v], win[j][v], s);
-            s = fmaf(w[W - 1][v], x[v], s);
+            for (int j = 0; j < W; j++) s = fmaf(w[j][v], win[j][v], s);
             y[v] = a.silu ? silu_f32(s) : s;
-#pragma unroll
-            for (int j = 0; j + 1 < W - 1; j++) win[j][v] = win[j + 1][v];
-            win[W - 2][v] = x[v];
         }
         store_row<T, V>(a.y, r * a.y_stride + d, y);
-    }
 #pragma unroll
-    for (int j = 0; j < W - 1; j++) store_row<T, V>(window, at + (int64_t)j * a.channels, win[j]);
+        for (int j = 0; j < W - 1; j++) store_row<T, V>(window, at + (int64_t)j * a.channels, win[j + 1]);
+    };
+    click(row);
+    if (later)
+        for (int64_t r = row + 1; r < a.rows; r++)
+            if (slots[r] == slot) click(r);
 }
 
 constexpr int kStripRows = 32;
