@@ -21,7 +21,7 @@ struct LossArgs {
     float *loss, *margin, *kl, *logp;
     void* dscores;
     float4* part;                             // [rows][splits] statistics of a row's parts
-    float2* stat;                             // [rows] (max, log2 of the sum) of a row
+    float2* stat;                             // [rows] (maximum, sum) of a row
     float* coef;                              // [rows] c_t, 0 where a row takes no part
     int64_t rows, n_items, scores_stride, dscores_stride;
     float scale, scale2;                      // scale2 = scale * log2(e), rounded
@@ -30,76 +30,117 @@ struct LossArgs {
     double beta, smoothing, clip_low, clip_high, kl_coef;
 };
 
-// What is known of a set of scores: its maximum m, l = sum of 2^(c (x - m)) and q = sum of (x - m) 2^(c (x - m)), c being scale *
-// log2(e) rounded to f32.  The rounding of c is the same for every score: it would move log l of all rows the same way (by 6e-8 for
-// scores of deviation 2), and the log-ratio of lists of different lengths by that times their difference.  q is the derivative of l by c
-// that takes it out again, to first order.  m is -inf for a set with nothing in it.
-struct Stat { float m, l, q; };
+// What is known of a set of scores: its maximum m, l = sum of 2^(c (x - m)), c being scale * log2(e) rounded to f32, and of a
+// sample of it ls = sum of 2^(c (x - m)) and qs = sum of (x - m) 2^(c (x - m)).  The rounding of c is the same for every score: it would
+// move log l of all rows the same way (by 6e-8 for scores of deviation 2), and the log-ratio of lists of different lengths by
+// that times their difference.  qs / ls, the derivative of log l by c, takes it out again; one score of each 16 bytes is
+// sample enough for a factor of a rounding.  m is -inf for a set with nothing in it.
+struct Stat { float m, l, ls, qs; };
 
 __device__ __forceinline__ Stat join(Stat a, Stat b, float c)
 {
     const float m = fmaxf(a.m, b.m), base = m == -INFINITY ? 0.0f : m;
-    // a set without a finite maximum has l = q = 0, or is NaN
+    // a set without a finite maximum has sums of 0, or NaN
     const float da = a.m == -INFINITY ? 0.0f : a.m - base, db = b.m == -INFINITY ? 0.0f : b.m - base;
     const float fa = fast_exp2(da * c), fb = fast_exp2(db * c);
-    return {m, a.l * fa + b.l * fb, (fa > 0.0f ? fmaf(da, a.l, a.q) * fa : 0.0f) + (fb > 0.0f ? fmaf(db, b.l, b.q) * fb : 0.0f)};
+    return {m, a.l * fa + b.l * fb, a.ls * fa + b.ls * fb, (fa > 0.0f ? fmaf(da, a.ls, a.qs) * fa : 0.0f) + (fb > 0.0f ? fmaf(db, b.ls, b.qs) * fb : 0.0f)};
+}
+
+__device__ __forceinline__ Stat join_lanes(Stat st, float c)
+{
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) st = join(st, {__shfl_xor(st.m, o, 64), __shfl_xor(st.l, o, 64), __shfl_xor(st.ls, o, 64), __shfl_xor(st.qs, o, 64)}, c);
+    return st;
+}
+
+// N vectors of V scores into a thread's statistics
+template <int V, int N>
+__device__ __forceinline__ void add_scores(Stat& st, const float (&x)[N][V], float c)
+{
+    float m = x[0][0];
+#pragma unroll
+    for (int n = 0; n < N; n++)
+#pragma unroll
+        for (int v = 0; v < V; v++) m = fmaxf(m, x[n][v]);
+    if (m > st.m) {   // rarely, after the first few
+        const float d = st.m == -INFINITY ? 0.0f : st.m - m, f = fast_exp2(d * c);
+        st.qs = f > 0.0f ? fmaf(d, st.ls, st.qs) * f : 0.0f;
+        st.ls *= f;
+        st.l *= f;
+        st.m = m;
+    }
+    const float base = st.m == -INFINITY ? 0.0f : st.m;
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        float l = 0.0f;
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            const float d = x[n][v] - base, e = fast_exp2(d * c);
+            l += e;
+            if (v == 0) {
+                st.ls += e;
+                st.qs = fmaf(fmaxf(d, -FLT_MAX), e, st.qs);   // a masked score adds 0, not -inf * 0
+            }
+        }
+        st.l += l;
+    }
+}
+
+template <class T, int V> __device__ __forceinline__ void unpack(const Pack<T, V>& p, float (&x)[V])
+{
+#pragma unroll
+    for (int v = 0; v < V; v++) x[v] = to_f32(p.v[v]);
+}
+
+// Where a row's 16-byte vectors begin and how many there are; what is in front and behind is taken singly
+struct Vectors { int64_t lead, n, tail; };
+template <class T> __device__ __forceinline__ Vectors vectors_of(const T* row, int64_t j0, int64_t j1)
+{
+    constexpr int V = 16 / sizeof(T);
+    const int64_t a0 = j0 + (int64_t)(((16 - ((uintptr_t)(row + j0) & 15)) & 15) / sizeof(T));
+    Vectors r;
+    r.lead = a0 < j1 ? a0 : j1;
+    r.n = (j1 - r.lead) / V;
+    r.tail = r.lead + r.n * V;
+    return r;
 }
 
 // the statistics of the scores [j0, j1) of a row, over the block; valid in every thread.  NaN scores give a NaN sum.
 template <class T>
 __device__ __forceinline__ Stat row_statistics(const T* __restrict__ row, int64_t j0, int64_t j1, float c, Stat* red)
 {
-    constexpr int V = 16 / sizeof(T);
-    Stat st = {-INFINITY, 0.0f, 0.0f};
-    auto add = [&](const float (&x)[V]) {
-        float m = x[0];
+    constexpr int V = 16 / sizeof(T), N = 4;   // four loads in flight per thread
+    Stat st = {-INFINITY, 0.0f, 0.0f, 0.0f};
+    const Vectors w = vectors_of(row, j0, j1);
+    const Pack<T, V>* p = reinterpret_cast<const Pack<T, V>*>(row + w.lead);
+    const int step = blockDim.x;
+    int64_t i = threadIdx.x;
+    for (; i + (N - 1) * step < w.n; i += N * step) {
+        Pack<T, V> raw[N];
 #pragma unroll
-        for (int v = 1; v < V; v++) m = fmaxf(m, x[v]);
-        if (m > st.m) {   // rarely, after the first few
-            const float d = st.m == -INFINITY ? 0.0f : st.m - m, f = fast_exp2(d * c);
-            st.q = f > 0.0f ? fmaf(d, st.l, st.q) * f : 0.0f;
-            st.l *= f;
-            st.m = m;
-        }
-        const float base = st.m == -INFINITY ? 0.0f : st.m;
-        float l = 0.0f, q = 0.0f;
+        for (int n = 0; n < N; n++) raw[n] = p[i + n * step];
+        float x[N][V];
 #pragma unroll
-        for (int v = 0; v < V; v++) {
-            const float d = x[v] - base, e = fast_exp2(d * c);
-            l += e;
-            q = fmaf(fmaxf(d, -FLT_MAX), e, q);   // a masked score adds 0, not -inf * 0
-        }
-        st.l += l;
-        st.q += q;
-    };
-    // 16-byte loads from the first aligned element on; what is in front of it and behind the last whole vector singly
-    const int64_t a0 = j0 + (int64_t)(((16 - ((uintptr_t)(row + j0) & 15)) & 15) / sizeof(T));
-    const int64_t lead = a0 < j1 ? a0 : j1, vecs = (j1 - lead) / V, tail = lead + vecs * V;
-    const Pack<T, V>* p = reinterpret_cast<const Pack<T, V>*>(row + lead);
-    for (int64_t i = threadIdx.x; i < vecs; i += blockDim.x) {
-        const Pack<T, V> raw = p[i];
-        float x[V];
-#pragma unroll
-        for (int v = 0; v < V; v++) x[v] = to_f32(raw.v[v]);
-        add(x);
+        for (int n = 0; n < N; n++) unpack<T, V>(raw[n], x[n]);
+        add_scores<V, N>(st, x, c);
     }
-    {
-        const int64_t n = (lead - j0) + (j1 - tail);   // at most 2 V - 2
-        if ((int64_t)threadIdx.x < n) {
-            const int64_t j = (int64_t)threadIdx.x < lead - j0 ? j0 + threadIdx.x : tail + (threadIdx.x - (lead - j0));
-            float x[V];
-#pragma unroll
-            for (int v = 0; v < V; v++) x[v] = v == 0 ? to_f32(row[j]) : -INFINITY;
-            add(x);
-        }
+    for (; i < w.n; i += step) {
+        float x[1][V];
+        unpack<T, V>(p[i], x[0]);
+        add_scores<V, 1>(st, x, c);
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) st = join(st, {__shfl_xor(st.m, o, 64), __shfl_xor(st.l, o, 64), __shfl_xor(st.q, o, 64)}, c);
+    const int64_t n = (w.lead - j0) + (j1 - w.tail);   // at most 2 V - 2
+    if ((int64_t)threadIdx.x < n) {
+        const int64_t j = (int64_t)threadIdx.x < w.lead - j0 ? j0 + threadIdx.x : w.tail + (threadIdx.x - (w.lead - j0));
+        const float x[1][1] = {{to_f32(row[j])}};
+        add_scores<1, 1>(st, x, c);
+    }
+    st = join_lanes(st, c);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = st;
     __syncthreads();
     st = red[0];
-    for (int w = 1; w < (int)blockDim.x / 64; w++) st = join(st, red[w], c);
+    for (int k = 1; k < (int)blockDim.x / 64; k++) st = join(st, red[k], c);
     return st;
 }
 
@@ -109,39 +150,38 @@ __device__ __forceinline__ bool row_counts(const LossArgs& a, int64_t row)
 }
 
 template <class T>
-__global__ __launch_bounds__(1024) void row_statistics_kernel(LossArgs a)
+__global__ __launch_bounds__(512) void row_statistics_kernel(LossArgs a)
 {
-    __shared__ Stat red[16];
+    __shared__ Stat red[8];
     const int64_t row = blockIdx.x / a.splits;
     const int split = blockIdx.x % a.splits;
     if (!row_counts(a, row)) return;
     if (a.off && (row < a.off[0] || row >= a.off[a.n_seq])) return;
     const int64_t per = (a.n_items + a.splits - 1) / a.splits, j0 = split * per, j1 = j0 + per < a.n_items ? j0 + per : a.n_items;
     const Stat st = row_statistics((const T*)a.scores + row * a.scores_stride, j0 < j1 ? j0 : j1, j1, a.scale2, red);
-    if (threadIdx.x == 0) a.part[blockIdx.x] = make_float4(st.m, st.l, st.q, 0.0f);
+    if (threadIdx.x == 0) a.part[blockIdx.x] = make_float4(st.m, st.l, st.ls, st.qs);
 }
 
-// log p of a row's item from its parts; false: the row takes no part
+__device__ __forceinline__ Stat part_of(const LossArgs& a, int64_t row, int k)
+{
+    const float4 p = a.part[row * a.splits + k];
+    return {p.x, p.y, p.z, p.w};
+}
+
+// log p of a row's item from the row's statistics; false: the row takes no part
 template <class T>
-__device__ __forceinline__ bool row_log_probability(const LossArgs& a, int64_t row, double& logp)
+__device__ __forceinline__ bool row_log_probability(const LossArgs& a, int64_t row, const Stat& st, double& logp)
 {
     logp = 0.0;
-    if (!row_counts(a, row)) return false;
-    Stat st = {-INFINITY, 0.0f, 0.0f};
-    for (int k = 0; k < a.splits; k++) {
-        const float4 p = a.part[row * a.splits + k];
-        st = join(st, {p.x, p.y, p.z}, a.scale2);
-    }
     if (st.m == -INFINITY && st.l == 0.0f) return false;
-    const double l = log((double)st.l);
-    a.stat[row] = make_float2(st.m, (float)(l * 1.4426950408889634));   // (base 2)
-    logp = (double)a.scale * ((double)to_f32(((const T*)a.scores)[row * a.scores_stride + a.item[row]]) - (double)st.m) - l - a.scale_rest * (double)st.q / (double)st.l;
+    const double l = log((double)st.l), mean = st.ls > 0.0f ? (double)st.qs / (double)st.ls : 0.0;
+    logp = (double)a.scale * ((double)to_f32(((const T*)a.scores)[row * a.scores_stride + a.item[row]]) - (double)st.m) - l - a.scale_rest * mean;
     return true;
 }
 
 __device__ __forceinline__ double softplus64(double v) { return fmax(v, 0.0) + log1p(exp(-fabs(v))); }
 
-// a block per pair; its threads take the rows of both lists, and add up in a fixed order
+// A block per pair adds up its two lists' rows in a fixed order: a thread per row, or a wavefront where a row has several parts.
 template <class T>
 __global__ __launch_bounds__(256) void preference_kernel(LossArgs a)
 {
@@ -154,12 +194,26 @@ __global__ __launch_bounds__(256) void preference_kernel(LossArgs a)
         const int64_t o = a.off[2 * p + k];
         begin[k] = o < 0 ? 0 : o > a.rows ? a.rows : o;
     }
+    const bool wide = a.splits > 1;
+    const int lane = wide ? threadIdx.x & 63 : 0, at = wide ? threadIdx.x >> 6 : threadIdx.x, step = wide ? 4 : 256;
 #pragma unroll
     for (int side = 0; side < 2; side++)
-        for (int64_t row = begin[side] + threadIdx.x; row < begin[side + 1]; row += 256) {
-            double logp;
-            const bool on = row_log_probability<T>(a, row, logp);
+        for (int64_t row = begin[side] + at; row < begin[side + 1]; row += step) {
+            double logp = 0.0;
+            bool on = row_counts(a, row);
+            Stat st = {-INFINITY, 0.0f, 0.0f, 0.0f};
+            if (on) {
+                if (wide) {
+                    for (int k = lane; k < a.splits; k += 64) st = join(st, part_of(a, row, k), a.scale2);
+                    st = join_lanes(st, a.scale2);
+                } else {
+                    st = part_of(a, row, 0);
+                }
+            }
+            if (lane) continue;
+            on = on && row_log_probability<T>(a, row, st, logp);
             a.logp[row] = (float)logp;
+            a.stat[row] = make_float2(st.m, st.l);
             if (on && a.ref_logp) logp -= (double)a.ref_logp[row];
             sum += side ? -logp : logp;
             a.coef[row] = on ? (side ? -1.0f : 1.0f) : 0.0f;
@@ -207,57 +261,93 @@ __device__ __forceinline__ void policy_row(const LossArgs& a, int64_t row, doubl
     if (!on) coef = 0.0f;
 }
 
+// a wavefront per row joins its parts
 template <class T>
 __global__ __launch_bounds__(256) void policy_kernel(LossArgs a)
 {
-    const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
     if (row >= a.rows) return;
-    double logp;
-    const bool on = row_log_probability<T>(a, row, logp);
+    Stat st = {-INFINITY, 0.0f, 0.0f, 0.0f};
+    const bool counts = row_counts(a, row);
+    if (counts)
+        for (int k = lane; k < a.splits; k += 64) st = join(st, part_of(a, row, k), a.scale2);
+    st = join_lanes(st, a.scale2);
+    if (lane) return;
+    double logp = 0.0;
+    const bool on = counts && row_log_probability<T>(a, row, st, logp);
+    a.stat[row] = make_float2(st.m, st.l);
     policy_row(a, row, logp, on, a.coef[row]);
 }
 
-// the gradient's elements [j0, j1) of a row
+// The gradient's elements [j0, j1) of a row, from its end to its beginning: where the same block has just read the row, what it
+// read last is still in the cache.
 template <class T>
-__device__ __forceinline__ void write_gradient(const LossArgs& a, int64_t row, int64_t j0, int64_t j1, float coef, float2 st)
+__device__ __forceinline__ void write_gradient(const LossArgs& a, int64_t row, int64_t j0, int64_t j1, float coef, float m, float l)
 {
-    constexpr int V = 16 / sizeof(T);
+    constexpr int V = 16 / sizeof(T), N = 4;
     const T* in = (const T*)a.scores + row * a.scores_stride;
     T* out = (T*)a.dscores + row * a.dscores_stride;
-    const float c = coef * a.scale;
-    const int item = a.item[row];
+    const float c = coef * a.scale, cl = -c / l;   // c (1[item] - 2^(c2 (x - m)) / l)
+    const int64_t item = a.item[row];
     auto of = [&](float x, int64_t j) {
-        const float p = fast_exp2((x - st.x) * a.scale2 - st.y);
-        return from_f32<T>(c * ((j == item ? 1.0f : 0.0f) - p));
+        const float e = cl * fast_exp2((x - m) * a.scale2);
+        return j == item ? c + e : e;
     };
-    const int64_t a0 = j0 + (int64_t)(((16 - ((uintptr_t)(out + j0) & 15)) & 15) / sizeof(T));
     const bool same = (((uintptr_t)(in + j0) ^ (uintptr_t)(out + j0)) & 15) == 0;   // rows of equal alignment move in 16-byte pieces
-    const int64_t lead = !same ? j1 : a0 < j1 ? a0 : j1, vecs = (j1 - lead) / V;
-    for (int64_t i = threadIdx.x; i < vecs; i += blockDim.x) {
-        const int64_t j = lead + i * V;
-        const Pack<T, V> q = *reinterpret_cast<const Pack<T, V>*>(in + j);
+    Vectors w = vectors_of(out, j0, j1);
+    if (!same) w = {j1, 0, j1};
+    const Pack<T, V>* p = reinterpret_cast<const Pack<T, V>*>(in + w.lead);
+    Pack<T, V>* q = reinterpret_cast<Pack<T, V>*>(out + w.lead);
+    auto vector_of = [&](const Pack<T, V>& raw, int64_t i) {
+        const int64_t j = w.lead + i * V;
+        float x[V];
+        unpack<T, V>(raw, x);
         Pack<T, V> o;
+        if (item >= j && item < j + V) {
 #pragma unroll
-        for (int v = 0; v < V; v++) o.v[v] = of(to_f32(q.v[v]), j + v);
-        *reinterpret_cast<Pack<T, V>*>(out + j) = o;
+            for (int v = 0; v < V; v++) o.v[v] = from_f32<T>(of(x[v], j + v));
+        } else {
+#pragma unroll
+            for (int v = 0; v < V; v++) o.v[v] = from_f32<T>(cl * fast_exp2((x[v] - m) * a.scale2));
+        }
+        return o;
+    };
+    const int step = blockDim.x;
+    const int64_t whole = w.n / (N * step) * (N * step);
+    for (int64_t i = whole + threadIdx.x; i < w.n; i += step) q[i] = vector_of(p[i], i);
+    for (int64_t i = whole - N * step + threadIdx.x; i >= 0; i -= N * step) {
+        Pack<T, V> raw[N];
+#pragma unroll
+        for (int n = 0; n < N; n++) raw[n] = p[i + n * step];
+#pragma unroll
+        for (int n = 0; n < N; n++) q[i + n * step] = vector_of(raw[n], i + n * step);
     }
-    for (int64_t j = j0 + threadIdx.x; j < lead; j += blockDim.x) out[j] = of(to_f32(in[j]), j);
-    for (int64_t j = lead + vecs * V + threadIdx.x; j < j1; j += blockDim.x) out[j] = of(to_f32(in[j]), j);
+    for (int64_t j = j0 + threadIdx.x; j < w.lead; j += step) out[j] = from_f32<T>(of(to_f32(in[j]), j));
+    for (int64_t j = w.tail + threadIdx.x; j < j1; j += step) out[j] = from_f32<T>(of(to_f32(in[j]), j));
 }
 
 template <class T>
 __device__ __forceinline__ void write_zeros(const LossArgs& a, int64_t row, int64_t j0, int64_t j1)
 {
+    constexpr int V = 16 / sizeof(T);
     T* out = (T*)a.dscores + row * a.dscores_stride;
-    for (int64_t j = j0 + threadIdx.x; j < j1; j += blockDim.x) out[j] = from_f32<T>(0.0f);
+    const Vectors w = vectors_of(out, j0, j1);
+    Pack<T, V> zero;
+#pragma unroll
+    for (int v = 0; v < V; v++) zero.v[v] = from_f32<T>(0.0f);
+    for (int64_t i = threadIdx.x; i < w.n; i += blockDim.x) reinterpret_cast<Pack<T, V>*>(out + w.lead)[i] = zero;
+    for (int64_t j = j0 + threadIdx.x; j < w.lead; j += blockDim.x) out[j] = zero.v[0];
+    for (int64_t j = w.tail + threadIdx.x; j < j1; j += blockDim.x) out[j] = zero.v[0];
 }
 
+// Rows in falling order: the last ones that the statistics read are the ones still in the Infinity Cache.
 template <class T>
-__global__ __launch_bounds__(1024) void gradient_kernel(LossArgs a)
+__global__ __launch_bounds__(512) void gradient_kernel(LossArgs a)
 {
-    const int64_t row = blockIdx.x / a.splits;
+    const int64_t row = a.rows - 1 - blockIdx.x / a.splits;
     const int split = blockIdx.x % a.splits;
-    const int64_t per = (a.n_items + a.splits - 1) / a.splits, j0 = split * per, j1 = j0 + per < a.n_items ? j0 + per : a.n_items;
+    const int64_t per = (a.n_items + a.splits - 1) / a.splits, j1 = (split + 1) * per < a.n_items ? (split + 1) * per : a.n_items, j0 = split * per < j1 ? split * per : j1;
     if (a.off && (row < a.off[0] || row >= a.off[a.n_seq])) {
         if (!a.zero_rest) return;
         write_zeros<T>(a, row, j0, j1);
@@ -266,7 +356,31 @@ __global__ __launch_bounds__(1024) void gradient_kernel(LossArgs a)
     }
     const float coef = a.coef[row];
     if (coef == 0.0f) write_zeros<T>(a, row, j0, j1);   // p is finite or the row's coefficient is NaN: nothing to read
-    else write_gradient<T>(a, row, j0, j1, coef, a.stat[row]);
+    else write_gradient<T>(a, row, j0, j1, coef, a.stat[row].x, a.stat[row].y);
+}
+
+// The policy loss where a block takes whole rows: it reads a row twice, but the second time from the cache (two blocks of a
+// compute unit hold 2 x 400 KB of bf16 rows of 200 000 items at a time, 200 MB over the chip, within the 256 MB of Infinity
+// Cache), and one launch does it all.
+template <class T>
+__global__ __launch_bounds__(1024) void policy_fused_kernel(LossArgs a)
+{
+    __shared__ Stat red[16];
+    __shared__ float coef_s;
+    const int64_t row = blockIdx.x;
+    const bool counts = row_counts(a, row);
+    Stat st = {-INFINITY, 0.0f, 0.0f, 0.0f};
+    if (counts) st = row_statistics((const T*)a.scores + row * a.scores_stride, 0, a.n_items, a.scale2, red);
+    if (threadIdx.x == 0) {
+        double logp = 0.0;
+        const bool on = counts && row_log_probability<T>(a, row, st, logp);
+        policy_row(a, row, logp, on, coef_s);
+    }
+    if (!a.dscores) return;
+    __syncthreads();
+    const float coef = coef_s;
+    if (coef == 0.0f) write_zeros<T>(a, row, 0, a.n_items);
+    else write_gradient<T>(a, row, 0, a.n_items, coef, st.m, st.l);
 }
 
 // rows of no list, where no gradient pass comes by
@@ -399,10 +513,20 @@ extern "C" int rec_policy_loss(const rec_loss_desc* d, const void* scores, int64
         DeviceScope scope;
         HIP_TRY(scope.enter(d->device));
         hipStream_t st = (hipStream_t)stream;
+        if (a.splits == 1) {
+            // rows of few items take smaller blocks: two 16-byte loads for each thread at least
+            const int64_t vectors = d->n_items * rec_type_size(d->type) / 16 / 2;
+            const int threads = vectors >= 1024 ? 1024 : vectors < 64 ? 64 : (int)(vectors + 63) / 64 * 64;
+#define CALL(T) policy_fused_kernel<T><<<(unsigned)d->rows, threads, 0, st>>>(a)
+            LOSS_DISPATCH(CALL)
+#undef CALL
+            HIP_TRY(hipGetLastError());
+            return 0;
+        }
         const unsigned blocks = (unsigned)(d->rows * a.splits);
 #define CALL(T)                                                                                     \
         row_statistics_kernel<T><<<blocks, kThreads, 0, st>>>(a);                                   \
-        policy_kernel<T><<<(unsigned)((d->rows + 255) / 256), 256, 0, st>>>(a);                     \
+        policy_kernel<T><<<(unsigned)((d->rows + 3) / 4), 256, 0, st>>>(a);                         \
         if (dscores) gradient_kernel<T><<<blocks, kThreads, 0, st>>>(a)
         LOSS_DISPATCH(CALL)
 #undef CALL

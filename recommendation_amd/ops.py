@@ -69,6 +69,7 @@ _SIGNATURES = {
     "rec_policy_loss_workspace": [_P],
 }
 _functions = {}
+_raw_stream = torch._C._cuda_getCurrentRawStream   # the handle of the current stream, without an object around it
 
 
 def _fn(name):
@@ -81,216 +82,252 @@ def _fn(name):
     return f
 
 
-def _need(ok, what):
-    if not ok:
-        raise ValueError("recsys operators: " + what)
+def _bad(what):
+    raise ValueError("recsys operators: " + what)
 
 
-def _rows(t, name, like=None, shape=None):
-    """A [rows, width] array of activations: (pointer, row stride)."""
-    _need(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} must be a tensor on the GPU")
-    _need(t.dim() == 2 if shape is None else tuple(t.shape) == tuple(shape), f"{name} must have the shape {tuple(shape) if shape is not None else '[rows, width]'}")
-    _need(t.dtype in _TYPE, f"{name} must be float32, float16 or bfloat16")
-    if like is not None:
-        _need(t.dtype == like.dtype and t.device == like.device, f"{name} must have the type and the device of the other activations")
-    rows, width = t.shape[0], t[0].numel() if t.dim() > 2 and t.shape[0] else (t.shape[1] if t.dim() == 2 else 0)
-    s = t.stride()
-    if t.dim() == 2:
-        _need(t.shape[1] <= 1 or s[1] == 1, f"the last dimension of {name} must be contiguous")
-    elif rows:
-        _need(t[0].is_contiguous(), f"the groups of a row of {name} must be contiguous")
-    # a single row's stride means nothing to torch; the rows of an array must not run into each other
-    stride = width if rows <= 1 else s[0]
-    _need(stride >= width, f"the rows of {name} overlap")
-    return t.data_ptr(), stride
+# A call of a few microseconds spends most of them here, so the checks take one pass over plain attributes; what is wrong is
+# found out in the functions that say so.
+def _first(t, name):
+    """The array that sets a call's type, GPU and shape: (type, torch type, device, rows, width)."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        _bad(f"{name} must be a tensor on the GPU")
+    dtype = t.dtype
+    kind = _TYPE.get(dtype)
+    if kind is None:
+        _bad(f"{name} must be float32, float16 or bfloat16")
+    shape = t.shape
+    if len(shape) != 2:
+        _bad(f"{name} must have the shape [rows, width]")
+    return kind, dtype, t.get_device(), shape[0], shape[1]
 
 
-def _f32(t, name, shape, like, dtype=torch.float32):
+def _rows(t, name, dtype, dev, rows, width):
+    """A [rows, width] array of activations, its rows anywhere: (pointer, row stride)."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == dev and t.shape == (rows, width):
+        s0, s1 = t.stride()
+        if s1 == 1 or width <= 1:
+            if rows <= 1 or width == 0:   # the stride of a single row means nothing to torch
+                return t.data_ptr(), width
+            if s0 >= width:
+                return t.data_ptr(), s0
+            _bad(f"the rows of {name} overlap")
+        _bad(f"the last dimension of {name} must be contiguous")
+    _bad_array(t, name, dtype, dev, (rows, width))
+
+
+def _groups(t, name, dtype, dev, rows, groups, states):
+    """A [rows, groups, states] array, the groups of a row contiguous: (pointer, row stride)."""
+    width = groups * states
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == dev and t.shape == (rows, groups, states):
+        s0, s1, s2 = t.stride()
+        if (s2 == 1 or states <= 1) and (s1 == states or groups <= 1):
+            if rows <= 1:
+                return t.data_ptr(), width
+            if s0 >= width:
+                return t.data_ptr(), s0
+            _bad(f"the rows of {name} overlap")
+        _bad(f"the groups of a row of {name} must be contiguous")
+    _bad_array(t, name, dtype, dev, (rows, groups, states))
+
+
+def _whole(t, name, shape, dtype, dev):
     """A contiguous array of a known shape, or None: its pointer."""
     if t is None:
         return None
-    _need(isinstance(t, torch.Tensor) and t.dtype == dtype and t.device == like.device, f"{name} must be {dtype} on the device of the activations")
-    _need(tuple(t.shape) == tuple(shape), f"{name} must have the shape {tuple(shape)}")
-    _need(t.is_contiguous(), f"{name} must be contiguous")
-    return t.data_ptr()
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == dev and t.shape == shape and t.is_contiguous():
+        return t.data_ptr()
+    _bad_array(t, name, dtype, dev, shape)
 
 
-def _offsets(t, like):
-    _need(isinstance(t, torch.Tensor) and t.dtype == torch.int64 and t.device == like.device and t.dim() == 1 and t.shape[0] >= 1 and t.is_contiguous(),
-          "seq_off must be a contiguous int64 vector on the device of the activations")
-    return t.data_ptr(), t.shape[0] - 1
+def _bad_array(t, name, dtype, dev, shape):
+    if not isinstance(t, torch.Tensor):
+        _bad(f"{name} must be a tensor")
+    if t.dtype is not dtype:
+        _bad(f"{name} must have the type {dtype}, not {t.dtype}")
+    if not t.is_cuda or t.get_device() != dev:
+        _bad(f"{name} must be on the GPU of the other arguments")
+    if tuple(t.shape) != tuple(shape):
+        _bad(f"{name} must have the shape {tuple(shape)}, not {tuple(t.shape)}")
+    _bad(f"{name} must be contiguous")
 
 
-def _stream(t):
-    return torch.cuda.current_stream(t.device).cuda_stream
-
-
-def _out(out, name, shape, like):
-    """The output array, and whether its rows outside all histories are the call's to clear."""
-    if out is None:
-        return torch.empty(shape, dtype=like.dtype, device=like.device), 1
-    _rows(out, name, like, shape)
-    return out, 0
-
-
-def _workspace(size, like):
-    if size < 0:
-        capi._check(-1)
-    return torch.empty(size, dtype=torch.uint8, device=like.device) if size else None
+def _offsets(t, dev):
+    if isinstance(t, torch.Tensor) and t.dtype is torch.int64 and t.get_device() == dev and t.dim() == 1 and t.is_contiguous() and len(t) >= 1:
+        return t.data_ptr(), len(t) - 1
+    _bad("seq_off must be a contiguous int64 vector of at least one entry on the GPU of the other arguments")
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _conv_desc(x, weight, n_seq, silu, zero_rest):
-    _need(isinstance(weight, torch.Tensor) and weight.dim() == 2, "weight must have the shape [channels, taps]")
-    return _ConvDesc(x.device.index, _TYPE[x.dtype], x.shape[0], n_seq, x.shape[1], weight.shape[1], 1 if silu else 0, zero_rest)
+def _space(size, like):
+    """A workspace: of the stream's own pool, so it may go back there when the call returns."""
+    if size <= 0:
+        if size < 0:
+            capi._check(-1)
+        return None, None
+    t = like.new_empty(size, dtype=torch.uint8)
+    return t, t.data_ptr()
+
+
+F32 = torch.float32
+
+
+def _conv(x, weight, bias, n_seq, silu, zero_rest):
+    kind, dtype, dev, rows, ch = _first(x, "x")
+    px, sx = _rows(x, "x", dtype, dev, rows, ch)
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
+        _bad("weight must have the shape [channels, taps]")
+    taps = weight.shape[1]
+    d = _ConvDesc(dev, kind, rows, n_seq, ch, taps, 1 if silu else 0, zero_rest)
+    return d, px, sx, dtype, dev, rows, ch, taps, _whole(weight, "weight", (ch, taps), F32, dev), _whole(bias, "bias", (ch,), F32, dev)
 
 
 def history_conv(x, weight, bias=None, *, seq_off, initial=None, silu=True, want_final=False, out=None):
     """(y, final window or None): x [rows, channels], weight [channels, taps], initial and final [histories, taps - 1, channels]."""
-    px, sx = _rows(x, "x")
-    off, n = _offsets(seq_off, x)
-    y, zero = _out(out, "out", x.shape, x)
-    d = _conv_desc(x, weight, n, silu, zero)
-    window = (n, max(0, d.taps - 1), d.channels)
-    args = (_f32(weight, "weight", (d.channels, d.taps), x), _f32(bias, "bias", (d.channels,), x), off, _f32(initial, "initial", window, x, x.dtype))
-    final = torch.empty(window, dtype=x.dtype, device=x.device) if want_final else None
-    py, sy = _rows(y, "out")
-    capi._check(_fn("rec_history_conv")(C.byref(d), px, sx, *args, py, sy, _ptr(final), _stream(x)))
+    off, n = _offsets(seq_off, x.get_device())
+    d, px, sx, dtype, dev, rows, ch, taps, w, b = _conv(x, weight, bias, n, silu, 1 if out is None else 0)
+    window = (n, max(0, taps - 1), ch)
+    i = _whole(initial, "initial", window, dtype, dev)
+    y = x.new_empty((rows, ch)) if out is None else out
+    py, sy = _rows(y, "out", dtype, dev, rows, ch)
+    final = x.new_empty(window) if want_final else None
+    capi._check(_fn("rec_history_conv")(C.byref(d), px, sx, w, b, off, i, py, sy, _ptr(final), _raw_stream(dev)))
     return y, final
 
 
 def history_conv_backward(dy, x, weight, bias=None, *, seq_off, initial=None, silu=True, dfinal=None, out=None):
     """ConvGradients for dy [rows, channels] and dfinal (the final window's gradient); dbias and dinitial are None without bias / initial."""
-    px, sx = _rows(x, "x")
-    pg, sg = _rows(dy, "dy", x, x.shape)
-    off, n = _offsets(seq_off, x)
-    dx, zero = _out(out, "out", x.shape, x)
-    d = _conv_desc(x, weight, n, silu, zero)
-    window = (n, max(0, d.taps - 1), d.channels)
-    args = (_f32(weight, "weight", (d.channels, d.taps), x), _f32(bias, "bias", (d.channels,), x), off, _f32(initial, "initial", window, x, x.dtype),
-            _f32(dfinal, "dfinal", window, x, x.dtype))
+    off, n = _offsets(seq_off, x.get_device())
+    d, px, sx, dtype, dev, rows, ch, taps, w, b = _conv(x, weight, bias, n, silu, 1 if out is None else 0)
+    pg, sg = _rows(dy, "dy", dtype, dev, rows, ch)
+    window = (n, max(0, taps - 1), ch)
+    i, df = _whole(initial, "initial", window, dtype, dev), _whole(dfinal, "dfinal", window, dtype, dev)
+    dx = x.new_empty((rows, ch)) if out is None else out
+    pd, sd = _rows(dx, "out", dtype, dev, rows, ch)
     dweight = torch.empty_like(weight)
     dbias = torch.empty_like(bias) if bias is not None else None
     dinitial = torch.empty_like(initial) if initial is not None else None
     size = _fn("rec_history_conv_backward_workspace")(C.byref(d))
-    ws = _workspace(size, x)
-    pd, sd = _rows(dx, "out")
-    capi._check(_fn("rec_history_conv_backward")(C.byref(d), pg, sg, px, sx, *args, pd, sd, _ptr(dweight), _ptr(dbias), _ptr(dinitial), _ptr(ws), size, _stream(x)))
+    ws, pw = _space(size, x)
+    capi._check(_fn("rec_history_conv_backward")(C.byref(d), pg, sg, px, sx, w, b, off, i, df, pd, sd, dweight.data_ptr(), _ptr(dbias), _ptr(dinitial), pw, size,
+                                                 _raw_stream(dev)))
     return ConvGradients(dx, dweight, dbias, dinitial)
 
 
 def history_conv_step(x, weight, bias=None, *, state, slots, silu=True, out=None):
     """y [rows, channels] of one click per row; state [slots, taps - 1, channels] (windows, of x's type) is updated in place at
     slots [rows] (int32)."""
-    px, sx = _rows(x, "x")
-    y, _ = _out(out, "out", x.shape, x)
-    _need(isinstance(state, torch.Tensor) and state.dim() == 3, "state must have the shape [slots, taps - 1, channels]")
-    d = _conv_desc(x, weight, state.shape[0], silu, 0)
-    w = _f32(weight, "weight", (d.channels, d.taps), x), _f32(bias, "bias", (d.channels,), x)
-    ps = _f32(state, "state", (d.n_seq, d.taps - 1, d.channels), x, x.dtype)
-    py, sy = _rows(y, "out")
-    capi._check(_fn("rec_history_conv_step")(C.byref(d), px, sx, *w, _f32(slots, "slots", (d.rows,), x, torch.int32), ps, py, sy, _stream(x)))
+    n = len(state)
+    d, px, sx, dtype, dev, rows, ch, taps, w, b = _conv(x, weight, bias, n, silu, 0)
+    ps = _whole(state, "state", (n, taps - 1, ch), dtype, dev)
+    y = x.new_empty((rows, ch)) if out is None else out
+    py, sy = _rows(y, "out", dtype, dev, rows, ch)
+    capi._check(_fn("rec_history_conv_step")(C.byref(d), px, sx, w, b, _whole(slots, "slots", (rows,), torch.int32, dev), ps, py, sy, _raw_stream(dev)))
     return y
 
 
 def _scan(u, delta, A, B, Cm, D, z, delta_bias, n_seq, initial, softplus, zero_rest):
-    pu, su = _rows(u, "u")
-    pd, sd = _rows(delta, "delta", u, u.shape)
-    pz, sz = _rows(z, "z", u, u.shape) if z is not None else (None, 0)
-    _need(isinstance(A, torch.Tensor) and A.dim() == 2, "A must have the shape [channels, states]")
-    rows, channels, states = u.shape[0], u.shape[1], A.shape[1]
-    _need(isinstance(B, torch.Tensor) and B.dim() == 3 and B.shape[1] >= 1, "B must have the shape [rows, groups, states]")
+    kind, dtype, dev, rows, ch = _first(u, "u")
+    pu, su = _rows(u, "u", dtype, dev, rows, ch)
+    pd, sd = _rows(delta, "delta", dtype, dev, rows, ch)
+    pz, sz = _rows(z, "z", dtype, dev, rows, ch) if z is not None else (None, 0)
+    if not isinstance(A, torch.Tensor) or A.dim() != 2:
+        _bad("A must have the shape [channels, states]")
+    states = A.shape[1]
+    if not isinstance(B, torch.Tensor) or B.dim() != 3:
+        _bad("B must have the shape [rows, groups, states]")
     groups = B.shape[1]
-    pB, sB = _rows(B, "B", u, (rows, groups, states))
-    pC, sC = _rows(Cm, "C", u, (rows, groups, states))
-    width = groups * states
-    d = _ScanDesc(u.device.index, _TYPE[u.dtype], rows, n_seq, channels, groups, states, 1 if softplus else 0, zero_rest)
-    i = _ScanInputs(pu, pd, pz, pB, pC, su, sd, sz, max(sB, width), max(sC, width), _f32(A, "A", (channels, states), u), _f32(D, "D", (channels,), u),
-                    _f32(delta_bias, "delta_bias", (channels,), u), _f32(initial, "initial", (n_seq, channels, states), u))
-    return d, i
+    pB, sB = _groups(B, "B", dtype, dev, rows, groups, states)
+    pC, sC = _groups(Cm, "C", dtype, dev, rows, groups, states)
+    d = _ScanDesc(dev, kind, rows, n_seq, ch, groups, states, 1 if softplus else 0, zero_rest)
+    i = _ScanInputs(pu, pd, pz, pB, pC, su, sd, sz, sB, sC, _whole(A, "A", (ch, states), F32, dev), _whole(D, "D", (ch,), F32, dev),
+                    _whole(delta_bias, "delta_bias", (ch,), F32, dev), _whole(initial, "initial", (n_seq, ch, states), F32, dev))
+    return d, i, dtype, dev, rows, ch, states
 
 
 def history_scan(u, delta, A, B, C_, D=None, z=None, delta_bias=None, *, seq_off, initial=None, softplus=True, want_final=False, want_checkpoints=False, out=None):
     """(y, final state or None, checkpoints or None): u, delta, z [rows, channels], A [channels, states], B, C [rows, groups, states],
     D, delta_bias [channels], initial and final [histories, channels, states] float32.  The gradient takes the checkpoints."""
-    y, zero = _out(out, "out", u.shape, u)
-    off, n = _offsets(seq_off, u)
-    d, i = _scan(u, delta, A, B, C_, D, z, delta_bias, n, initial, softplus, zero)
-    py, sy = _rows(y, "out")
-    state = (d.channels, d.states)
-    final = torch.empty((n,) + state, dtype=torch.float32, device=u.device) if want_final else None
-    kept = torch.empty((-(-d.rows // SCAN_CHECKPOINT),) + state, dtype=torch.float32, device=u.device) if want_checkpoints else None
+    off, n = _offsets(seq_off, u.get_device())
+    d, i, dtype, dev, rows, ch, states = _scan(u, delta, A, B, C_, D, z, delta_bias, n, initial, softplus, 1 if out is None else 0)
+    y = u.new_empty((rows, ch)) if out is None else out
+    py, sy = _rows(y, "out", dtype, dev, rows, ch)
+    final = u.new_empty((n, ch, states), dtype=F32) if want_final else None
+    kept = u.new_empty((-(-rows // SCAN_CHECKPOINT), ch, states), dtype=F32) if want_checkpoints else None
     size = _fn("rec_history_scan_workspace")(C.byref(d))
-    ws = _workspace(size, u)
-    capi._check(_fn("rec_history_scan")(C.byref(d), C.byref(i), off, py, sy, _ptr(final), _ptr(kept), _ptr(ws), size, _stream(u)))
+    ws, pw = _space(size, u)
+    capi._check(_fn("rec_history_scan")(C.byref(d), C.byref(i), off, py, sy, _ptr(final), _ptr(kept), pw, size, _raw_stream(dev)))
     return y, final, kept
 
 
 def history_scan_backward(dy, u, delta, A, B, C_, D=None, z=None, delta_bias=None, *, seq_off, checkpoints, initial=None, softplus=True, dfinal=None):
     """ScanGradients for dy [rows, channels] and dfinal (the final state's gradient); dD, dz, ddelta_bias and dinitial are None
     where the call has no D, z, delta_bias or initial."""
-    off, n = _offsets(seq_off, u)
-    d, i = _scan(u, delta, A, B, C_, D, z, delta_bias, n, initial, softplus, 1)
-    pg, sg = _rows(dy, "dy", u, u.shape)
-    state = (d.channels, d.states)
-    kept = _f32(checkpoints, "checkpoints", (-(-d.rows // SCAN_CHECKPOINT),) + state, u)
-    _need(kept is not None, "the gradient needs the forward call's checkpoints")
-    df = _f32(dfinal, "dfinal", (n,) + state, u)
-
-    def like(t, shape, dtype):
-        return torch.empty(shape, dtype=dtype, device=u.device) if t is not None else None
-
-    rows, group = tuple(u.shape), (d.rows, d.groups, d.states)
-    du, ddelta, dz = like(u, rows, u.dtype), like(u, rows, u.dtype), like(z, rows, u.dtype)
-    dB, dC = like(u, group, u.dtype), like(u, group, u.dtype)
-    f = torch.float32
-    dA, dD, dbias, dinitial = like(A, state, f), like(D, state[:1], f), like(delta_bias, state[:1], f), like(initial, (n,) + state, f)
-    o = _ScanGradientPointers(_ptr(du), _ptr(ddelta), _ptr(dz), _ptr(dB), _ptr(dC), _ptr(dA), _ptr(dD), _ptr(dbias), _ptr(dinitial))
+    off, n = _offsets(seq_off, u.get_device())
+    d, i, dtype, dev, rows, ch, states = _scan(u, delta, A, B, C_, D, z, delta_bias, n, initial, softplus, 1)
+    pg, sg = _rows(dy, "dy", dtype, dev, rows, ch)
+    if checkpoints is None:
+        _bad("the gradient needs the forward call's checkpoints")
+    kept = _whole(checkpoints, "checkpoints", (-(-rows // SCAN_CHECKPOINT), ch, states), F32, dev)
+    df = _whole(dfinal, "dfinal", (n, ch, states), F32, dev)
+    du, ddelta = u.new_empty((rows, ch)), u.new_empty((rows, ch))
+    dz = u.new_empty((rows, ch)) if z is not None else None
+    dB, dC = u.new_empty(B.shape), u.new_empty(B.shape)
+    dA = torch.empty_like(A)
+    dD = torch.empty_like(D) if D is not None else None
+    dbias = torch.empty_like(delta_bias) if delta_bias is not None else None
+    dinitial = torch.empty_like(initial) if initial is not None else None
+    o = _ScanGradientPointers(du.data_ptr(), ddelta.data_ptr(), _ptr(dz), dB.data_ptr(), dC.data_ptr(), dA.data_ptr(), _ptr(dD), _ptr(dbias), _ptr(dinitial))
     size = _fn("rec_history_scan_backward_workspace")(C.byref(d))
-    ws = _workspace(size, u)
-    capi._check(_fn("rec_history_scan_backward")(C.byref(d), pg, sg, C.byref(i), off, kept, df, C.byref(o), _ptr(ws), size, _stream(u)))
+    ws, pw = _space(size, u)
+    capi._check(_fn("rec_history_scan_backward")(C.byref(d), pg, sg, C.byref(i), off, kept, df, C.byref(o), pw, size, _raw_stream(dev)))
     return ScanGradients(du, ddelta, dA, dB, dC, dD, dz, dbias, dinitial)
 
 
 def history_scan_step(u, delta, A, B, C_, D=None, z=None, delta_bias=None, *, state, slots, softplus=True, out=None):
     """y [rows, channels] of one click per row; state [slots, channels, states] float32 is updated in place at slots [rows] (int32)."""
-    y, _ = _out(out, "out", u.shape, u)
-    _need(isinstance(state, torch.Tensor) and state.dim() == 3, "state must have the shape [slots, channels, states]")
-    d, i = _scan(u, delta, A, B, C_, D, z, delta_bias, state.shape[0], None, softplus, 0)
-    ps = _f32(state, "state", (d.n_seq, d.channels, d.states), u)
-    py, sy = _rows(y, "out")
-    capi._check(_fn("rec_history_scan_step")(C.byref(d), C.byref(i), _f32(slots, "slots", (d.rows,), u, torch.int32), ps, py, sy, _stream(u)))
+    n = len(state)
+    d, i, dtype, dev, rows, ch, states = _scan(u, delta, A, B, C_, D, z, delta_bias, n, None, softplus, 0)
+    ps = _whole(state, "state", (n, ch, states), F32, dev)
+    y = u.new_empty((rows, ch)) if out is None else out
+    py, sy = _rows(y, "out", dtype, dev, rows, ch)
+    capi._check(_fn("rec_history_scan_step")(C.byref(d), C.byref(i), _whole(slots, "slots", (rows,), torch.int32, dev), ps, py, sy, _raw_stream(dev)))
     return y
 
 
-def _gradient(scores, grad_weight, n, out):
-    """(pointer to the weights, dscores or None, its pointer and stride, whether its rows outside all lists are to be cleared)"""
-    _need(grad_weight is not None or out is None, "out is the gradient's: it needs grad_weight")
+def _gradient(scores, grad_weight, n, out, dtype, dev, rows, width):
+    """(pointer to the weights, dscores or None, its pointer and stride)"""
     if grad_weight is None:
-        return None, None, None, 0, 1
-    w = _f32(grad_weight, "grad_weight", (n,), scores)
-    ds, zero = _out(out, "out", scores.shape, scores)
-    return (w, ds, *_rows(ds, "out"), zero)
+        if out is not None:
+            _bad("out is the gradient's: it needs grad_weight")
+        return None, None, None, 0
+    w = _whole(grad_weight, "grad_weight", (n,), F32, dev)
+    ds = scores.new_empty((rows, width)) if out is None else out
+    return (w, ds, *_rows(ds, "out", dtype, dev, rows, width))
 
 
 def preference_loss(scores, items, seq_off, ref_logp=None, *, beta=0.1, label_smoothing=0.0, scale=1.0, grad_weight=None, out=None):
     """PreferenceLoss(loss [pairs], margin [pairs], logp [rows], dscores): scores [rows, catalogue], items [rows] (int32), list 2p of
     seq_off [2 pairs + 1] preferred to list 2p + 1, ref_logp [rows].  With grad_weight [pairs], dscores is the gradient of
     sum(grad_weight * loss); out=scores writes it over the scores."""
-    p, s = _rows(scores, "scores")
-    off, n = _offsets(seq_off, scores)
-    _need(n % 2 == 0, "seq_off must have 2 pairs + 1 entries")
-    rows, pairs, dev = scores.shape[0], n // 2, scores.device
-    w, ds, pd, sd, zero = _gradient(scores, grad_weight, pairs, out)
-    d = _LossDesc(dev.index, _TYPE[scores.dtype], rows, scores.shape[1], scale, zero)
-    args = _f32(items, "items", (rows,), scores, torch.int32), off, pairs, _f32(ref_logp, "ref_logp", (rows,), scores), beta, label_smoothing, w
-    loss, margin, logp = (torch.empty(k, dtype=torch.float32, device=dev) for k in (pairs, pairs, rows))
+    kind, dtype, dev, rows, width = _first(scores, "scores")
+    off, n = _offsets(seq_off, dev)
+    if n % 2:
+        _bad("seq_off must have 2 pairs + 1 entries")
+    pairs = n // 2
+    p, s = _rows(scores, "scores", dtype, dev, rows, width)
+    w, ds, pd, sd = _gradient(scores, grad_weight, pairs, out, dtype, dev, rows, width)
+    d = _LossDesc(dev, kind, rows, width, scale, 1 if out is None else 0)
+    i, r = _whole(items, "items", (rows,), torch.int32, dev), _whole(ref_logp, "ref_logp", (rows,), F32, dev)
+    logp = scores.new_empty(rows, dtype=F32)
+    loss, margin = scores.new_empty((2, pairs), dtype=F32).unbind()
     size = _fn("rec_preference_loss_workspace")(C.byref(d), pairs)
-    ws = _workspace(size, scores)
-    capi._check(_fn("rec_preference_loss")(C.byref(d), p, s, *args, _ptr(loss), _ptr(margin), _ptr(logp), pd, sd, _ptr(ws), size, _stream(scores)))
+    ws, pw = _space(size, scores)
+    capi._check(_fn("rec_preference_loss")(C.byref(d), p, s, i, off, pairs, r, beta, label_smoothing, w, loss.data_ptr(), margin.data_ptr(), logp.data_ptr(), pd, sd, pw, size,
+                                           _raw_stream(dev)))
     return PreferenceLoss(loss, margin, logp, ds)
 
 
@@ -298,15 +335,20 @@ def policy_loss(scores, items, old_logp, advantage, ref_logp=None, *, clip_low=0
     """PolicyLoss(loss [rows], kl [rows] or None, logp [rows], dscores): scores [rows, catalogue], items [rows] (int32; a row with an
     item outside the catalogue takes no part), old_logp, advantage and ref_logp [rows].  With grad_weight [rows], dscores is the
     gradient of sum(grad_weight * loss); out=scores writes it over the scores."""
-    p, s = _rows(scores, "scores")
-    rows, dev = scores.shape[0], scores.device
-    w, ds, pd, sd, _ = _gradient(scores, grad_weight, rows, out)
-    d = _LossDesc(dev.index, _TYPE[scores.dtype], rows, scores.shape[1], scale, 0)
-    args = (_f32(items, "items", (rows,), scores, torch.int32), _f32(old_logp, "old_logp", (rows,), scores), _f32(advantage, "advantage", (rows,), scores),
-            _f32(ref_logp, "ref_logp", (rows,), scores), clip_low, clip_high, kl_coef, w)
-    loss, logp = (torch.empty(rows, dtype=torch.float32, device=dev) for _ in range(2))
-    kl = torch.empty(rows, dtype=torch.float32, device=dev) if ref_logp is not None else None
+    kind, dtype, dev, rows, width = _first(scores, "scores")
+    p, s = _rows(scores, "scores", dtype, dev, rows, width)
+    w, ds, pd, sd = _gradient(scores, grad_weight, rows, out, dtype, dev, rows, width)
+    d = _LossDesc(dev, kind, rows, width, scale, 0)
+    vec = (rows,)
+    i = _whole(items, "items", vec, torch.int32, dev)
+    old, adv, ref = _whole(old_logp, "old_logp", vec, F32, dev), _whole(advantage, "advantage", vec, F32, dev), _whole(ref_logp, "ref_logp", vec, F32, dev)
+    if ref_logp is None:
+        loss, logp = scores.new_empty((2, rows), dtype=F32).unbind()
+        kl = None
+    else:
+        loss, logp, kl = scores.new_empty((3, rows), dtype=F32).unbind()
     size = _fn("rec_policy_loss_workspace")(C.byref(d))
-    ws = _workspace(size, scores)
-    capi._check(_fn("rec_policy_loss")(C.byref(d), p, s, *args, _ptr(loss), _ptr(kl), _ptr(logp), pd, sd, _ptr(ws), size, _stream(scores)))
+    ws, pw = _space(size, scores)
+    capi._check(_fn("rec_policy_loss")(C.byref(d), p, s, i, old, adv, ref, clip_low, clip_high, kl_coef, w, loss.data_ptr(), _ptr(kl), logp.data_ptr(), pd, sd, pw, size,
+                                       _raw_stream(dev)))
     return PolicyLoss(loss, kl, logp, ds)
