@@ -11,6 +11,7 @@
 // (only from the last history's beginning on, and only if it goes on), the second links the chunks of each history, the third
 // walks again from the linked states and writes y.  With one chunk the first two are not launched.
 #include "operators.h"
+#include <type_traits>
 
 namespace {
 
@@ -54,17 +55,48 @@ template <int LN> struct Place {
     }
 };
 
-// four of a channel's states, of an f32 array [...][channels][states]
+// Four of a channel's states, of an f32 array [...][channels][states].  The array's leading index is the same for the whole
+// block, so an address is a scalar base and a 32-bit offset of the lane (channels * states * 4 < 2^29).
+template <int LN>
 __device__ __forceinline__ void load_states(const float* p, int64_t lead, const ScanArgs& a, int d, int n0, bool on, float (&h)[4])
 {
+    struct alignas(4) Four { float v[4]; };
+    const float* base = p + lead * ((int64_t)a.channels * a.states);
+    const int at = d * a.states + n0;
+    if (!p) {
 #pragma unroll
-    for (int e = 0; e < 4; e++) h[e] = on && p && n0 + e < a.states ? p[(lead * a.channels + d) * a.states + n0 + e] : 0.0f;
+        for (int e = 0; e < 4; e++) h[e] = 0.0f;
+    } else if (a.states == 4 * LN) {
+        const Four f = *reinterpret_cast<const Four*>(base + at);
+#pragma unroll
+        for (int e = 0; e < 4; e++) h[e] = on ? f.v[e] : 0.0f;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) h[e] = on && n0 + e < a.states ? base[at + e] : 0.0f;
+    }
 }
+template <int LN>
 __device__ __forceinline__ void store_states(float* p, int64_t lead, const ScanArgs& a, int d, int n0, bool on, const float (&h)[4])
 {
+    struct alignas(4) Four { float v[4]; };
+    float* base = p + lead * ((int64_t)a.channels * a.states);
+    const int at = d * a.states + n0;
+    if (!on) return;
+    if (a.states == 4 * LN) {
+        *reinterpret_cast<Four*>(base + at) = Four{{h[0], h[1], h[2], h[3]}};
+        return;
+    }
 #pragma unroll
     for (int e = 0; e < 4; e++)
-        if (on && n0 + e < a.states) p[(lead * a.channels + d) * a.states + n0 + e] = h[e];
+        if (n0 + e < a.states) base[at + e] = h[e];
+}
+
+// `v`, computed whether or not the choice that follows wants it: a choice that is the same for the whole launch would otherwise
+// become a branch for each of a thread's values, and keep their loads and exps from overlapping.
+__device__ __forceinline__ float computed(float v)
+{
+    asm volatile("" : "+v"(v));
+    return v;
 }
 
 template <class T>
@@ -74,16 +106,51 @@ __device__ __forceinline__ float delta_of(const ScanArgs& a, int64_t row, int d,
     return a.softplus ? softplus_f32(raw) : raw;
 }
 
-// B or C of the tile's rows, zero where the row is not one of [lo, hi)
-template <class T, int NP>
-__device__ __forceinline__ void stage_group(const void* p, int64_t stride, const ScanArgs& a, int g, int64_t t0, int64_t lo, int64_t hi, float (&s)[TT][NP])
-{
-    for (int i = threadIdx.x; i < TT * NP; i += 256) {
-        const int r = i / NP, n = i % NP;
-        const int64_t row = t0 + r;
-        s[r][n] = n < a.states && row >= lo && row < hi ? to_f32(((const T*)p)[row * stride + (int64_t)g * a.states + n]) : 0.0f;
+// What a thread stages of a tile: PT (row, channel) pairs, 256 apart, all of one channel, and NB values each of B and C.
+// Loads come first and unconditionally (a row or channel outside the chunk takes the nearest inside), so that all of a tile's are
+// in flight together; what does not count is set to zero when it is staged.
+template <class T, int LN, bool U, bool Z, bool DY, bool GB, bool GC> struct Tile {
+    static constexpr int CH = 256 / LN, NP = 4 * LN, PT = TT * CH / 256, NB = TT * NP > 256 ? TT * NP / 256 : 1;
+    T d[PT], u[U ? PT : 1], z[Z ? PT : 1], g[DY ? PT : 1], b[GB ? NB : 1], c[GC ? NB : 1];
+    // the row of pair k: where a wavefront's pairs are of one row, a scalar
+    static __device__ __forceinline__ int row(int k)
+    {
+        const int t = CH >= 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x & ~63u) : (int)threadIdx.x;
+        return (t + 256 * k) / CH;
     }
-}
+    static __device__ __forceinline__ int channel() { return threadIdx.x % CH; }
+    __device__ __forceinline__ void fetch(const ScanArgs& a, const Place<LN>& p, int64_t t0)
+    {
+        const int dd = p.ch0 + min(channel(), p.nch - 1);
+#pragma unroll
+        for (int k = 0; k < PT; k++) {
+            const int64_t at = t0 + row(k) < p.r1 ? t0 + row(k) : p.r1 - 1;
+            d[k] = ((const T*)a.delta + at * a.delta_stride)[dd];
+            if (U) u[k] = ((const T*)a.u + at * a.u_stride)[dd];
+            if (Z) z[k] = ((const T*)(a.z ? a.z : a.u) + at * (a.z ? a.z_stride : a.u_stride))[dd];
+            if (DY) g[k] = ((const T*)a.dy + at * a.dy_stride)[dd];
+        }
+#pragma unroll
+        for (int k = 0; k < NB; k++) {
+            const int i = threadIdx.x + 256 * k, n = i % NP < a.states ? i % NP : a.states - 1;
+            const int64_t r = t0 + i / NP % TT, at = r < p.r1 ? r : p.r1 - 1;
+            if (GB) b[k] = ((const T*)a.B + at * a.B_stride)[p.g * a.states + n];
+            if (GC) c[k] = ((const T*)a.C + at * a.C_stride)[p.g * a.states + n];
+        }
+    }
+    // B and C of rows [lo, hi)
+    __device__ __forceinline__ void stage_groups(const ScanArgs& a, int64_t t0, int64_t lo, int64_t hi, float (*sB)[NP], float (*sC)[NP])
+    {
+#pragma unroll
+        for (int k = 0; k < NB; k++) {
+            const int i = threadIdx.x + 256 * k, r = i / NP, n = i % NP;
+            const bool counts = n < a.states && t0 + r >= lo && t0 + r < hi;
+            if (TT * NP < 256 && r >= TT) continue;
+            if (GB) sB[r][n] = counts ? to_f32(b[k]) : 0.0f;
+            if (GC) sC[r][n] = counts ? to_f32(c[k]) : 0.0f;
+        }
+    }
+};
 
 // first pass: the state a chunk's last history has at the chunk's end, for a state of zero in front of the chunk
 template <class T, int LN>
@@ -102,41 +169,43 @@ __global__ __launch_bounds__(256) void scan_local_kernel(ScanArgs a)
     if (!goes_on) return;
     const int64_t from = begin > p.r0 ? begin : p.r0;
     float A2[4], h[4], span = 0.0f;
-    load_states(a.A, 0, a, p.d, p.lane_n, p.on, A2);
+    load_states<LN>(a.A, 0, a, p.d, p.lane_n, p.on, A2);
 #pragma unroll
     for (int e = 0; e < 4; e++) A2[e] *= REC_LOG2E;
-    load_states(begin >= p.r0 ? a.initial : nullptr, s, a, p.d, p.lane_n, p.on, h);
+    load_states<LN>(begin >= p.r0 ? a.initial : nullptr, s, a, p.d, p.lane_n, p.on, h);
+    Tile<T, LN, true, false, false, true, false> t;
+    const int ch = t.channel();
+    const bool mine = ch < p.nch;
+    const float bias = mine && a.delta_bias ? a.delta_bias[p.ch0 + ch] : 0.0f;
+    t.fetch(a, p, from);
     for (int64_t t0 = from; t0 < p.r1; t0 += TT) {
-        const int nt = (int)(p.r1 - t0 < TT ? p.r1 - t0 : TT);
         __syncthreads();
-        for (int i = threadIdx.x; i < TT * CH; i += 256) {
-            const int r = i / CH, c = i % CH;
-            float2 v = make_float2(0.0f, 0.0f);
-            if (r < nt && c < p.nch) {
-                float raw;
-                v.x = delta_of<T>(a, t0 + r, p.ch0 + c, raw);
-                v.y = v.x * to_f32(((const T*)a.u)[(t0 + r) * a.u_stride + p.ch0 + c]);
-            }
-            sd[r][c] = v;
+#pragma unroll
+        for (int k = 0; k < t.PT; k++) {
+            const bool counts = mine && t0 + t.row(k) < p.r1;
+            const float raw = to_f32(t.d[k]) + bias, sp = computed(softplus_f32(raw)), delta = a.softplus ? sp : raw;
+            sd[t.row(k)][ch] = counts ? make_float2(delta, delta * to_f32(t.u[k])) : make_float2(0.0f, 0.0f);
         }
-        stage_group<T, NP>(a.B, a.B_stride, a, p.g, t0, t0, t0 + nt, sB);
+        t.stage_groups(a, t0, t0, p.r1, sB, nullptr);
         __syncthreads();
-        for (int r = 0; r < nt; r++) {
+        if (t0 + TT < p.r1) t.fetch(a, p, t0 + TT);
+#pragma unroll
+        for (int r = 0; r < TT; r++) {   // rows behind the chunk's last move nothing: exp(0) and 0
             const float2 v = sd[r][p.ch];
             span += v.x;
 #pragma unroll
             for (int e = 0; e < 4; e++) h[e] = fmaf(fast_exp2(v.x * A2[e]), h[e], v.y * sB[r][p.lane_n + e]);
         }
     }
-    store_states(a.link, p.chunk + 1, a, p.d, p.lane_n, p.on, h);
+    store_states<LN>(a.link, p.chunk + 1, a, p.d, p.lane_n, p.on, h);
     if (p.on && p.lane_n == 0) a.span[(int64_t)p.chunk * a.channels + p.d] = span;
 }
 
 // second pass: the state handed into chunk c + 1 is exp(A span) of what was handed into c (where c's history came from there), plus
-// what c adds.  Such steps compose, so 32 threads share the chunks of a channel's state: each composes a run of them, then
+// what c adds.  Such steps compose, so 64 threads share the chunks of a channel's state: each composes a run of them, then
 // walks it again from what the runs in front of it lead to.  (One thread after the other's loads took 0.3 us per chunk.)
 // The gradient takes the same steps from the back.
-constexpr int LINK_COLS = 16, LINK_RUNS = 32;
+constexpr int LINK_COLS = 16, LINK_RUNS = 64;
 template <bool BACK>
 __global__ __launch_bounds__(LINK_COLS * LINK_RUNS) void scan_link_kernel(ScanArgs a)
 {
@@ -176,23 +245,18 @@ __global__ __launch_bounds__(LINK_COLS * LINK_RUNS) void scan_link_kernel(ScanAr
     }
 }
 
-// What a thread stages of a tile: PT (row, channel) pairs, 256 apart
-template <class T, int LN> struct Pairs {
-    static constexpr int CH = 256 / LN, PT = TT * CH / 256;
-    static __device__ __forceinline__ int row(int k) { return (threadIdx.x + 256 * k) / CH; }
-    static __device__ __forceinline__ int channel() { return threadIdx.x % CH; }   // the same for all of a thread's pairs
-};
-
-// one value per row of a group of LN rows, summed over a channel's lanes: lane j of them keeps row j's
-template <int LN> __device__ __forceinline__ float sums_of_rows(const float (&v)[LN])
+// Sums over a channel's lanes are taken for GR rows together: lane j < GR of the channel keeps, and writes, row j's.
+template <int LN> constexpr int rows_together() { return LN < 4 ? LN : 4; }
+template <int LN, int GR> __device__ __forceinline__ void write_sums(float (*to)[256 / LN + 16], int r, int ch, const float (&v)[GR])
 {
+    const int j = threadIdx.x % LN;
     float mine = group_sum_dpp<LN>(v[0]);
 #pragma unroll
-    for (int k = 1; k < LN; k++) {
+    for (int k = 1; k < GR; k++) {
         const float s = group_sum_dpp<LN>(v[k]);
-        mine = (int)(threadIdx.x % LN) == k ? s : mine;
+        mine = j == k ? s : mine;
     }
-    return mine;
+    if (GR == LN || j < GR) to[r + j][ch] = mine;
 }
 
 // third pass
@@ -200,61 +264,44 @@ template <class T, int LN>
 __global__ __launch_bounds__(256) void scan_forward_kernel(ScanArgs a)
 {
     using P = Place<LN>;
-    using Q = Pairs<T, LN>;
-    constexpr int CH = P::CH, NP = 4 * LN, PT = Q::PT;
+    constexpr int CH = P::CH, NP = 4 * LN, GR = rows_together<LN>();
     __shared__ float2 sd[TT][CH];
-    __shared__ alignas(16) float sB[TT][NP], sC[TT][NP], sy[TT][CH + 16];   // rows of sy 16 banks apart: LN rows are written at once
+    __shared__ alignas(16) float sB[TT][NP], sC[TT][NP], sy[TT][CH + 16];   // rows of sy 16 banks apart: GR rows are written at once
     const P p(a);
     const int64_t lo = a.off[0], hi = a.off[a.n_seq];
     SeqCursor c;
     c.begin(a.off, a.n_seq, p.r0);
     float A2[4], h[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    load_states(a.A, 0, a, p.d, p.lane_n, p.on, A2);
+    load_states<LN>(a.A, 0, a, p.d, p.lane_n, p.on, A2);
 #pragma unroll
     for (int e = 0; e < 4; e++) A2[e] *= REC_LOG2E;
     if (c.inside(a.n_seq)) {
-        if (a.off[c.s] >= p.r0) load_states(a.initial, c.s, a, p.d, p.lane_n, p.on, h);
-        else if (p.chunk > 0) load_states(a.link, p.chunk, a, p.d, p.lane_n, p.on, h);
+        if (a.off[c.s] >= p.r0) load_states<LN>(a.initial, c.s, a, p.d, p.lane_n, p.on, h);
+        else if (p.chunk > 0) load_states<LN>(a.link, p.chunk, a, p.d, p.lane_n, p.on, h);
     }
-    const int ch = Q::channel(), d = p.ch0 + ch;
+    Tile<T, LN, true, true, false, true, true> t;
+    constexpr int PT = decltype(t)::PT;
+    const int ch = t.channel(), d = p.ch0 + ch;
     const bool mine = ch < p.nch;
     const float bias = mine && a.delta_bias ? a.delta_bias[d] : 0.0f, Dd = mine && a.D ? a.D[d] : 0.0f;
-    T rd[PT], ru[PT], rz[PT];   // the next tile's, loaded while this one is walked
-    auto fetch = [&](int64_t t0) {
-#pragma unroll
-        for (int k = 0; k < PT; k++) {
-            const int64_t row = t0 + Q::row(k);
-            rd[k] = ru[k] = rz[k] = (T)0.0f;
-            if (mine && row < p.r1) {
-                rd[k] = ((const T*)a.delta)[row * a.delta_stride + d];
-                ru[k] = ((const T*)a.u)[row * a.u_stride + d];
-                if (a.z) rz[k] = ((const T*)a.z)[row * a.z_stride + d];
-            }
-        }
-    };
-    fetch(p.r0);
+    t.fetch(a, p, p.r0);
     for (int64_t t0 = p.r0; t0 < p.r1; t0 += TT) {
         const int nt = (int)(p.r1 - t0 < TT ? p.r1 - t0 : TT);
-        float u[PT], z[PT];
+        const int64_t blo = lo > t0 ? lo : t0, bhi = hi < t0 + nt ? hi : t0 + nt;   // a row of no history moves nothing
+        float u[PT], gate[PT];
 #pragma unroll
         for (int k = 0; k < PT; k++) {
-            const int64_t row = t0 + Q::row(k);
-            u[k] = to_f32(ru[k]);
-            z[k] = to_f32(rz[k]);
-            float2 v = make_float2(0.0f, 0.0f);   // a row of no history moves nothing
-            if (mine && row >= lo && row < hi && row < p.r1) {
-                const float raw = to_f32(rd[k]) + bias;
-                v.x = a.softplus ? softplus_f32(raw) : raw;
-                v.y = v.x * u[k];
-            }
-            sd[Q::row(k)][ch] = v;
+            const int64_t row = t0 + t.row(k);
+            u[k] = to_f32(t.u[k]);
+            gate[k] = computed(silu_f32(to_f32(t.z[k])));
+            gate[k] = a.z ? gate[k] : 1.0f;
+            const float raw = to_f32(t.d[k]) + bias, sp = computed(softplus_f32(raw)), delta = a.softplus ? sp : raw;
+            sd[t.row(k)][ch] = mine && row >= blo && row < bhi ? make_float2(delta, delta * u[k]) : make_float2(0.0f, 0.0f);
         }
-        const int64_t blo = lo > t0 ? lo : t0, bhi = hi < t0 + nt ? hi : t0 + nt;
-        stage_group<T, NP>(a.B, a.B_stride, a, p.g, t0, blo, bhi, sB);
-        stage_group<T, NP>(a.C, a.C_stride, a, p.g, t0, blo, bhi, sC);
+        t.stage_groups(a, t0, blo, bhi, sB, sC);
         __syncthreads();
-        if (t0 + TT < p.r1) fetch(t0 + TT);
-        if (a.checkpoints) store_states(a.checkpoints, t0 / TT, a, p.d, p.lane_n, p.on, h);
+        if (t0 + TT < p.r1) t.fetch(a, p, t0 + TT);
+        if (a.checkpoints) store_states<LN>(a.checkpoints, t0 / TT, a, p.d, p.lane_n, p.on, h);
         auto step = [&](int r) {
             const float2 v = sd[r][p.ch];
             float y = 0.0f;
@@ -267,28 +314,28 @@ __global__ __launch_bounds__(256) void scan_forward_kernel(ScanArgs a)
         };
         if (nt == TT && t0 + TT < c.next) {   // no history begins or ends here
 #pragma unroll
-            for (int r = 0; r < TT; r += LN) {
-                float y[LN];
+            for (int r = 0; r < TT; r += GR) {
+                float y[GR];
 #pragma unroll
-                for (int k = 0; k < LN; k++) y[k] = step(r + k);
-                sy[r + threadIdx.x % LN][p.ch] = sums_of_rows<LN>(y);
+                for (int k = 0; k < GR; k++) y[k] = step(r + k);
+                write_sums<LN, GR>(sy, r, p.ch, y);
             }
         } else {
             for (int r = 0; r < nt; r++) {
                 const int64_t row = t0 + r;
                 if (row >= c.next) {
                     c.advance(a.off, a.n_seq, row);
-                    load_states(c.inside(a.n_seq) ? a.initial : nullptr, c.s, a, p.d, p.lane_n, p.on, h);
+                    load_states<LN>(c.inside(a.n_seq) ? a.initial : nullptr, c.s, a, p.d, p.lane_n, p.on, h);
                 }
                 const float y = group_sum_dpp<LN>(step(r));
                 if (p.lane_n == 0) sy[r][p.ch] = y;
-                if (a.final_state && row + 1 == c.next && c.inside(a.n_seq)) store_states(a.final_state, c.s, a, p.d, p.lane_n, p.on, h);
+                if (a.final_state && row + 1 == c.next && c.inside(a.n_seq)) store_states<LN>(a.final_state, c.s, a, p.d, p.lane_n, p.on, h);
             }
         }
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < PT; k++) {
-            const int r = Q::row(k);
+            const int r = t.row(k);
             const int64_t row = t0 + r;
             if (r >= nt || !mine) continue;
             T* y = (T*)a.y + row * a.y_stride + d;
@@ -298,8 +345,7 @@ __global__ __launch_bounds__(256) void scan_forward_kernel(ScanArgs a)
             }
             float v = sy[r][ch];
             if (a.D) v = fmaf(Dd, u[k], v);
-            if (a.z) v *= silu_f32(z[k]);
-            *y = from_f32<T>(v);
+            *y = from_f32<T>(v * gate[k]);
         }
     }
 }
@@ -333,46 +379,55 @@ __global__ __launch_bounds__(256) void scan_local_backward_kernel(ScanArgs a)
     if (!came) return;
     const int64_t to = end < p.r1 ? end : p.r1;
     float A2[4], g[4], span = 0.0f;
-    load_states(a.A, 0, a, p.d, p.lane_n, p.on, A2);
+    load_states<LN>(a.A, 0, a, p.d, p.lane_n, p.on, A2);
 #pragma unroll
     for (int e = 0; e < 4; e++) A2[e] *= REC_LOG2E;
-    load_states(end <= p.r1 ? a.dfinal : nullptr, s, a, p.d, p.lane_n, p.on, g);
-    for (int64_t t1 = to; t1 > p.r0; t1 -= TT) {
-        const int64_t t0 = t1 - TT > p.r0 ? t1 - TT : p.r0;
-        const int nt = (int)(t1 - t0);
+    load_states<LN>(end <= p.r1 ? a.dfinal : nullptr, s, a, p.d, p.lane_n, p.on, g);
+    Tile<T, LN, false, true, true, false, true> t;
+    const int ch = t.channel();
+    const bool mine = ch < p.nch;
+    const float bias = mine && a.delta_bias ? a.delta_bias[p.ch0 + ch] : 0.0f;
+    int64_t t0 = p.r0 + (to - 1 - p.r0) / TT * TT;
+    t.fetch(a, p, t0);
+    for (; t0 >= p.r0; t0 -= TT) {
         __syncthreads();
-        for (int i = threadIdx.x; i < TT * CH; i += 256) {
-            const int r = i / CH, c = i % CH;
-            float2 v = make_float2(0.0f, 0.0f);
-            if (r < nt && c < p.nch) {
-                float raw;
-                v.x = delta_of<T>(a, t0 + r, p.ch0 + c, raw);
-                v.y = to_f32(((const T*)a.dy)[(t0 + r) * a.dy_stride + p.ch0 + c]);
-                if (a.z) v.y *= silu_f32(to_f32(((const T*)a.z)[(t0 + r) * a.z_stride + p.ch0 + c]));
-            }
-            sd[r][c] = v;
+#pragma unroll
+        for (int k = 0; k < t.PT; k++) {
+            const bool counts = mine && t0 + t.row(k) < to;
+            const float raw = to_f32(t.d[k]) + bias, sp = computed(softplus_f32(raw)), delta = a.softplus ? sp : raw, gy = to_f32(t.g[k]), gate = computed(silu_f32(to_f32(t.z[k])));
+            sd[t.row(k)][ch] = counts ? make_float2(delta, a.z ? gy * gate : gy) : make_float2(0.0f, 0.0f);
         }
-        stage_group<T, NP>(a.C, a.C_stride, a, p.g, t0, t0, t0 + nt, sC);
+        t.stage_groups(a, t0, t0, to, nullptr, sC);
         __syncthreads();
-        for (int r = nt - 1; r >= 0; r--) {
+        if (t0 > p.r0) t.fetch(a, p, t0 - TT);
+#pragma unroll
+        for (int r = TT - 1; r >= 0; r--) {   // rows behind the history's last move nothing
             const float2 v = sd[r][p.ch];
             span += v.x;
 #pragma unroll
             for (int e = 0; e < 4; e++) g[e] = fast_exp2(v.x * A2[e]) * fmaf(sC[r][p.lane_n + e], v.y, g[e]);
         }
     }
-    store_states(a.link, p.chunk, a, p.d, p.lane_n, p.on, g);
+    store_states<LN>(a.link, p.chunk, a, p.d, p.lane_n, p.on, g);
     if (p.on && p.lane_n == 0) a.span[(int64_t)p.chunk * a.channels + p.d] = span;
 }
 
+// What is staged in LDS is read again behind this line: without it the compiler keeps all that the walk forwards has read
+// (160 registers) for the walk backwards.
+#define REC_READ_AGAIN()                          \
+    do {                                          \
+        asm volatile("" ::: "memory");            \
+        __builtin_amdgcn_sched_barrier(0);        \
+    } while (0)
+
 // third pass: per 16 rows, the states again from the checkpoint in front of them, then the gradient backwards.  A lane keeps the
-// tile's states and decays in registers (128 of them), which is cheaper than the 64 exps it would take to have the decays again.
+// tile's states in registers (64 of them).  Keeping the decays as well left room for one wavefront per SIMD instead of three.
 template <class T, int LN>
-__global__ __launch_bounds__(256) void scan_backward_kernel(ScanArgs a)
+__global__ __launch_bounds__(256, 2) void scan_backward_kernel(ScanArgs a)
 {
     using P = Place<LN>;
-    using Q = Pairs<T, LN>;
-    constexpr int CH = P::CH, NP = 4 * LN, PT = Q::PT, ROW = CH + 16;
+    using Q = Tile<T, LN, true, true, true, true, true>;
+    constexpr int CH = P::CH, NP = 4 * LN, PT = Q::PT, ROW = CH + 16, GR = rows_together<LN>();
     __shared__ float2 sd[TT][CH];                  // delta, delta * u
     __shared__ float sg[TT][CH];                   // dys
     __shared__ alignas(16) float sB[TT][NP], sC[TT][NP];
@@ -380,16 +435,16 @@ __global__ __launch_bounds__(256) void scan_backward_kernel(ScanArgs a)
     __shared__ alignas(16) float s_bc[4][TT][2][NP];           // dB, dC of each wavefront's channels
     const P p(a);
     const int64_t lo = a.off[0], hi = a.off[a.n_seq];
-    float A[4], A2[4], G[4] = {0.0f, 0.0f, 0.0f, 0.0f}, dA[4] = {0.0f, 0.0f, 0.0f, 0.0f}, dD = 0.0f, dbias = 0.0f;
-    load_states(a.A, 0, a, p.d, p.lane_n, p.on, A);
+    float A2[4], G[4] = {0.0f, 0.0f, 0.0f, 0.0f}, dA[4] = {0.0f, 0.0f, 0.0f, 0.0f}, dD = 0.0f, dbias = 0.0f;
+    load_states<LN>(a.A, 0, a, p.d, p.lane_n, p.on, A2);
 #pragma unroll
-    for (int e = 0; e < 4; e++) A2[e] = A[e] * REC_LOG2E;
+    for (int e = 0; e < 4; e++) A2[e] *= REC_LOG2E;
     // the sequence (n_seq: none) of the row at hand, walking backwards, and its first row
     int s = sequence_of(a.off, a.n_seq, p.r1 - 1);
     int64_t begin = s >= 0 ? a.off[s] : -1;
     if (s >= 0 && s < a.n_seq) {
-        if (a.off[s + 1] <= p.r1) load_states(a.dfinal, s, a, p.d, p.lane_n, p.on, G);
-        else if (p.chunk + 1 < a.chunks) load_states(a.link, p.chunk + 1, a, p.d, p.lane_n, p.on, G);
+        if (a.off[s + 1] <= p.r1) load_states<LN>(a.dfinal, s, a, p.d, p.lane_n, p.on, G);
+        else if (p.chunk + 1 < a.chunks) load_states<LN>(a.link, p.chunk + 1, a, p.d, p.lane_n, p.on, G);
     }
     auto step_back = [&](int& q, int64_t& b) {   // to the sequence in front, past empty ones
         const int64_t at = b;
@@ -409,109 +464,113 @@ __global__ __launch_bounds__(256) void scan_backward_kernel(ScanArgs a)
             if (b == t0) break;
             step_back(s0, b);
         }
+        Q t;
+        t.fetch(a, p, t0);
+        float h0[4];   // the state in front of the tile
+        load_states<LN>(a.checkpoints_in, t0 / TT, a, p.d, p.lane_n, p.on, h0);
+        const int64_t blo = lo > t0 ? lo : t0, bhi = hi < t0 + nt ? hi : t0 + nt;
         __syncthreads();
-        float raw[PT], u[PT], zz[PT], gy[PT];
+        float u[PT], dsp[PT], dgate[PT];   // u, the derivative of softplus, dy times the derivative of the gate
 #pragma unroll
         for (int k = 0; k < PT; k++) {
             const int r = Q::row(k);
-            const int64_t row = t0 + r;
-            float2 v = make_float2(0.0f, 0.0f);
-            raw[k] = u[k] = zz[k] = gy[k] = 0.0f;
-            float ys = 0.0f;
-            if (mine && r < nt && row >= lo && row < hi) {
-                raw[k] = to_f32(((const T*)a.delta)[row * a.delta_stride + d]) + bias;
-                u[k] = to_f32(((const T*)a.u)[row * a.u_stride + d]);
-                gy[k] = to_f32(((const T*)a.dy)[row * a.dy_stride + d]);
-                if (a.z) zz[k] = to_f32(((const T*)a.z)[row * a.z_stride + d]);
-                v.x = a.softplus ? softplus_f32(raw[k]) : raw[k];
-                v.y = v.x * u[k];
-                ys = a.z ? gy[k] * silu_f32(zz[k]) : gy[k];
-            }
-            sd[r][ch] = v;
-            sg[r][ch] = ys;
+            const bool counts = mine && t0 + r >= blo && t0 + r < bhi;
+            const float raw = to_f32(t.d[k]) + bias, gy = to_f32(t.g[k]), z = to_f32(t.z[k]);
+            const float sp = computed(softplus_f32(raw)), ss = computed(sigmoid_f32(raw)), sz = computed(sigmoid_f32(z));
+            const float delta = a.softplus ? sp : raw;
+            u[k] = to_f32(t.u[k]);
+            dsp[k] = a.softplus ? ss : 1.0f;
+            dgate[k] = gy * (sz * fmaf(z, 1.0f - sz, 1.0f));
+            sd[r][ch] = counts ? make_float2(delta, delta * u[k]) : make_float2(0.0f, 0.0f);
+            sg[r][ch] = counts ? (a.z ? gy * (z * sz) : gy) : 0.0f;
         }
-        const int64_t blo = lo > t0 ? lo : t0, bhi = hi < t0 + nt ? hi : t0 + nt;
-        stage_group<T, NP>(a.B, a.B_stride, a, p.g, t0, blo, bhi, sB);
-        stage_group<T, NP>(a.C, a.C_stride, a, p.g, t0, blo, bhi, sC);
+        t.stage_groups(a, t0, blo, bhi, sB, sC);
         __syncthreads();
-        float h0[4], hs[TT][4], ea[TT][4];   // the state in front of the tile, behind each row, and each row's decay
-        load_states(a.checkpoints_in, t0 / TT, a, p.d, p.lane_n, p.on, h0);
-        if (bounds & 1) load_states(s0 >= 0 && s0 < a.n_seq ? a.initial : nullptr, s0, a, p.d, p.lane_n, p.on, h0);
+        // A tile in which no history begins is walked without a look at the bounds: one stretch of code, in which the reads of the
+        // rows ahead are in flight.
+        auto walk = [&](auto bounded) {
+            constexpr bool BOUNDED = decltype(bounded)::value;
+            float hs[TT][4];   // the state behind each row
+            if (BOUNDED && (bounds & 1)) load_states<LN>(s0 >= 0 && s0 < a.n_seq ? a.initial : nullptr, s0, a, p.d, p.lane_n, p.on, h0);
 #pragma unroll
-        for (int r0 = 0; r0 < TT; r0 += LN) {
-            float y[LN];
+            for (int r0 = 0; r0 < TT; r0 += GR) {
+                float y[GR];
 #pragma unroll
-            for (int k = 0; k < LN; k++) {
-                const int r = r0 + k;
-                float h[4];
+                for (int k = 0; k < GR; k++) {
+                    const int r = r0 + k;
+                    if (r % 4 == 0) REC_READ_AGAIN();
+                    float h[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) h[e] = r == 0 ? h0[e] : hs[r > 0 ? r - 1 : 0][e];
-                if (r > 0 && ((bounds >> r) & 1)) {
-                    s0 = sequence_of(a.off, a.n_seq, t0 + r);
-                    load_states(s0 >= 0 && s0 < a.n_seq ? a.initial : nullptr, s0, a, p.d, p.lane_n, p.on, h);
+                    for (int e = 0; e < 4; e++) h[e] = r == 0 ? h0[e] : hs[r > 0 ? r - 1 : 0][e];
+                    if (BOUNDED && r > 0 && ((bounds >> r) & 1)) {
+                        if (a.initial)
+                            do s0++; while (s0 < a.n_seq && a.off[s0 + 1] <= t0 + r);
+                        load_states<LN>(s0 >= 0 && s0 < a.n_seq ? a.initial : nullptr, s0, a, p.d, p.lane_n, p.on, h);
+                    }
+                    const float2 v = sd[r][p.ch];
+                    y[k] = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        hs[r][e] = fmaf(fast_exp2(v.x * A2[e]), h[e], v.y * sB[r][p.lane_n + e]);
+                        y[k] = fmaf(hs[r][e], sC[r][p.lane_n + e], y[k]);
+                    }
                 }
+                if (a.z) write_sums<LN, GR>(s_in, r0, p.ch, y);
+            }
+            float vB[2][4], vC[2][4], gB[GR], qA[GR];
+#pragma unroll
+            for (int r = TT - 1; r >= 0; r--) {
+                if (r % 2 == 1) REC_READ_AGAIN();
                 const float2 v = sd[r][p.ch];
-                y[k] = 0.0f;
+                const float ys = sg[r][p.ch];
+                float hb[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) hb[e] = r == 0 ? h0[e] : hs[r > 0 ? r - 1 : 0][e];
+                const bool bound = BOUNDED && ((bounds >> r) & 1);
+                if (r > 0 && bound) load_states<LN>(s >= 0 && s < a.n_seq ? a.initial : nullptr, s, a, p.d, p.lane_n, p.on, hb);
+                gB[r % GR] = qA[r % GR] = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    ea[r][e] = fast_exp2(v.x * A2[e]);
-                    hs[r][e] = fmaf(ea[r][e], h[e], v.y * sB[r][p.lane_n + e]);
-                    y[k] = fmaf(hs[r][e], sC[r][p.lane_n + e], y[k]);
+                    const float b = sB[r][p.lane_n + e];
+                    const float g = fmaf(sC[r][p.lane_n + e], ys, G[e]);
+                    vB[r % 2][e] = g * v.y;
+                    vC[r % 2][e] = hs[r][e] * ys;
+                    gB[r % GR] = fmaf(g, b, gB[r % GR]);
+                    G[e] = fast_exp2(v.x * A2[e]) * g;
+                    const float q = G[e] * hb[e];
+                    qA[r % GR] = fmaf(q, A2[e], qA[r % GR]);   // (A, times ln 2 below)
+                    dA[e] = fmaf(q, v.x, dA[e]);
+                }
+                if (bound) {   // in front of this row another sequence ends, or none does
+                    if (s >= 0 && s < a.n_seq && a.dinitial) store_states<LN>(a.dinitial, s, a, p.d, p.lane_n, p.on, G);
+                    step_back(s, begin);
+                    load_states<LN>(s >= 0 ? a.dfinal : nullptr, s, a, p.d, p.lane_n, p.on, G);
+                }
+                if (r % GR == 0) {
+                    write_sums<LN, GR>(s_gB, r, p.ch, gB);
+                    write_sums<LN, GR>(s_qA, r, p.ch, qA);
+                }
+                if (r % 2 == 0) {
+                    // Two rows' 16 values, over the wavefront's channels: each fold halves the values and leaves the halves of the
+                    // lanes with different ones (bit 5 of the lane: the row, bit 4: dB or dC); what is left is summed inside 16 lanes.
+                    float w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) w[e] = row_sum_strided<LN>(fold16(fold32(vB[0][e], vB[1][e]), fold32(vC[0][e], vC[1][e])));
+                    float* to = s_bc[wave][r + (lane >> 5)][(lane >> 4) & 1] + p.lane_n;
+                    const int copy = lane % 16 / LN;   // lanes with the same sums
+                    if constexpr (LN <= 4) {
+                        const float mine4 = copy == 0 ? w[0] : copy == 1 ? w[1] : copy == 2 ? w[2] : w[3];
+                        if (copy < 4) to[copy] = mine4;
+                    } else if constexpr (LN == 8) {
+                        *reinterpret_cast<float2*>(to + 2 * copy) = copy ? make_float2(w[2], w[3]) : make_float2(w[0], w[1]);
+                    } else {
+                        *reinterpret_cast<float4*>(to) = make_float4(w[0], w[1], w[2], w[3]);
+                    }
                 }
             }
-            if (a.z) s_in[r0 + threadIdx.x % LN][p.ch] = sums_of_rows<LN>(y);
-        }
-        float vB[2][4], vC[2][4], gB[LN], qA[LN];
-#pragma unroll
-        for (int r = TT - 1; r >= 0; r--) {
-            const float2 v = sd[r][p.ch];
-            const float ys = sg[r][p.ch];
-            float hb[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) hb[e] = r == 0 ? h0[e] : hs[r > 0 ? r - 1 : 0][e];
-            const bool bound = (bounds >> r) & 1;
-            if (r > 0 && bound) load_states(s >= 0 && s < a.n_seq ? a.initial : nullptr, s, a, p.d, p.lane_n, p.on, hb);
-            gB[r % LN] = qA[r % LN] = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float b = sB[r][p.lane_n + e];
-                const float g = fmaf(sC[r][p.lane_n + e], ys, G[e]);
-                vB[r % 2][e] = g * v.y;
-                vC[r % 2][e] = hs[r][e] * ys;
-                gB[r % LN] = fmaf(g, b, gB[r % LN]);
-                G[e] = ea[r][e] * g;
-                const float q = G[e] * hb[e];
-                qA[r % LN] = fmaf(q, A[e], qA[r % LN]);
-                dA[e] = fmaf(q, v.x, dA[e]);
-            }
-            if (bound) {   // in front of this row another sequence ends, or none does
-                if (s >= 0 && s < a.n_seq && a.dinitial) store_states(a.dinitial, s, a, p.d, p.lane_n, p.on, G);
-                step_back(s, begin);
-                load_states(s >= 0 ? a.dfinal : nullptr, s, a, p.d, p.lane_n, p.on, G);
-            }
-            if (r % LN == 0) {
-                const int at = r + threadIdx.x % LN;
-                s_gB[at][p.ch] = sums_of_rows<LN>(gB);
-                s_qA[at][p.ch] = sums_of_rows<LN>(qA);
-            }
-            if (r % 2 == 0) {
-                // Two rows' 16 values, over the wavefront's channels: each fold halves the values and leaves the halves of the
-                // lanes with different ones (bit 5 of the lane: the row, bit 4: dB or dC); what is left is summed inside 16 lanes.
-                float w[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) w[e] = row_sum_strided<LN>(fold16(fold32(vB[0][e], vB[1][e]), fold32(vC[0][e], vC[1][e])));
-                float* to = s_bc[wave][r + (lane >> 5)][(lane >> 4) & 1] + p.lane_n;
-                const int copy = lane % 16 / LN;   // lanes with the same sums
-                if constexpr (LN <= 4) {
-                    const float mine4 = copy == 0 ? w[0] : copy == 1 ? w[1] : copy == 2 ? w[2] : w[3];
-                    if (copy < 4) to[copy] = mine4;
-                } else if constexpr (LN == 8) {
-                    *reinterpret_cast<float2*>(to + 2 * copy) = copy ? make_float2(w[2], w[3]) : make_float2(w[0], w[1]);
-                } else {
-                    *reinterpret_cast<float4*>(to) = make_float4(w[0], w[1], w[2], w[3]);
-                }
-            }
-        }
+        };
+        if (bounds == 0) walk(std::false_type{});
+        else walk(std::true_type{});
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < PT; k++) {
@@ -527,11 +586,10 @@ __global__ __launch_bounds__(256) void scan_backward_kernel(ScanArgs a)
             }
             const float2 v = sd[r][ch];
             const float ys = sg[r][ch], g = s_gB[r][ch];
-            float dd = fmaf(u[k], g, s_qA[r][ch]);
-            if (a.softplus) dd *= sigmoid_f32(raw[k]);
+            const float dd = fmaf(u[k], g, s_qA[r][ch] * 0.69314718055994530942f) * dsp[k];
             ((T*)a.du)[at] = from_f32<T>(a.D ? fmaf(v.x, g, Dd * ys) : v.x * g);
             ((T*)a.ddelta)[at] = from_f32<T>(dd);
-            if (a.z) ((T*)a.dz)[at] = from_f32<T>(gy[k] * (a.D ? fmaf(Dd, u[k], s_in[r][ch]) : s_in[r][ch]) * dsilu_f32(zz[k]));
+            if (a.z) ((T*)a.dz)[at] = from_f32<T>(dgate[k] * (a.D ? fmaf(Dd, u[k], s_in[r][ch]) : s_in[r][ch]));
             dD = fmaf(ys, u[k], dD);
             dbias += dd;
         }
@@ -550,7 +608,7 @@ __global__ __launch_bounds__(256) void scan_backward_kernel(ScanArgs a)
     }
     if (!a.part_a) return;
     float* part = a.part_a + (int64_t)p.chunk * (a.channels * a.states + 2 * a.channels);
-    store_states(part, 0, a, p.d, p.lane_n, p.on, dA);
+    store_states<LN>(part, 0, a, p.d, p.lane_n, p.on, dA);
     // a thread's pairs are of one channel: the threads of a channel in order
     __syncthreads();
     float *red_D = &s_in[0][0], *red_b = &s_gB[0][0];   // 16 * CH >= 256 each
@@ -597,12 +655,12 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a, const int32_
     }
     if (earlier) return;
     float A2[4];
-    load_states(a.A, 0, a, d, n0, true, A2);
+    load_states<LN>(a.A, 0, a, d, n0, true, A2);
 #pragma unroll
     for (int e = 0; e < 4; e++) A2[e] *= REC_LOG2E;
     auto click = [&](int64_t r) {   // the state goes through memory, so that rows of a shared slot are steps like any other
         float h[4], raw, y = 0.0f;
-        load_states(state, slot, a, d, n0, true, h);
+        load_states<LN>(state, slot, a, d, n0, true, h);
         const float delta = delta_of<T>(a, r, d, raw), u = to_f32(((const T*)a.u)[r * a.u_stride + d]);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -612,7 +670,7 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a, const int32_
             h[e] = fmaf(fast_exp2(delta * A2[e]), h[e], delta * u * b);
             y = fmaf(h[e], c, y);
         }
-        store_states(state, slot, a, d, n0, true, h);
+        store_states<LN>(state, slot, a, d, n0, true, h);
         y = group_sum_dpp<LN>(y);
         if (n0 == 0) {
             if (a.D) y = fmaf(a.D[d], u, y);
@@ -668,17 +726,18 @@ RowsOf channel_rows(const rec_scan_desc* d, const void* p, int64_t stride)
 
 int lanes_of(int states) { return states <= 4 ? 1 : states <= 8 ? 2 : states <= 16 ? 4 : states <= 32 ? 8 : 16; }
 
-// How the rows are cut.  A walk of one row takes a block about 0.1 us whatever else runs, a chunk more costs its first pass (two
-// thirds of the third) and a state handed over; so chunks are as long as they can be while the launch still has about
-// eight blocks per compute unit, between 32 and 512 rows.
+// How the rows are cut.  A chunk more costs its first pass (two thirds of the third, over the chunk's last history) and a state
+// handed over, so chunks are as long as they can be while the launch still fills the chip: `blocks` of them, between 32 and
+// 512 rows.
 struct Cut { int tiles_per_group, tiles, chunk, chunks; };
-Cut cut_of(const rec_scan_desc* d)
+constexpr int kForwardBlocks = 2048, kBackwardBlocks = 2048;
+Cut cut_of(const rec_scan_desc* d, int blocks)
 {
     Cut c;
     const int ch = 256 / lanes_of(d->states), per = d->channels / d->groups;
     c.tiles_per_group = (per + ch - 1) / ch;
     c.tiles = c.tiles_per_group * d->groups;
-    int64_t rows = d->rows * c.tiles / 1024 / TT * TT;
+    int64_t rows = d->rows * c.tiles / blocks / TT * TT;
     if (rows < 32) rows = 32;
     if (rows > 512) rows = 512;
     c.chunk = (int)rows;
@@ -727,7 +786,7 @@ int check_workspace(const void* p, int64_t has, int64_t needs)
 extern "C" int64_t rec_history_scan_workspace(const rec_scan_desc* d)
 {
     if (check_desc(d)) return -1;
-    return link_bytes(d, cut_of(d));
+    return link_bytes(d, cut_of(d, kForwardBlocks));
 }
 
 extern "C" int rec_history_scan(const rec_scan_desc* d, const rec_scan_inputs* in, const int64_t* seq_off, void* y, int64_t y_stride,
@@ -739,7 +798,7 @@ extern "C" int rec_history_scan(const rec_scan_desc* d, const rec_scan_inputs* i
         REC_REFUSE(!seq_off || (d->rows > 0 && !y), "null argument");
         REC_REFUSE(y_stride < d->channels || y_stride > INT32_MAX, "a row stride is smaller than the channels, or beyond 2^31-1");
         REC_REFUSE(overlaps_inputs(d, in, channel_rows(d, y, y_stride)), "the output overlaps an input");
-        const Cut c = cut_of(d);
+        const Cut c = cut_of(d, kForwardBlocks);
         if (int rc = check_workspace(workspace, workspace_bytes, link_bytes(d, c))) return rc;
         if (int rc = rec_check_device(d->device)) return rc;
         const int64_t blocks = (int64_t)c.chunks * c.tiles, n = (int64_t)d->channels * d->states;
@@ -779,7 +838,7 @@ static int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 extern "C" int64_t rec_history_scan_backward_workspace(const rec_scan_desc* d)
 {
     if (check_desc(d)) return -1;
-    const Cut c = cut_of(d);
+    const Cut c = cut_of(d, kBackwardBlocks);
     return round16(link_bytes(d, c)) + round16(backward_part_a(d, c)) + backward_part_bc(d, c);
 }
 
@@ -801,7 +860,7 @@ extern "C" int rec_history_scan_backward(const rec_scan_desc* d, const void* dy,
         }
         if (int rc = check_workspace(workspace, workspace_bytes, rec_history_scan_backward_workspace(d))) return rc;
         if (int rc = rec_check_device(d->device)) return rc;
-        const Cut c = cut_of(d);
+        const Cut c = cut_of(d, kBackwardBlocks);
         const int64_t blocks = (int64_t)c.chunks * c.tiles, n = (int64_t)d->channels * d->states;
         if (int rc = check_blocks(blocks)) return rc;
         const int64_t empty_blocks = out->dinitial ? (n * d->n_seq + 255) / 256 : 0;
@@ -858,7 +917,7 @@ extern "C" int rec_history_scan_step(const rec_scan_desc* d, const rec_scan_inpu
         REC_REFUSE(overlaps_inputs(d, in, yr) || overlaps_inputs(d, in, pool) || rec_overlap(pool, yr), "the inputs, y and the state must not overlap");
         if (int rc = rec_check_device(d->device)) return rc;
         if (d->rows == 0) return 0;
-        Cut c = cut_of(d);
+        Cut c = cut_of(d, kForwardBlocks);
         c.chunk = 0; c.chunks = 0;
         ScanArgs a = {};
         fill(a, d, in, c);
