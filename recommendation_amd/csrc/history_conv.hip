@@ -2,9 +2,13 @@
 //
 //   v[t][d] = bias[d] + sum_{j < W} weight[d][j] x[t - (W-1) + j][d],   y = silu(v) or v
 //
-// 2 W flop per element read and written: bound by memory.  A thread owns V neighbouring channels (one 16-byte access per row
-// where alignment allows) and walks a strip of consecutive rows with the window in registers, so a row is read once plus W-1
-// rows of halo per strip (these come from the cache).  Where a history begins inside the strip, the window is replaced by that history's own.
+// About 2 W flop per element read and written, four times that in the gradient: bound by memory, the gradient by its vector
+// instructions close behind.  A thread owns V neighbouring channels and walks a strip of consecutive rows with the window in
+// registers, so a row is read once plus W-1 rows of halo per strip (these come from the cache), its loads a few rows ahead.
+// Where a history begins inside the strip, the window is replaced by that history's own.  A wavefront has one strip where the
+// channels allow: what it knows of the histories is scalar then, and the registers hold windows (gradient over 598 655 x 128
+// bf16, W = 4: 88 registers and 134 us against 138 and 165 with a strip per thread).  V = 2: with V = 4 the gradient takes 205 us, with 8 375,
+// their registers leaving one or two wavefronts per SIMD.
 #include "operators.h"
 
 namespace {
@@ -87,30 +91,59 @@ __device__ __forceinline__ void final_windows(const ConvArgs& a, int64_t i)
     store_row<T, V>(a.final_window, ((int64_t)s * (W - 1) + q) * a.channels + d, v);
 }
 
-template <class T, int W, int V>
+constexpr int kForwardGroup = 4, kBackwardGroup = 2;
+// GROUP rows of a strip, loaded together and a group ahead of the walk; a row behind the array's end takes the last one
+template <int GROUP, class T, int V>
+__device__ __forceinline__ void fetch_rows(const void* base, int64_t stride, int64_t r, int64_t rows, int d, Pack<T, V> (&raw)[GROUP])
+{
+#pragma unroll
+    for (int k = 0; k < GROUP; k++) {
+        const int64_t at = r + k < rows ? r + k : rows - 1;
+        raw[k] = *reinterpret_cast<const Pack<T, V>*>((const T*)base + at * stride + d);
+    }
+}
+template <class T, int V> __device__ __forceinline__ void unpack(const Pack<T, V>& p, float (&x)[V])
+{
+#pragma unroll
+    for (int v = 0; v < V; v++) x[v] = to_f32(p.v[v]);
+}
+
+// The strip and the channels of a thread: `ct` threads share a strip, 256 / ct strips a block.  ONE: a wavefront has one strip, which
+// then is a scalar, and with it all that is known of the histories in it.
+template <int V, bool ONE> struct Place {
+    int64_t strip;
+    int cv, d;
+    bool on;
+    __device__ __forceinline__ Place(const ConvArgs& a)
+    {
+        const int ct = ONE ? 64 : a.ct, part = threadIdx.x / ct;
+        strip = (int64_t)(blockIdx.x / a.tiles) * (256 / ct) + (ONE ? __builtin_amdgcn_readfirstlane(part) : part);
+        cv = blockIdx.x % a.tiles * ct + threadIdx.x % ct;
+        on = cv < a.nvec;
+        d = on ? cv * V : 0;
+    }
+};
+
+template <class T, int W, int V, bool ONE>
 __global__ __launch_bounds__(256) void conv_forward_kernel(ConvArgs a)
 {
     if ((int)blockIdx.x >= a.main_blocks) {
         final_windows<T, W, V>(a, (int64_t)(blockIdx.x - a.main_blocks) * 256 + threadIdx.x);
         return;
     }
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t strip = i / a.nvec;
-    if (strip >= a.strips) return;
-    const int d = (int)(i - strip * a.nvec) * V;
-    const int64_t r0 = strip * a.strip_rows, r1 = r0 + a.strip_rows < a.rows ? r0 + a.strip_rows : a.rows;
+    constexpr int GROUP = kForwardGroup;
+    const Place<V, ONE> p(a);
+    if (p.strip >= a.strips || !p.on) return;
+    const int d = p.d;
+    const int64_t strip = p.strip, r0 = strip * a.strip_rows, r1 = r0 + a.strip_rows < a.rows ? r0 + a.strip_rows : a.rows;
+    Pack<T, V> ahead[GROUP];
+    fetch_rows<GROUP, T, V>(a.x, a.x_stride, r0, a.rows, d, ahead);
     float w[W][V], b[V], win[W - 1][V];
     load_filter<W, V>(a, d, w, b);
     SeqCursor c;
     c.begin(a.off, a.n_seq, r0);
     load_window<T, W, V>(a, c.s, c.inside(a.n_seq) ? a.off[c.s] : r0, r0, d, win);
-    for (int64_t r = r0; r < r1; r++) {
-        float x[V], y[V];
-        load_row<T, V>(a.x, r * a.x_stride + d, x);
-        if (r >= c.next) {
-            c.advance(a.off, a.n_seq, r);
-            load_window<T, W, V>(a, c.s, r, r, d, win);
-        }
+    auto step = [&](const float (&x)[V], float (&y)[V]) {
 #pragma unroll
         for (int v = 0; v < V; v++) {
             float s = b[v];
@@ -122,12 +155,36 @@ __global__ __launch_bounds__(256) void conv_forward_kernel(ConvArgs a)
             for (int j = 0; j + 1 < W - 1; j++) win[j][v] = win[j + 1][v];
             win[W - 2][v] = x[v];
         }
-        if (c.inside(a.n_seq)) {
-            store_row<T, V>(a.y, r * a.y_stride + d, y);
-        } else if (a.zero_rest) {
+    };
+    for (int64_t r = r0; r < r1; r += GROUP) {
+        float x[GROUP][V], y[V];
 #pragma unroll
-            for (int v = 0; v < V; v++) y[v] = 0.0f;
-            store_row<T, V>(a.y, r * a.y_stride + d, y);
+        for (int k = 0; k < GROUP; k++) unpack<T, V>(ahead[k], x[k]);
+        if (r + GROUP < r1) fetch_rows<GROUP, T, V>(a.x, a.x_stride, r + GROUP, a.rows, d, ahead);
+        if (r + GROUP <= r1 && r + GROUP <= c.next && c.inside(a.n_seq)) {   // all of one history
+#pragma unroll
+            for (int k = 0; k < GROUP; k++) {
+                step(x[k], y);
+                store_row<T, V>(a.y, (r + k) * a.y_stride + d, y);
+            }
+            continue;
+        }
+#pragma unroll
+        for (int k = 0; k < GROUP; k++) {
+            const int64_t row = r + k;
+            if (row >= r1) continue;
+            if (row >= c.next) {
+                c.advance(a.off, a.n_seq, row);
+                load_window<T, W, V>(a, c.s, row, row, d, win);
+            }
+            step(x[k], y);
+            if (c.inside(a.n_seq)) {
+                store_row<T, V>(a.y, row * a.y_stride + d, y);
+            } else if (a.zero_rest) {
+#pragma unroll
+                for (int v = 0; v < V; v++) y[v] = 0.0f;
+                store_row<T, V>(a.y, row * a.y_stride + d, y);
+            }
         }
     }
 }
@@ -135,7 +192,7 @@ __global__ __launch_bounds__(256) void conv_forward_kernel(ConvArgs a)
 // The gradient walks the same strips.  acc[i] collects dx of the W rows up to the current one; the oldest is complete W-1 rows
 // later, so a strip reads W-1 rows past its end.  The window in front of a history's first row is W-1 rows like any other
 // to the walk: what arrives there is dinitial, and dfinal enters at the last W-1 rows, of the window too if the history is shorter.
-template <class T, int W, int V>
+template <class T, int W, int V, bool ONE>
 __global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs a)
 {
     if ((int)blockIdx.x >= a.main_blocks) {   // dinitial of empty histories: their window passes through
@@ -151,11 +208,11 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs a)
         store_row<T, V>(a.dinitial, at, v);
         return;
     }
-    const int tile = blockIdx.x % a.tiles, lane_c = threadIdx.x % a.ct;
-    const int cv = tile * a.ct + lane_c;
-    const bool on = cv < a.nvec;
-    const int d = on ? cv * V : 0;
-    const int per = 256 / a.ct;   // strips a block walks at a time
+    constexpr int GROUP = kBackwardGroup;
+    const Place<V, ONE> p(a);
+    const int ct = ONE ? 64 : a.ct, lane_c = threadIdx.x % ct, d = p.d;
+    const bool on = p.on;
+    const int per = 256 / ct;   // strips a block walks at a time
     const int blocks_r = a.main_blocks / a.tiles;
     float w[W][V], b[V], dw[W][V], db[V];
     load_filter<W, V>(a, d, w, b);
@@ -165,8 +222,11 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs a)
 #pragma unroll
         for (int j = 0; j < W; j++) dw[j][v] = 0.0f;
     }
-    for (int64_t strip = (int64_t)(blockIdx.x / a.tiles) * per + threadIdx.x / a.ct; on && strip < a.strips; strip += (int64_t)blocks_r * per) {
-        const int64_t r0 = strip * a.strip_rows, r1 = r0 + a.strip_rows < a.rows ? r0 + a.strip_rows : a.rows;
+    for (int64_t strip = p.strip; on && strip < a.strips; strip += (int64_t)blocks_r * per) {
+        const int64_t r0 = strip * a.strip_rows, r1 = r0 + a.strip_rows < a.rows ? r0 + a.strip_rows : a.rows, r2 = r1 + (W - 1);
+        Pack<T, V> ahead_x[GROUP], ahead_g[GROUP];
+        fetch_rows<GROUP, T, V>(a.x, a.x_stride, r0, a.rows, d, ahead_x);
+        fetch_rows<GROUP, T, V>(a.dy, a.dy_stride, r0, a.rows, d, ahead_g);
         SeqCursor c;
         c.begin(a.off, a.n_seq, r0);
         int64_t start = c.inside(a.n_seq) ? a.off[c.s] : r0;
@@ -185,63 +245,84 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs a)
                 if (q >= 0) store_row<T, V>(a.dinitial, ((int64_t)c.s * (W - 1) + q) * a.channels + d, g);
             }
         };
-        for (int64_t r = r0; r < r1 + (W - 1); r++) {
-            if (r >= c.next || r >= a.rows) {
-                if (c.inside(a.n_seq)) {   // the history ended with row r - 1
-#pragma unroll
-                    for (int i = 0; i < W - 1; i++) {
-                        float g[V], f[V];
-#pragma unroll
-                        for (int v = 0; v < V; v++) f[v] = 0.0f;
-                        if (a.dfinal) load_row<T, V>(a.dfinal, ((int64_t)c.s * (W - 1) + i) * a.channels + d, f);
-#pragma unroll
-                        for (int v = 0; v < V; v++) g[v] = acc[i][v] + f[v];
-                        emit(r - (W - 1) + i, g);
-                    }
-                }
-                if (r >= r1) break;
-                c.advance(a.off, a.n_seq, r);
-                start = r;
-                load_window<T, W, V>(a, c.s, start, r, d, win);
-#pragma unroll
-                for (int i = 0; i < W; i++)
-#pragma unroll
-                    for (int v = 0; v < V; v++) acc[i][v] = 0.0f;
-            }
-            if (!c.inside(a.n_seq)) {
-                if (r >= r1) break;
-                if (a.zero_rest) store_row<T, V>(a.dx, r * a.dx_stride + d, acc[0]);   // zeros
-                continue;
-            }
-            float x[V], g[V];
-            load_row<T, V>(a.x, r * a.x_stride + d, x);
-            load_row<T, V>(a.dy, r * a.dy_stride + d, g);
-            const bool own = r < r1;
+        // one row; `done` receives the row W-1 in front of it
+        auto step = [&](const float (&x)[V], const float (&g)[V], bool own, float (&done)[V]) {
 #pragma unroll
             for (int v = 0; v < V; v++) {
                 float s = b[v];
 #pragma unroll
                 for (int j = 0; j < W - 1; j++) s = fmaf(w[j][v], win[j][v], s);
                 s = fmaf(w[W - 1][v], x[v], s);
-                const float dv = a.silu ? g[v] * dsilu_f32(s) : g[v];
+                const float dv = a.silu ? g[v] * dsilu_f32(s) : g[v], mine = own ? dv : 0.0f;
 #pragma unroll
                 for (int i = 0; i < W; i++) acc[i][v] = fmaf(w[i][v], dv, acc[i][v]);
-                if (own) {
 #pragma unroll
-                    for (int j = 0; j < W - 1; j++) dw[j][v] = fmaf(dv, win[j][v], dw[j][v]);
-                    dw[W - 1][v] = fmaf(dv, x[v], dw[W - 1][v]);
-                    db[v] += dv;
-                }
+                for (int j = 0; j < W - 1; j++) dw[j][v] = own ? fmaf(dv, win[j][v], dw[j][v]) : dw[j][v];
+                dw[W - 1][v] = own ? fmaf(dv, x[v], dw[W - 1][v]) : dw[W - 1][v];
+                db[v] += mine;
 #pragma unroll
                 for (int j = 0; j + 1 < W - 1; j++) win[j][v] = win[j + 1][v];
                 win[W - 2][v] = x[v];
-            }
-            emit(r - (W - 1), acc[0]);
-#pragma unroll
-            for (int v = 0; v < V; v++) {
+                done[v] = acc[0][v];
 #pragma unroll
                 for (int i = 0; i + 1 < W; i++) acc[i][v] = acc[i + 1][v];
                 acc[W - 1][v] = 0.0f;
+            }
+        };
+        bool over = false;
+        for (int64_t r = r0; r < r2 && !over; r += GROUP) {
+            float x[GROUP][V], g[GROUP][V], done[V];
+#pragma unroll
+            for (int k = 0; k < GROUP; k++) {
+                unpack<T, V>(ahead_x[k], x[k]);
+                unpack<T, V>(ahead_g[k], g[k]);
+            }
+            if (r + GROUP < r2) {
+                fetch_rows<GROUP, T, V>(a.x, a.x_stride, r + GROUP, a.rows, d, ahead_x);
+                fetch_rows<GROUP, T, V>(a.dy, a.dy_stride, r + GROUP, a.rows, d, ahead_g);
+            }
+            const int64_t first = (start > r0 ? start : r0) + (W - 1);
+            if (r >= first && r + GROUP <= r1 && r + GROUP <= c.next && c.inside(a.n_seq)) {   // all of one history, and so are the rows finished
+#pragma unroll
+                for (int k = 0; k < GROUP; k++) {
+                    step(x[k], g[k], true, done);
+                    store_row<T, V>(a.dx, (r + k - (W - 1)) * a.dx_stride + d, done);
+                }
+                continue;
+            }
+#pragma unroll
+            for (int k = 0; k < GROUP; k++) {
+                const int64_t row = r + k;
+                if (over || row >= r2) continue;
+                if (row >= c.next || row >= a.rows) {
+                    if (c.inside(a.n_seq)) {   // the history ended with the row in front
+#pragma unroll
+                        for (int i = 0; i < W - 1; i++) {
+                            float f[V];
+#pragma unroll
+                            for (int v = 0; v < V; v++) f[v] = 0.0f;
+                            if (a.dfinal) load_row<T, V>(a.dfinal, ((int64_t)c.s * (W - 1) + i) * a.channels + d, f);
+#pragma unroll
+                            for (int v = 0; v < V; v++) f[v] += acc[i][v];
+                            emit(row - (W - 1) + i, f);
+                        }
+                    }
+                    if (row >= r1) { over = true; continue; }
+                    c.advance(a.off, a.n_seq, row);
+                    start = row;
+                    load_window<T, W, V>(a, c.s, start, row, d, win);
+#pragma unroll
+                    for (int i = 0; i < W; i++)
+#pragma unroll
+                        for (int v = 0; v < V; v++) acc[i][v] = 0.0f;
+                }
+                if (!c.inside(a.n_seq)) {
+                    if (row >= r1) { over = true; continue; }
+                    if (a.zero_rest) store_row<T, V>(a.dx, row * a.dx_stride + d, acc[0]);   // zeros
+                    continue;
+                }
+                step(x[k], g[k], row < r1, done);
+                emit(row - (W - 1), done);
             }
         }
     }
@@ -249,21 +330,17 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs a)
     // the block's sums, over its strips in a fixed order
     __shared__ float red[256][V + 1];
     float* part = a.partial + (int64_t)(blockIdx.x / a.tiles) * a.channels * (W + 1);
+#pragma unroll
     for (int j = 0; j <= W; j++) {
         __syncthreads();
 #pragma unroll
-        for (int v = 0; v < V; v++) {
-            float s = db[v];
-#pragma unroll
-            for (int k = 0; k < W; k++) s = j == k ? dw[k][v] : s;
-            red[threadIdx.x][v] = s;
-        }
+        for (int v = 0; v < V; v++) red[threadIdx.x][v] = j < W ? dw[j < W ? j : 0][v] : db[v];
         __syncthreads();
-        if ((int)threadIdx.x < a.ct && on) {
+        if ((int)threadIdx.x < ct && on) {
 #pragma unroll
             for (int v = 0; v < V; v++) {
                 float s = 0.0f;
-                for (int k = 0; k < per; k++) s += red[k * a.ct + lane_c][v];
+                for (int k = 0; k < per; k++) s += red[k * ct + lane_c][v];
                 part[j < W ? (int64_t)(d + v) * W + j : (int64_t)a.channels * W + d + v] = s;
             }
         }
@@ -313,7 +390,15 @@ __global__ __launch_bounds__(256) void conv_step_kernel(ConvArgs a, const int32_
             if (slots[r] == slot) click(r);
 }
 
-constexpr int kStripRows = 32;
+// Rows of a strip: long strips read fewer rows twice (gradient above: 163, 142, 134 us at 32, 64, 128 rows), short ones give a small
+// call more threads (2048 x 128 f32 forward: 15 us at 32 rows, 5 at 4).  64k threads fill the chip.
+int strip_rows_of(int64_t rows, int64_t nvec, int longest)
+{
+    const int64_t s = rows * nvec / 65536 / 4 * 4;
+    return (int)(s < 4 ? 4 : s > longest ? longest : s);
+}
+constexpr int kForwardVec = 2, kBackwardVec = 2;
+constexpr int kForwardStrip = 128, kBackwardStrip = 128;
 constexpr int kBackwardBlocks = 2048;   // at most, per tile of channels: bounds the partial sums
 
 int check_desc(const rec_conv_desc* d)
@@ -348,34 +433,42 @@ Layout layout_of(const rec_conv_desc* d, int widest, std::initializer_list<const
     bool wide = d->channels % widest == 0;
     for (const void* p : ptrs) wide = wide && rec_aligned(p, (size_t)widest * size);
     for (int64_t s : strides) wide = wide && s % widest == 0;
-    const int v = wide ? widest : 1;
+    // 33 to 64 channels are one wavefront's at V = 1 and half of one's at V = 2 (gradient over 598 655 x 64 bf16: 90 us against 118)
+    const int v = wide && (widest > 2 || d->channels > 64 || d->channels <= 32) ? widest : 1;
     return {v, d->channels / v};
 }
 
-struct BackwardGrid { int ct, tiles, per, blocks_r; int64_t strips; };
-BackwardGrid backward_grid(const rec_conv_desc* d, int nvec)
+struct Grid { int ct, tiles, per, blocks_r, strip_rows; int64_t strips; };
+Grid grid_of(const rec_conv_desc* d, int nvec, int longest, int64_t most_blocks)
 {
-    BackwardGrid g;
+    Grid g;
     g.ct = 64;
     while (g.ct > 1 && g.ct / 2 >= nvec) g.ct /= 2;
     g.tiles = (nvec + g.ct - 1) / g.ct;
     g.per = 256 / g.ct;
-    g.strips = (d->rows + kStripRows - 1) / kStripRows;
-    const int64_t most = (g.strips + g.per - 1) / g.per;
-    g.blocks_r = (int)(most < kBackwardBlocks ? most : kBackwardBlocks);
+    g.strip_rows = strip_rows_of(d->rows, nvec, longest);
+    g.strips = (d->rows + g.strip_rows - 1) / g.strip_rows;
+    const int64_t all = (g.strips + g.per - 1) / g.per, rounds = (all + most_blocks - 1) / most_blocks;
+    g.blocks_r = rounds ? (int)((all + rounds - 1) / rounds) : 0;   // each block as many strips as any other
     return g;
 }
 
-#define CONV_TAPS(T, V, CALL)                                                                         \
-    switch (d->taps) {                                                                                \
-    case 2: CALL(T, 2, V); break; case 3: CALL(T, 3, V); break; case 4: CALL(T, 4, V); break;         \
-    case 5: CALL(T, 5, V); break; case 6: CALL(T, 6, V); break; case 7: CALL(T, 7, V); break;         \
-    default: CALL(T, 8, V); break;                                                                    \
+#define CONV_TAPS(T, V, ONE, CALL)                                                                                    \
+    switch (d->taps) {                                                                                                \
+    case 2: CALL(T, 2, V, ONE); break; case 3: CALL(T, 3, V, ONE); break; case 4: CALL(T, 4, V, ONE); break;          \
+    case 5: CALL(T, 5, V, ONE); break; case 6: CALL(T, 6, V, ONE); break; case 7: CALL(T, 7, V, ONE); break;          \
+    default: CALL(T, 8, V, ONE); break;                                                                               \
     }
-#define CONV_DISPATCH(WIDE32, WIDE16, vec, CALL)                                                      \
-    if (d->type == REC_TYPE_F32) { if (vec > 1) { CONV_TAPS(float, WIDE32, CALL) } else { CONV_TAPS(float, 1, CALL) } }             \
-    else if (d->type == REC_TYPE_F16) { if (vec > 1) { CONV_TAPS(_Float16, WIDE16, CALL) } else { CONV_TAPS(_Float16, 1, CALL) } }  \
-    else { if (vec > 1) { CONV_TAPS(__bf16, WIDE16, CALL) } else { CONV_TAPS(__bf16, 1, CALL) } }
+#define CONV_TYPE(T, WIDE, vec, one, CALL)                                                                            \
+    {                                                                                                                 \
+        if (vec == 1) { if (one) { CONV_TAPS(T, 1, true, CALL) } else { CONV_TAPS(T, 1, false, CALL) } }              \
+        else if (one) { CONV_TAPS(T, WIDE, true, CALL) }                                                              \
+        else { CONV_TAPS(T, WIDE, false, CALL) }                                                                      \
+    }
+#define CONV_DISPATCH(WIDE32, WIDE16, vec, one, CALL)                                                                 \
+    if (d->type == REC_TYPE_F32) CONV_TYPE(float, WIDE32, vec, one, CALL)                                             \
+    else if (d->type == REC_TYPE_F16) CONV_TYPE(_Float16, WIDE16, vec, one, CALL)                                     \
+    else CONV_TYPE(__bf16, WIDE16, vec, one, CALL)
 
 int check_blocks(int64_t blocks)
 {
@@ -393,24 +486,25 @@ extern "C" int rec_history_conv(const rec_conv_desc* d, const void* x, int64_t x
         REC_REFUSE(!weight || !seq_off || (d->rows > 0 && (!x || !y)), "null argument");
         if (int rc = check_stride(x_stride, d)) return rc;
         if (int rc = check_stride(y_stride, d)) return rc;
-        const int size = rec_type_size(d->type), wide = 16 / size;
+        const int wide = kForwardVec;
         REC_REFUSE(rec_overlap(rows_of(d, x, x_stride), rows_of(d, y, y_stride)), "the output overlaps the input");
         if (int rc = rec_check_device(d->device)) return rc;
         const Layout l = layout_of(d, wide, {x, y, initial, final_window}, {x_stride, y_stride});
+        const Grid g = grid_of(d, l.nvec, kForwardStrip, INT32_MAX);
         ConvArgs a = {};
         a.x = x; a.initial = initial; a.y = y; a.final_window = final_window; a.weight = weight; a.bias = bias; a.off = seq_off;
         a.x_stride = x_stride; a.y_stride = y_stride; a.rows = d->rows; a.n_seq = d->n_seq; a.channels = d->channels; a.nvec = l.nvec;
-        a.silu = d->silu; a.zero_rest = d->zero_rest; a.strip_rows = kStripRows;
-        a.strips = (d->rows + kStripRows - 1) / kStripRows;
-        const int64_t main_blocks = (a.strips * l.nvec + 255) / 256;
+        a.silu = d->silu; a.zero_rest = d->zero_rest; a.strip_rows = g.strip_rows; a.strips = g.strips;
+        a.ct = g.ct; a.tiles = g.tiles;
+        const int64_t main_blocks = (int64_t)g.blocks_r * g.tiles;
         const int64_t more = final_window ? ((int64_t)d->n_seq * (d->taps - 1) * l.nvec + 255) / 256 : 0;
         if (int rc = check_blocks(main_blocks + more)) return rc;
         if (main_blocks + more == 0) return 0;
         a.main_blocks = (int)main_blocks;
         DeviceScope scope;
         HIP_TRY(scope.enter(d->device));
-#define CALL(T, W, V) conv_forward_kernel<T, W, V><<<(unsigned)(main_blocks + more), 256, 0, (hipStream_t)stream>>>(a)
-        CONV_DISPATCH(4, 8, l.vec, CALL)
+#define CALL(T, W, V, ONE) conv_forward_kernel<T, W, V, ONE><<<(unsigned)(main_blocks + more), 256, 0, (hipStream_t)stream>>>(a)
+        CONV_DISPATCH(kForwardVec, kForwardVec, l.vec, g.ct == 64, CALL)
 #undef CALL
         HIP_TRY(hipGetLastError());
         return 0;
@@ -420,10 +514,10 @@ extern "C" int rec_history_conv(const rec_conv_desc* d, const void* x, int64_t x
 extern "C" int64_t rec_history_conv_backward_workspace(const rec_conv_desc* d)
 {
     if (check_desc(d)) return -1;
-    // the narrow layout has at most as many blocks as the limit, whatever the alignment of the arrays turns out to be
-    const int64_t strips = (d->rows + kStripRows - 1) / kStripRows;
-    const int64_t blocks = strips < kBackwardBlocks ? strips : kBackwardBlocks;
-    return blocks * d->channels * (d->taps + 1) * 4;
+    // as much as the layout that takes the most blocks needs, whatever the alignment of the arrays turns out to be
+    const int narrow = grid_of(d, d->channels, kBackwardStrip, kBackwardBlocks).blocks_r;
+    const int wide = d->channels % kBackwardVec == 0 ? grid_of(d, d->channels / kBackwardVec, kBackwardStrip, kBackwardBlocks).blocks_r : 0;
+    return (int64_t)(narrow > wide ? narrow : wide) * d->channels * (d->taps + 1) * 4;
 }
 
 extern "C" int rec_history_conv_backward(const rec_conv_desc* d, const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,
@@ -443,12 +537,12 @@ extern "C" int rec_history_conv_backward(const rec_conv_desc* d, const void* dy,
         REC_REFUSE(sums && workspace_bytes < rec_history_conv_backward_workspace(d), "the workspace is too small");
         REC_REFUSE(sums && rec_history_conv_backward_workspace(d) > 0 && (!workspace || !rec_aligned(workspace, 16)), "the workspace is null or not aligned to 16 bytes");
         if (int rc = rec_check_device(d->device)) return rc;
-        const Layout l = layout_of(d, 4, {x, dy, dx, initial, dfinal, dinitial}, {x_stride, dy_stride, dx_stride});
-        const BackwardGrid g = backward_grid(d, l.nvec);
+        const Layout l = layout_of(d, kBackwardVec, {x, dy, dx, initial, dfinal, dinitial}, {x_stride, dy_stride, dx_stride});
+        const Grid g = grid_of(d, l.nvec, kBackwardStrip, kBackwardBlocks);
         ConvArgs a = {};
         a.x = x; a.initial = initial; a.dy = dy; a.dfinal = dfinal; a.dx = dx; a.dinitial = dinitial; a.weight = weight; a.bias = bias;
         a.off = seq_off; a.x_stride = x_stride; a.dy_stride = dy_stride; a.dx_stride = dx_stride; a.rows = d->rows; a.n_seq = d->n_seq;
-        a.channels = d->channels; a.nvec = l.nvec; a.silu = d->silu; a.zero_rest = d->zero_rest; a.strip_rows = kStripRows;
+        a.channels = d->channels; a.nvec = l.nvec; a.silu = d->silu; a.zero_rest = d->zero_rest; a.strip_rows = g.strip_rows;
         a.strips = g.strips; a.ct = g.ct; a.tiles = g.tiles;
         a.partial = sums ? (float*)workspace : nullptr;
         const int64_t main_blocks = (int64_t)g.blocks_r * g.tiles;
@@ -458,8 +552,8 @@ extern "C" int rec_history_conv_backward(const rec_conv_desc* d, const void* dy,
         DeviceScope scope;
         HIP_TRY(scope.enter(d->device));
         if (main_blocks + more > 0) {
-#define CALL(T, W, V) conv_backward_kernel<T, W, V><<<(unsigned)(main_blocks + more), 256, 0, (hipStream_t)stream>>>(a)
-            CONV_DISPATCH(4, 4, l.vec, CALL)
+#define CALL(T, W, V, ONE) conv_backward_kernel<T, W, V, ONE><<<(unsigned)(main_blocks + more), 256, 0, (hipStream_t)stream>>>(a)
+            CONV_DISPATCH(kBackwardVec, kBackwardVec, l.vec, g.ct == 64, CALL)
 #undef CALL
             HIP_TRY(hipGetLastError());
         }
@@ -494,8 +588,8 @@ extern "C" int rec_history_conv_step(const rec_conv_desc* d, const void* x, int6
         if (int rc = check_blocks(blocks)) return rc;
         DeviceScope scope;
         HIP_TRY(scope.enter(d->device));
-#define CALL(T, W, V) conv_step_kernel<T, W, V><<<(unsigned)blocks, threads, 0, (hipStream_t)stream>>>(a, slots, (T*)window)
-        CONV_DISPATCH(4, 8, l.vec, CALL)
+#define CALL(T, W, V, ONE) conv_step_kernel<T, W, V><<<(unsigned)blocks, threads, 0, (hipStream_t)stream>>>(a, slots, (T*)window)
+        CONV_DISPATCH(4, 8, l.vec, false, CALL)
 #undef CALL
         HIP_TRY(hipGetLastError());
         return 0;
