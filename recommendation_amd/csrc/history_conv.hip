@@ -354,8 +354,11 @@ __global__ __launch_bounds__(256) void conv_step_kernel(ConvArgs a, const int32_
     const int64_t row = blockIdx.x / a.tiles;
     const int cv = (int)(blockIdx.x % a.tiles) * (int)blockDim.x + threadIdx.x, d = cv * V;
     const int slot = slots[row];
-    bool earlier, later;
-    slot_is_shared(slots, a.rows, row, slot, earlier, later);
+    __shared__ unsigned seen[4];
+    look_for_slot(slots, a.rows, row, slot, seen);
+    __syncthreads();
+    const unsigned shared = slots_seen(seen);
+    const bool earlier = shared & 1, later = shared & 2;
     if (cv >= a.nvec) return;
     float y[V];
     if (slot < 0 || slot >= a.n_seq) {

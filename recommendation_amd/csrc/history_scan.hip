@@ -29,7 +29,7 @@ struct ScanArgs {
     float *part_a;               // backward: [chunks][channels * states + 2 * channels]: dA, dD, ddelta_bias
     int64_t u_stride, delta_stride, z_stride, B_stride, C_stride, y_stride, dy_stride;
     int64_t rows;
-    int n_seq, channels, groups, per, states, chunk, chunks, tiles, tiles_per_group, softplus, zero_rest;
+    int main_blocks, n_seq, channels, groups, per, states, chunk, chunks, tiles, tiles_per_group, softplus, zero_rest;
 };
 
 // the block's place: a chunk of rows, a run of channels of one group
@@ -97,13 +97,6 @@ __device__ __forceinline__ float computed(float v)
 {
     asm volatile("" : "+v"(v));
     return v;
-}
-
-template <class T>
-__device__ __forceinline__ float delta_of(const ScanArgs& a, int64_t row, int d, float& raw)
-{
-    raw = to_f32(((const T*)a.delta)[row * a.delta_stride + d]) + (a.delta_bias ? a.delta_bias[d] : 0.0f);
-    return a.softplus ? softplus_f32(raw) : raw;
 }
 
 // What a thread stages of a tile: PT (row, channel) pairs, 256 apart, all of one channel, and NB values each of B and C.
@@ -260,9 +253,23 @@ template <int LN, int GR> __device__ __forceinline__ void write_sums(float (*to)
 }
 
 // third pass
+// Empty histories: their state passes through (forwards initial -> final_state, backwards dfinal -> dinitial).  Blocks behind
+// the walk's take them, a value per thread.
+__device__ __forceinline__ void pass_empty(const ScanArgs& a, const float* from, float* to)
+{
+    const int64_t i = (int64_t)(blockIdx.x - a.main_blocks) * 256 + threadIdx.x, n = (int64_t)a.channels * a.states;
+    if (i >= n * a.n_seq) return;
+    const int64_t s = i / n;
+    if (a.off[s + 1] <= a.off[s]) to[i] = from ? from[i] : 0.0f;
+}
+
 template <class T, int LN>
 __global__ __launch_bounds__(256) void scan_forward_kernel(ScanArgs a)
 {
+    if ((int)blockIdx.x >= a.main_blocks) {
+        pass_empty(a, a.initial, a.final_state);
+        return;
+    }
     using P = Place<LN>;
     constexpr int CH = P::CH, NP = 4 * LN, GR = rows_together<LN>();
     __shared__ float2 sd[TT][CH];
@@ -350,15 +357,6 @@ __global__ __launch_bounds__(256) void scan_forward_kernel(ScanArgs a)
     }
 }
 
-// empty histories: their state passes through (forward: initial -> final_state, backward: dfinal -> dinitial)
-__global__ __launch_bounds__(256) void scan_empty_kernel(ScanArgs a, const float* from, float* to)
-{
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = (int64_t)a.channels * a.states;
-    if (i >= n * a.n_seq) return;
-    const int64_t s = i / n;
-    if (a.off[s + 1] <= a.off[s]) to[i] = from ? from[i] : 0.0f;
-}
-
 // ---- gradient.  With G_t = dL/dh_t:   G_t = C_t dys_t + exp(delta_{t+1} A) G_{t+1}   (dfinal in place of the second term at a
 // history's last row), dys = dy silu(z).  The chunks are linked as above, from the back.
 
@@ -425,6 +423,10 @@ __global__ __launch_bounds__(256) void scan_local_backward_kernel(ScanArgs a)
 template <class T, int LN>
 __global__ __launch_bounds__(256, 2) void scan_backward_kernel(ScanArgs a)
 {
+    if ((int)blockIdx.x >= a.main_blocks) {
+        pass_empty(a, a.dfinal, a.dinitial);
+        return;
+    }
     using P = Place<LN>;
     using Q = Tile<T, LN, true, true, true, true, true>;
     constexpr int CH = P::CH, NP = 4 * LN, PT = Q::PT, ROW = CH + 16, GR = rows_together<LN>();
@@ -637,51 +639,129 @@ __global__ __launch_bounds__(256) void scan_sum_groups_kernel(ScanArgs a)
     ((T*)(i / a.states % 2 ? a.dC : a.dB))[at] = from_f32<T>(v);
 }
 
-// ---- single clicks: a block per row and up to 256 / LN of its channels; the state moves through registers once
-template <class T, int LN>
+// ---- single clicks: a block per row; bound by the state, which is read and written once (4 bytes a value each way), and by
+// the waits in between.  Four pieces of 256 / LN channels at a time: a thread prepares whole channels (delta, delta * u, the gate), then
+// takes four states of one channel of each piece, and everything a row needs is asked for at once, before the block looks for
+// other rows of its slot.
+// The code is kept short (one copy of everything; WHOLE: all 4 LN states of a lane group exist and lie on boundaries of four): a
+// launch this small waits for its instructions, too.
+constexpr int PIECES = 4;
+template <class T, int LN, bool WHOLE>
 __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a, const int32_t* __restrict__ slots, float* state)
 {
-    constexpr int CH = 256 / LN;
-    const int64_t row = blockIdx.x / a.tiles;
-    const int tile = blockIdx.x % a.tiles, g = tile / a.tiles_per_group, ch0 = g * a.per + tile % a.tiles_per_group * CH;
-    const int ch = threadIdx.x / LN, n0 = threadIdx.x % LN * 4, d = ch0 + ch;
+    struct alignas(4) Four { float v[4]; };
+    constexpr int CH = 256 / LN, ALL = PIECES * CH, PT = ALL > 256 ? ALL / 256 : 1;
+    __shared__ float2 sd[ALL];
+    __shared__ float sy[ALL];
+    __shared__ unsigned seen[4];
+    const int row = blockIdx.x, rows = (int)a.rows;
+    const int ch = threadIdx.x / LN, n0 = threadIdx.x % LN * 4;
     const int slot = slots[row];
-    bool earlier, later;
-    slot_is_shared(slots, a.rows, row, slot, earlier, later);
-    if (d >= (g + 1) * a.per) return;
-    if (slot < 0 || slot >= a.n_seq) {
-        if (n0 == 0) ((T*)a.y)[row * a.y_stride + d] = from_f32<T>(0.0f);
-        return;
-    }
-    if (earlier) return;
-    float A2[4];
-    load_states<LN>(a.A, 0, a, d, n0, true, A2);
+    const bool valid = slot >= 0 && slot < a.n_seq;
+    // (a row without a slot reads A in the state's place - a pool may be empty - and stores nothing)
+    float* pool = valid ? state + (int64_t)slot * a.channels * a.states : const_cast<float*>(a.A);
+    auto states = [&](const float* p, int d, float (&v)[4]) {   // of a channel that exists
+        if (WHOLE) {
+            const Four f = *reinterpret_cast<const Four*>(p + d * a.states + n0);
 #pragma unroll
-    for (int e = 0; e < 4; e++) A2[e] *= REC_LOG2E;
-    auto click = [&](int64_t r) {   // the state goes through memory, so that rows of a shared slot are steps like any other
-        float h[4], raw, y = 0.0f;
-        load_states<LN>(state, slot, a, d, n0, true, h);
-        const float delta = delta_of<T>(a, r, d, raw), u = to_f32(((const T*)a.u)[r * a.u_stride + d]);
+            for (int e = 0; e < 4; e++) v[e] = f.v[e];
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            if (n0 + e >= a.states) continue;
-            const float b = to_f32(((const T*)a.B)[r * a.B_stride + (int64_t)g * a.states + n0 + e]);
-            const float c = to_f32(((const T*)a.C)[r * a.C_stride + (int64_t)g * a.states + n0 + e]);
-            h[e] = fmaf(fast_exp2(delta * A2[e]), h[e], delta * u * b);
-            y = fmaf(h[e], c, y);
-        }
-        store_states<LN>(state, slot, a, d, n0, true, h);
-        y = group_sum_dpp<LN>(y);
-        if (n0 == 0) {
-            if (a.D) y = fmaf(a.D[d], u, y);
-            if (a.z) y *= silu_f32(to_f32(((const T*)a.z)[r * a.z_stride + d]));
-            ((T*)a.y)[r * a.y_stride + d] = from_f32<T>(y);
+            for (int e = 0; e < 4; e++) v[e] = p[d * a.states + min(n0 + e, a.states - 1)];
         }
     };
-    click(row);
-    if (later)
-        for (int64_t r = row + 1; r < a.rows; r++)
-            if (slots[r] == slot) click(r);
+    for (int tile0 = 0; tile0 < a.tiles; tile0 += PIECES) {
+        int group[PIECES], first[PIECES], count[PIECES];   // a piece's group, first channel and channels: scalars
+#pragma unroll
+        for (int k = 0; k < PIECES; k++) {
+            const int tile = min(tile0 + k, a.tiles - 1);
+            group[k] = a.groups == 1 ? 0 : tile / a.tiles_per_group;
+            const int part = (tile - group[k] * a.tiles_per_group) * CH;
+            first[k] = group[k] * a.per + part;
+            count[k] = tile0 + k < a.tiles ? min(CH, a.per - part) : 0;
+        }
+        int mine[PT];
+#pragma unroll
+        for (int k = 0; k < PT; k++) {
+            const int v = threadIdx.x + 256 * k, q = v / CH;
+            mine[k] = -1;
+#pragma unroll
+            for (int i = 0; i < PIECES; i++)
+                if (q == i && v % CH < count[i]) mine[k] = first[i] + v % CH;
+        }
+        for (int r = row;;) {
+            T rd[PT], ru[PT], rz[PT];
+            Pack<T, 4> rb[PIECES], rc[PIECES];
+            float bias[PT], D[PT], h[PIECES][4], A[PIECES][4];
+#pragma unroll
+            for (int k = 0; k < PT; k++) {
+                const int at = mine[k] < 0 ? 0 : mine[k];
+                rd[k] = ((const T*)a.delta + r * a.delta_stride)[at];
+                ru[k] = ((const T*)a.u + r * a.u_stride)[at];
+                rz[k] = ((const T*)(a.z ? a.z : a.u) + r * (a.z ? a.z_stride : a.u_stride))[at];
+                bias[k] = a.delta_bias ? a.delta_bias[at] : 0.0f;
+                D[k] = a.D ? a.D[at] : 0.0f;
+            }
+#pragma unroll
+            for (int k = 0; k < PIECES; k++) {   // (a row of a shared slot finds the state as the one before it has left it: in memory)
+                const int d = first[k] + min(ch, max(count[k], 1) - 1);
+                states(a.A, d, A[k]);
+                states(pool, d, h[k]);
+                const T *b = (const T*)a.B + r * a.B_stride + group[k] * a.states, *c = (const T*)a.C + r * a.C_stride + group[k] * a.states;
+                if (WHOLE) {
+                    rb[k] = *reinterpret_cast<const Pack<T, 4>*>(b + n0);
+                    rc[k] = *reinterpret_cast<const Pack<T, 4>*>(c + n0);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) { rb[k].v[e] = b[min(n0 + e, a.states - 1)]; rc[k].v[e] = c[min(n0 + e, a.states - 1)]; }
+                }
+            }
+            if (r == row && tile0 == 0) look_for_slot(slots, a.rows, row, slot, seen);
+            float gate[PT], u[PT];
+#pragma unroll
+            for (int k = 0; k < PT; k++) {
+                const float raw = to_f32(rd[k]) + bias[k], sp = computed(softplus_f32(raw)), delta = a.softplus ? sp : raw;
+                u[k] = to_f32(ru[k]);
+                gate[k] = computed(silu_f32(to_f32(rz[k])));
+                if (PT > 1 || (int)threadIdx.x < ALL) sd[threadIdx.x + 256 * k] = make_float2(delta, delta * u[k]);
+            }
+            __syncthreads();
+            const unsigned shared = slots_seen(seen);
+            if (valid && (shared & 1)) return;   // the first row of a slot takes the others along
+#pragma unroll
+            for (int k = 0; k < PIECES; k++) {
+                const float2 v = sd[k * CH + ch];
+                float y = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    h[k][e] = fmaf(fast_exp2(v.x * (A[k][e] * REC_LOG2E)), h[k][e], v.y * to_f32(rb[k].v[e]));
+                    if (WHOLE || n0 + e < a.states) y = fmaf(h[k][e], to_f32(rc[k].v[e]), y);
+                }
+                if (valid && ch < count[k]) {
+                    float* p = pool + (first[k] + ch) * a.states + n0;
+                    if (WHOLE) *reinterpret_cast<Four*>(p) = Four{{h[k][0], h[k][1], h[k][2], h[k][3]}};
+                    else
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (n0 + e < a.states) p[e] = h[k][e];
+                }
+                y = group_sum_dpp<LN>(y);
+                if (n0 == 0) sy[k * CH + ch] = y;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < PT; k++) {
+                if (mine[k] < 0) continue;
+                float y = sy[threadIdx.x + 256 * k];
+                if (a.D) y = fmaf(D[k], u[k], y);
+                if (a.z) y *= gate[k];
+                ((T*)a.y)[r * a.y_stride + mine[k]] = from_f32<T>(valid ? y : 0.0f);
+            }
+            if (!valid || !(shared & 2)) break;
+            do r++; while (r < rows && slots[r] != slot);
+            if (r >= rows) break;
+        }
+    }
 }
 
 // ---- host
@@ -727,7 +807,7 @@ RowsOf channel_rows(const rec_scan_desc* d, const void* p, int64_t stride)
 int lanes_of(int states) { return states <= 4 ? 1 : states <= 8 ? 2 : states <= 16 ? 4 : states <= 32 ? 8 : 16; }
 
 // How the rows are cut.  A chunk more costs its first pass (two thirds of the third, over the chunk's last history) and a state
-// handed over, so chunks are as long as they can be while the launch still fills the chip: `blocks` of them, between 32 and
+// handed over, so chunks are as long as they can be while the launch still fills the chip: `blocks` of them, between 16 and
 // 512 rows.
 struct Cut { int tiles_per_group, tiles, chunk, chunks; };
 constexpr int kForwardBlocks = 2048, kBackwardBlocks = 2048;
@@ -738,7 +818,7 @@ Cut cut_of(const rec_scan_desc* d, int blocks)
     c.tiles_per_group = (per + ch - 1) / ch;
     c.tiles = c.tiles_per_group * d->groups;
     int64_t rows = d->rows * c.tiles / blocks / TT * TT;
-    if (rows < 32) rows = 32;
+    if (rows < 16) rows = 16;
     if (rows > 512) rows = 512;
     c.chunk = (int)rows;
     c.chunks = (int)((d->rows + rows - 1) / rows);
@@ -802,12 +882,12 @@ extern "C" int rec_history_scan(const rec_scan_desc* d, const rec_scan_inputs* i
         if (int rc = check_workspace(workspace, workspace_bytes, link_bytes(d, c))) return rc;
         if (int rc = rec_check_device(d->device)) return rc;
         const int64_t blocks = (int64_t)c.chunks * c.tiles, n = (int64_t)d->channels * d->states;
-        if (int rc = check_blocks(blocks)) return rc;
         const int64_t empty_blocks = final_state ? (n * d->n_seq + 255) / 256 : 0;
-        if (int rc = check_blocks(empty_blocks)) return rc;
+        if (int rc = check_blocks(blocks + empty_blocks)) return rc;
         ScanArgs a = {};
         fill(a, d, in, c);
         a.off = seq_off; a.y = y; a.y_stride = y_stride; a.final_state = final_state; a.checkpoints = checkpoints;
+        a.main_blocks = (int)blocks;
         a.link = (float*)workspace;
         a.span = a.link + c.chunks * n;
         a.kind = (int*)(a.span + (int64_t)c.chunks * d->channels);
@@ -820,12 +900,11 @@ extern "C" int rec_history_scan(const rec_scan_desc* d, const rec_scan_inputs* i
 #undef CALL
             scan_link_kernel<false><<<(unsigned)((n + LINK_COLS - 1) / LINK_COLS), LINK_COLS * LINK_RUNS, 0, st>>>(a);
         }
-        if (blocks > 0) {
-#define CALL(T, LN) scan_forward_kernel<T, LN><<<(unsigned)blocks, 256, 0, st>>>(a)
+        if (blocks + empty_blocks > 0) {
+#define CALL(T, LN) scan_forward_kernel<T, LN><<<(unsigned)(blocks + empty_blocks), 256, 0, st>>>(a)
             SCAN_DISPATCH(CALL)
 #undef CALL
         }
-        if (empty_blocks > 0) scan_empty_kernel<<<(unsigned)empty_blocks, 256, 0, st>>>(a, in->initial, final_state);
         HIP_TRY(hipGetLastError());
         return 0;
     });
@@ -862,15 +941,15 @@ extern "C" int rec_history_scan_backward(const rec_scan_desc* d, const void* dy,
         if (int rc = rec_check_device(d->device)) return rc;
         const Cut c = cut_of(d, kBackwardBlocks);
         const int64_t blocks = (int64_t)c.chunks * c.tiles, n = (int64_t)d->channels * d->states;
-        if (int rc = check_blocks(blocks)) return rc;
         const int64_t empty_blocks = out->dinitial ? (n * d->n_seq + 255) / 256 : 0;
         const int64_t sum_blocks = c.tiles_per_group > 1 ? (d->rows * d->groups * 2 * d->states + 255) / 256 : 0;
-        if (int rc = check_blocks(empty_blocks > sum_blocks ? empty_blocks : sum_blocks)) return rc;
+        if (int rc = check_blocks(blocks + empty_blocks > sum_blocks ? blocks + empty_blocks : sum_blocks)) return rc;
         const bool params = out->dA || out->dD || out->ddelta_bias;
         ScanArgs a = {};
         fill(a, d, in, c);
         a.off = seq_off; a.dy = dy; a.dy_stride = dy_stride; a.checkpoints_in = checkpoints; a.dfinal = dfinal;
         a.du = out->du; a.ddelta = out->ddelta; a.dz = out->dz; a.dB = out->dB; a.dC = out->dC; a.dinitial = out->dinitial;
+        a.main_blocks = (int)blocks;
         char* ws = (char*)workspace;
         a.link = (float*)ws;
         a.span = a.link + c.chunks * n;
@@ -887,8 +966,8 @@ extern "C" int rec_history_scan_backward(const rec_scan_desc* d, const void* dy,
 #undef CALL
             scan_link_kernel<true><<<(unsigned)((n + LINK_COLS - 1) / LINK_COLS), LINK_COLS * LINK_RUNS, 0, st>>>(a);
         }
-        if (blocks > 0) {
-#define CALL(T, LN) scan_backward_kernel<T, LN><<<(unsigned)blocks, 256, 0, st>>>(a)
+        if (blocks + empty_blocks > 0) {
+#define CALL(T, LN) scan_backward_kernel<T, LN><<<(unsigned)(blocks + empty_blocks), 256, 0, st>>>(a)
             SCAN_DISPATCH(CALL)
 #undef CALL
         }
@@ -897,7 +976,6 @@ extern "C" int rec_history_scan_backward(const rec_scan_desc* d, const void* dy,
             else if (d->type == REC_TYPE_F16) scan_sum_groups_kernel<_Float16><<<(unsigned)sum_blocks, 256, 0, st>>>(a);
             else scan_sum_groups_kernel<__bf16><<<(unsigned)sum_blocks, 256, 0, st>>>(a);
         }
-        if (empty_blocks > 0) scan_empty_kernel<<<(unsigned)empty_blocks, 256, 0, st>>>(a, dfinal, out->dinitial);
         HIP_TRY(hipGetLastError());
         if (!params) return 0;
         return launch_sum_partials(part_a, c.chunks, n + 2 * d->channels, out->dA, n, out->dD, d->channels, out->ddelta_bias, st);
@@ -922,13 +1000,20 @@ extern "C" int rec_history_scan_step(const rec_scan_desc* d, const rec_scan_inpu
         ScanArgs a = {};
         fill(a, d, in, c);
         a.y = y; a.y_stride = y_stride;
-        const int64_t blocks = d->rows * c.tiles;
-        if (int rc = check_blocks(blocks)) return rc;
+        // four states of B and C in one load: no group's last four reach into the next, and all begin on a multiple of four
+        const size_t four = 4 * (size_t)rec_type_size(d->type);
+        const bool whole = d->states == 4 * lanes_of(d->states) && rec_aligned(in->B, four) && rec_aligned(in->C, four) && in->B_stride % 4 == 0 && in->C_stride % 4 == 0;
         DeviceScope scope;
         HIP_TRY(scope.enter(d->device));
-#define CALL(T, LN) scan_step_kernel<T, LN><<<(unsigned)blocks, 256, 0, (hipStream_t)stream>>>(a, slots, state)
-        SCAN_DISPATCH(CALL)
+        if (whole) {
+#define CALL(T, LN) scan_step_kernel<T, LN, true><<<(unsigned)d->rows, 256, 0, (hipStream_t)stream>>>(a, slots, state)
+            SCAN_DISPATCH(CALL)
 #undef CALL
+        } else {
+#define CALL(T, LN) scan_step_kernel<T, LN, false><<<(unsigned)d->rows, 256, 0, (hipStream_t)stream>>>(a, slots, state)
+            SCAN_DISPATCH(CALL)
+#undef CALL
+        }
         HIP_TRY(hipGetLastError());
         return 0;
     });

@@ -145,17 +145,26 @@ template <int LN> __device__ __forceinline__ float row_sum_strided(float v)
     return v;
 }
 
-// Rows of a step that name the same slot: `earlier`, whether a row in front of `row` names `slot`, `later`, whether one behind
-// it does.  The block's threads share the reading of the slots; every thread of the block calls it with the block's row.
-__device__ __forceinline__ void slot_is_shared(const int32_t* __restrict__ slots, int64_t rows, int64_t row, int slot, bool& earlier, bool& later)
+// Rows of a step that name the same slot.  The block's threads look through the slots together: each wavefront leaves what it has
+// seen in `seen` (bit 0: a row in front of `row` names `slot`, bit 1: one behind it does); behind the next barrier
+// slots_seen() joins them.
+__device__ __forceinline__ void look_for_slot(const int32_t* __restrict__ slots, int64_t rows, int64_t row, int slot, unsigned (&seen)[4])
 {
+    const int n = (int)rows, me = (int)row;   // a step has at most 65536 rows
     bool e = false, l = false;
-    for (int64_t i = threadIdx.x; i < rows; i += blockDim.x) {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
         const bool same = slots[i] == slot;
-        e |= same && i < row;
-        l |= same && i > row;
+        e |= same && i < me;
+        l |= same && i > me;
     }
-    earlier = __syncthreads_or(e);
-    later = __syncthreads_or(l);
+    const unsigned bits = (__any(e) ? 1u : 0u) | (__any(l) ? 2u : 0u);
+    if ((threadIdx.x & 63) == 0) seen[threadIdx.x >> 6] = bits;
+}
+__device__ __forceinline__ unsigned slots_seen(const unsigned (&seen)[4])
+{
+    unsigned bits = 0;
+    for (unsigned w = 0; w < blockDim.x / 64; w++) bits |= seen[w];
+    return bits;
 }
 #endif

@@ -100,6 +100,42 @@ def test_conv_and_gradient(case, layout):
     assert not y[:lo].any() and not y[hi:].any() and not g.dx[:lo].any() and not g.dx[hi:].any()
 
 
+@pytest.mark.parametrize("ch,W,tn", [(128, 4, "bf16"), (64, 3, "f32"), (96, 2, "f16")])
+def test_conv_long_strips_against_whole_arrays_in_64_bits(ch, W, tn):
+    """Enough rows for the longest strips; the reference shifts whole arrays on the GPU."""
+    src = Source(ch, TYPES[tn])
+    rows, n = 300001, 3000
+    off = torch.cat([torch.zeros(1, dtype=torch.int64), torch.randint(0, rows + 1, (n - 1,), generator=src.gen).sort().values, torch.tensor([rows])]).to(DEV)
+    x, dy = src(rows, ch)[0], src(rows, ch)[0]
+    w, b = src.f32(ch, W, scale=0.5)[0], src.f32(ch)[0]
+    x6, dy6, w6 = x.double(), dy.double(), w.double()
+    t = torch.arange(rows, device=DEV)
+    seq = torch.searchsorted(off, t, right=True) - 1
+    at, left = t - off[seq], off[seq + 1] - 1 - t
+
+    def behind(v, k):   # row t - k of the same history, or 0
+        return torch.where((at >= k)[:, None], torch.roll(v, k, 0), torch.zeros((), dtype=torch.float64, device=DEV))
+
+    def ahead(v, k):
+        return torch.where((left >= k)[:, None], torch.roll(v, -k, 0), torch.zeros((), dtype=torch.float64, device=DEV))
+
+    v, M = b.double().expand(rows, ch), b.double().abs().expand(rows, ch)
+    for j in range(W):
+        v, M = v + w6[:, j] * behind(x6, W - 1 - j), M + (w6[:, j] * behind(x6, W - 1 - j)).abs()
+    g = torch.sigmoid(v)
+    y, _ = ops.history_conv(x, w, b, seq_off=off)
+    close(y, (v * g).cpu(), (U * (1.1 * (W + 2) * M + (v * g).abs() * (M + 5))).cpu(), "y")
+    d, D = dy6 * g * (1 + v * (1 - g)), dy6.abs() * (1.1 + 0.5 * M)
+    got = ops.history_conv_backward(dy, x, w, b, seq_off=off)
+    c = U * (2 * W + 16 + float(M.max()))
+    want, size = sum(w6[:, W - 1 - k] * ahead(d, k) for k in range(W)), sum(w6[:, W - 1 - k].abs() * ahead(D, k) for k in range(W))
+    close(got.dx, want.cpu(), (c * size).cpu(), "dx")
+    dw, size = [(d * behind(x6, W - 1 - j)).sum(0) for j in range(W)], [(D * behind(x6, W - 1 - j).abs()).sum(0) for j in range(W)]
+    # a thread adds up at most 4 strips of 128 rows one after the other, a block's threads and the blocks after that
+    close(got.dweight, torch.stack(dw, 1).cpu(), ((c + U * 600) * torch.stack(size, 1)).cpu(), "dweight")
+    close(got.dbias, d.sum(0).cpu(), ((c + U * 600) * D.sum(0)).cpu(), "dbias")
+
+
 def test_conv_many_rows_over_blocks():
     """More rows than one walk of all blocks takes: the partial sums go around."""
     src = Source(5, torch.float32)
@@ -572,6 +608,10 @@ def test_nothing_to_do():
     none = torch.zeros(0, dtype=torch.int32, device=DEV)
     assert ops.history_conv_step(x, w, state=i.clone(), slots=none).shape == (0, 8)
     assert ops.history_scan_step(x, x, A, B, B, state=h.clone(), slots=none).shape == (0, 8)
+    # a pool without slots, and rows that name one all the same
+    lost = torch.zeros(3, dtype=torch.int32, device=DEV)
+    assert not ops.history_conv_step(torch.ones(3, 8, device=DEV), w, state=i[:0], slots=lost).any()
+    assert not ops.history_scan_step(torch.ones(3, 8, device=DEV), torch.ones(3, 8, device=DEV), A, torch.ones(3, 1, 4, device=DEV), torch.ones(3, 1, 4, device=DEV), state=h[:0], slots=lost).any()
     r = ops.policy_loss(torch.zeros(0, 9, device=DEV), none, torch.zeros(0, device=DEV), torch.zeros(0, device=DEV), grad_weight=torch.zeros(0, device=DEV))
     assert r.loss.shape == (0,) and r.dscores.shape == (0, 9)
     r = ops.preference_loss(torch.zeros(0, 9, device=DEV), none, offsets([0, 0, 0]))
