@@ -16,6 +16,7 @@
 namespace {
 
 constexpr int TT = REC_SCAN_CHECKPOINT;   // rows staged at a time
+constexpr int HALF = 8;                   // rows whose states the gradient keeps
 
 struct ScanArgs {
     const void *u, *delta, *z, *B, *C, *dy;
@@ -213,29 +214,49 @@ __global__ __launch_bounds__(LINK_COLS * LINK_RUNS) void scan_link_kernel(ScanAr
     // step k: forwards from chunk k, whose state goes to slot k + 1; backwards from chunk `steps - k`, whose gradient is in its own slot
     auto chunk_of = [&](int k) { return BACK ? steps - k : k; };
     auto slot_of = [&](int k) { return (int64_t)(BACK ? steps - k : k + 1) * n + i; };
+    // four steps' loads at a time: the stores in between keep the compiler from running ahead
+    constexpr int AHEAD = 4;
+    auto walk = [&](auto&& step) {
+        for (int k = k0; k < k1; k += AHEAD) {
+            int kind[AHEAD];
+            float own[AHEAD], span[AHEAD];
+#pragma unroll
+            for (int e = 0; e < AHEAD; e++) {
+                const int at = min(k + e, k1 - 1), c = chunk_of(at);
+                kind[e] = a.kind[c];
+                own[e] = a.link[slot_of(at)];
+                span[e] = a.span[(int64_t)c * a.channels + d];
+            }
+#pragma unroll
+            for (int e = 0; e < AHEAD; e++)
+                if (k + e < k1) step(k + e, kind[e], own[e], fast_exp2(A2 * span[e]));
+        }
+    };
     float P = 1.0f, H = 0.0f;
-    if (on) {
-#pragma unroll 4
-        for (int k = k0; k < k1; k++) {
-            const int c = chunk_of(k), kind = a.kind[c];
-            const float own = a.link[slot_of(k)], f = fast_exp2(A2 * a.span[(int64_t)c * a.channels + d]);
+    if (on)
+        walk([&](int, int kind, float own, float f) {
             P = kind == 2 ? P * f : 0.0f;
             H = kind == 2 ? fmaf(f, H, own) : kind == 1 ? own : 0.0f;
+        });
+    // what the runs up to each one lead to, by doubling
+    for (int o = 1; o < LINK_RUNS; o *= 2) {
+        sP[run][col] = P;
+        sH[run][col] = H;
+        __syncthreads();
+        if (run >= o) {
+            if (P != 0.0f) H = fmaf(P, sH[run - o][col], H);   // (a run that takes nothing over ignores what is in front of it, infinite or not)
+            P *= sP[run - o][col];
         }
+        __syncthreads();
     }
-    sP[run][col] = P;
     sH[run][col] = H;
     __syncthreads();
-    float h = 0.0f;
-    for (int r = 0; r < run; r++) h = sP[r][col] == 0.0f ? sH[r][col] : fmaf(sP[r][col], h, sH[r][col]);
+    float h = run > 0 ? sH[run - 1][col] : 0.0f;
     if (!on) return;
-#pragma unroll 4
-    for (int k = k0; k < k1; k++) {
-        const int c = chunk_of(k), kind = a.kind[c];
-        const float own = a.link[slot_of(k)], f = fast_exp2(A2 * a.span[(int64_t)c * a.channels + d]);
+    walk([&](int k, int kind, float own, float f) {
         h = kind == 2 ? fmaf(f, h, own) : kind == 1 ? own : 0.0f;
         a.link[slot_of(k)] = h;
-    }
+    });
 }
 
 // Sums over a channel's lanes are taken for GR rows together: lane j < GR of the channel keeps, and writes, row j's.
@@ -410,6 +431,15 @@ __global__ __launch_bounds__(256) void scan_local_backward_kernel(ScanArgs a)
     if (p.on && p.lane_n == 0) a.span[(int64_t)p.chunk * a.channels + p.d] = span;
 }
 
+// zeros instead of h, without a branch
+__device__ __forceinline__ void clear_if(float (&h)[4], bool clear)
+{
+    unsigned keep = __builtin_amdgcn_readfirstlane(clear ? 0u : ~0u);
+    asm volatile("" : "+s"(keep));   // or the cleared states of the walk forwards would be kept, next to the states, for the one backwards
+#pragma unroll
+    for (int e = 0; e < 4; e++) h[e] = __uint_as_float(__float_as_uint(h[e]) & keep);
+}
+
 // What is staged in LDS is read again behind this line: without it the compiler keeps all that the walk forwards has read
 // (160 registers) for the walk backwards.
 #define REC_READ_AGAIN()                          \
@@ -420,8 +450,8 @@ __global__ __launch_bounds__(256) void scan_local_backward_kernel(ScanArgs a)
 
 // third pass: per 16 rows, the states again from the checkpoint in front of them, then the gradient backwards.  A lane keeps the
 // tile's states in registers (64 of them).  Keeping the decays as well left room for one wavefront per SIMD instead of three.
-template <class T, int LN>
-__global__ __launch_bounds__(256, 2) void scan_backward_kernel(ScanArgs a)
+template <class T, int LN, bool STATES>
+__global__ __launch_bounds__(256, STATES ? 2 : 3) void scan_backward_kernel(ScanArgs a)
 {
     if ((int)blockIdx.x >= a.main_blocks) {
         pass_empty(a, a.dfinal, a.dinitial);
@@ -435,6 +465,7 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(ScanArgs a)
     __shared__ alignas(16) float sB[TT][NP], sC[TT][NP];
     __shared__ float s_in[TT][ROW], s_gB[TT][ROW], s_qA[TT][ROW];
     __shared__ alignas(16) float s_bc[4][TT][2][NP];           // dB, dC of each wavefront's channels
+    __shared__ float s_own[3][PT][256];            // what a thread wants back after the walk: u, the derivative of softplus, dy times the derivative of the gate
     const P p(a);
     const int64_t lo = a.off[0], hi = a.off[a.n_seq];
     float A2[4], G[4] = {0.0f, 0.0f, 0.0f, 0.0f}, dA[4] = {0.0f, 0.0f, 0.0f, 0.0f}, dD = 0.0f, dbias = 0.0f;
@@ -460,19 +491,19 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(ScanArgs a)
     for (int64_t t0 = (p.r1 - 1) / TT * TT; t0 >= p.r0; t0 -= TT) {
         const int nt = (int)(p.r1 - t0 < TT ? p.r1 - t0 : TT);
         unsigned bounds = 0;   // the tile's rows that begin a sequence, or the rows behind the last one
-        int s0 = s;            // the sequence of row t0
+        int q = s;
         for (int64_t b = begin; b >= t0;) {
             if (b < t0 + nt) bounds |= 1u << (b - t0);
             if (b == t0) break;
-            step_back(s0, b);
+            step_back(q, b);
         }
+        bounds = __builtin_amdgcn_readfirstlane(bounds);   // the same in every lane
         Q t;
         t.fetch(a, p, t0);
         float h0[4];   // the state in front of the tile
         load_states<LN>(a.checkpoints_in, t0 / TT, a, p.d, p.lane_n, p.on, h0);
         const int64_t blo = lo > t0 ? lo : t0, bhi = hi < t0 + nt ? hi : t0 + nt;
         __syncthreads();
-        float u[PT], dsp[PT], dgate[PT];   // u, the derivative of softplus, dy times the derivative of the gate
 #pragma unroll
         for (int k = 0; k < PT; k++) {
             const int r = Q::row(k);
@@ -480,99 +511,128 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(ScanArgs a)
             const float raw = to_f32(t.d[k]) + bias, gy = to_f32(t.g[k]), z = to_f32(t.z[k]);
             const float sp = computed(softplus_f32(raw)), ss = computed(sigmoid_f32(raw)), sz = computed(sigmoid_f32(z));
             const float delta = a.softplus ? sp : raw;
-            u[k] = to_f32(t.u[k]);
-            dsp[k] = a.softplus ? ss : 1.0f;
-            dgate[k] = gy * (sz * fmaf(z, 1.0f - sz, 1.0f));
-            sd[r][ch] = counts ? make_float2(delta, delta * u[k]) : make_float2(0.0f, 0.0f);
+            const float u = to_f32(t.u[k]);
+            s_own[0][k][threadIdx.x] = u;
+            s_own[1][k][threadIdx.x] = a.softplus ? ss : 1.0f;
+            s_own[2][k][threadIdx.x] = gy * (sz * fmaf(z, 1.0f - sz, 1.0f));
+            sd[r][ch] = counts ? make_float2(delta, delta * u) : make_float2(0.0f, 0.0f);
             sg[r][ch] = counts ? (a.z ? gy * (z * sz) : gy) : 0.0f;
         }
         t.stage_groups(a, t0, blo, bhi, sB, sC);
         __syncthreads();
-        // A tile in which no history begins is walked without a look at the bounds: one stretch of code, in which the reads of the
-        // rows ahead are in flight.
+        // Half a tile at a time, the later half first, so that only eight rows' states are kept (with sixteen there is room for two
+        // wavefronts per SIMD instead of three).  A tile in which no history begins is walked without a look at the bounds.
         auto walk = [&](auto bounded) {
             constexpr bool BOUNDED = decltype(bounded)::value;
-            float hs[TT][4];   // the state behind each row
-            if (BOUNDED && (bounds & 1)) load_states<LN>(s0 >= 0 && s0 < a.n_seq ? a.initial : nullptr, s0, a, p.d, p.lane_n, p.on, h0);
+            // the state of row r from the one in front of it
+            auto enter = [&](int r, float (&h)[4]) {
+                if (!BOUNDED) return;
+                const bool bound = (bounds >> r) & 1;
+                if (!STATES) {
+                    clear_if(h, bound);
+                } else if (bound) {
+                    const int at = sequence_of(a.off, a.n_seq, t0 + r);
+                    load_states<LN>(at >= 0 && at < a.n_seq ? a.initial : nullptr, at, a, p.d, p.lane_n, p.on, h);
+                }
+            };
+#pragma unroll 1
+            for (int half = TT - HALF; half >= 0; half -= HALF) {
+                float h[4], first[4], hs[HALF][4];   // the state in front of the half, and behind each of its rows
 #pragma unroll
-            for (int r0 = 0; r0 < TT; r0 += GR) {
-                float y[GR];
+                for (int e = 0; e < 4; e++) h[e] = h0[e];
+                if (half > 0) {
 #pragma unroll
-                for (int k = 0; k < GR; k++) {
-                    const int r = r0 + k;
-                    if (r % 4 == 0) REC_READ_AGAIN();
-                    float h[4];
+                    for (int r = 0; r < HALF; r++) {
+                        enter(r, h);
+                        const float2 v = sd[r][p.ch];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) h[e] = r == 0 ? h0[e] : hs[r > 0 ? r - 1 : 0][e];
-                    if (BOUNDED && r > 0 && ((bounds >> r) & 1)) {
-                        if (a.initial)
-                            do s0++; while (s0 < a.n_seq && a.off[s0 + 1] <= t0 + r);
-                        load_states<LN>(s0 >= 0 && s0 < a.n_seq ? a.initial : nullptr, s0, a, p.d, p.lane_n, p.on, h);
+                        for (int e = 0; e < 4; e++) h[e] = fmaf(fast_exp2(v.x * A2[e]), h[e], v.y * sB[r][p.lane_n + e]);
                     }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) first[e] = h[e];
+#pragma unroll
+                for (int r0 = 0; r0 < HALF; r0 += GR) {
+                    float y[GR];
+#pragma unroll
+                    for (int k = 0; k < GR; k++) {
+                        const int i = r0 + k, r = half + i;
+                        if (i % 4 == 0) REC_READ_AGAIN();
+#pragma unroll
+                        for (int e = 0; e < 4; e++) h[e] = i == 0 ? first[e] : hs[i > 0 ? i - 1 : 0][e];
+                        enter(r, h);
+                        const float2 v = sd[r][p.ch];
+                        y[k] = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            hs[i][e] = fmaf(fast_exp2(v.x * A2[e]), h[e], v.y * sB[r][p.lane_n + e]);
+                            y[k] = fmaf(hs[i][e], sC[r][p.lane_n + e], y[k]);
+                        }
+                    }
+                    if (a.z) write_sums<LN, GR>(s_in, half + r0, p.ch, y);
+                }
+                float vB[2][4], vC[2][4], gB[GR], qA[GR];
+#pragma unroll
+                for (int i = HALF - 1; i >= 0; i--) {
+                    const int r = half + i;
+                    if (i % 2 == 1) REC_READ_AGAIN();
                     const float2 v = sd[r][p.ch];
-                    y[k] = 0.0f;
+                    const float ys = sg[r][p.ch];
+                    float hb[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) hb[e] = i == 0 ? first[e] : hs[i > 0 ? i - 1 : 0][e];
+                    enter(r, hb);
+                    gB[i % GR] = qA[i % GR] = 0.0f;
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        hs[r][e] = fmaf(fast_exp2(v.x * A2[e]), h[e], v.y * sB[r][p.lane_n + e]);
-                        y[k] = fmaf(hs[r][e], sC[r][p.lane_n + e], y[k]);
+                        const float b = sB[r][p.lane_n + e];
+                        const float g = fmaf(sC[r][p.lane_n + e], ys, G[e]);
+                        vB[i % 2][e] = g * v.y;
+                        vC[i % 2][e] = hs[i][e] * ys;
+                        gB[i % GR] = fmaf(g, b, gB[i % GR]);
+                        G[e] = fast_exp2(v.x * A2[e]) * g;
+                        const float q = G[e] * hb[e];
+                        qA[i % GR] = fmaf(q, A2[e], qA[i % GR]);   // (A, times ln 2 below)
+                        dA[e] = fmaf(q, v.x, dA[e]);
                     }
-                }
-                if (a.z) write_sums<LN, GR>(s_in, r0, p.ch, y);
-            }
-            float vB[2][4], vC[2][4], gB[GR], qA[GR];
+                    if (BOUNDED) {
+                        const bool bound = (bounds >> r) & 1;
+                        if (!STATES) {
+                            clear_if(G, bound);
+                        } else if (bound) {   // in front of this row another sequence ends, or none does
+                            if (s >= 0 && s < a.n_seq && a.dinitial) store_states<LN>(a.dinitial, s, a, p.d, p.lane_n, p.on, G);
+                            step_back(s, begin);
+                            load_states<LN>(s >= 0 ? a.dfinal : nullptr, s, a, p.d, p.lane_n, p.on, G);
+                        }
+                    }
+                    if (i % GR == 0) {
+                        write_sums<LN, GR>(s_gB, r, p.ch, gB);
+                        write_sums<LN, GR>(s_qA, r, p.ch, qA);
+                    }
+                    if (i % 2 == 0) {
+                        // Two rows' 16 values, over the wavefront's channels: each fold halves the values and leaves the halves of the
+                        // lanes with different ones (bit 5 of the lane: the row, bit 4: dB or dC); what is left is summed inside 16 lanes.
+                        float w[4];
 #pragma unroll
-            for (int r = TT - 1; r >= 0; r--) {
-                if (r % 2 == 1) REC_READ_AGAIN();
-                const float2 v = sd[r][p.ch];
-                const float ys = sg[r][p.ch];
-                float hb[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) hb[e] = r == 0 ? h0[e] : hs[r > 0 ? r - 1 : 0][e];
-                const bool bound = BOUNDED && ((bounds >> r) & 1);
-                if (r > 0 && bound) load_states<LN>(s >= 0 && s < a.n_seq ? a.initial : nullptr, s, a, p.d, p.lane_n, p.on, hb);
-                gB[r % GR] = qA[r % GR] = 0.0f;
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float b = sB[r][p.lane_n + e];
-                    const float g = fmaf(sC[r][p.lane_n + e], ys, G[e]);
-                    vB[r % 2][e] = g * v.y;
-                    vC[r % 2][e] = hs[r][e] * ys;
-                    gB[r % GR] = fmaf(g, b, gB[r % GR]);
-                    G[e] = fast_exp2(v.x * A2[e]) * g;
-                    const float q = G[e] * hb[e];
-                    qA[r % GR] = fmaf(q, A2[e], qA[r % GR]);   // (A, times ln 2 below)
-                    dA[e] = fmaf(q, v.x, dA[e]);
-                }
-                if (bound) {   // in front of this row another sequence ends, or none does
-                    if (s >= 0 && s < a.n_seq && a.dinitial) store_states<LN>(a.dinitial, s, a, p.d, p.lane_n, p.on, G);
-                    step_back(s, begin);
-                    load_states<LN>(s >= 0 ? a.dfinal : nullptr, s, a, p.d, p.lane_n, p.on, G);
-                }
-                if (r % GR == 0) {
-                    write_sums<LN, GR>(s_gB, r, p.ch, gB);
-                    write_sums<LN, GR>(s_qA, r, p.ch, qA);
-                }
-                if (r % 2 == 0) {
-                    // Two rows' 16 values, over the wavefront's channels: each fold halves the values and leaves the halves of the
-                    // lanes with different ones (bit 5 of the lane: the row, bit 4: dB or dC); what is left is summed inside 16 lanes.
-                    float w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) w[e] = row_sum_strided<LN>(fold16(fold32(vB[0][e], vB[1][e]), fold32(vC[0][e], vC[1][e])));
-                    float* to = s_bc[wave][r + (lane >> 5)][(lane >> 4) & 1] + p.lane_n;
-                    const int copy = lane % 16 / LN;   // lanes with the same sums
-                    if constexpr (LN <= 4) {
-                        const float mine4 = copy == 0 ? w[0] : copy == 1 ? w[1] : copy == 2 ? w[2] : w[3];
-                        if (copy < 4) to[copy] = mine4;
-                    } else if constexpr (LN == 8) {
-                        *reinterpret_cast<float2*>(to + 2 * copy) = copy ? make_float2(w[2], w[3]) : make_float2(w[0], w[1]);
-                    } else {
-                        *reinterpret_cast<float4*>(to) = make_float4(w[0], w[1], w[2], w[3]);
+                        for (int e = 0; e < 4; e++) w[e] = row_sum_strided<LN>(fold16(fold32(vB[0][e], vB[1][e]), fold32(vC[0][e], vC[1][e])));
+                        float* to = s_bc[wave][r + (lane >> 5)][(lane >> 4) & 1] + p.lane_n;
+                        const int copy = lane % 16 / LN;   // lanes with the same sums
+                        if constexpr (LN <= 4) {
+                            const float mine4 = copy == 0 ? w[0] : copy == 1 ? w[1] : copy == 2 ? w[2] : w[3];
+                            if (copy < 4) to[copy] = mine4;
+                        } else if constexpr (LN == 8) {
+                            *reinterpret_cast<float2*>(to + 2 * copy) = copy ? make_float2(w[2], w[3]) : make_float2(w[0], w[1]);
+                        } else {
+                            *reinterpret_cast<float4*>(to) = make_float4(w[0], w[1], w[2], w[3]);
+                        }
                     }
                 }
             }
         };
         if (bounds == 0) walk(std::false_type{});
         else walk(std::true_type{});
+        if (!STATES)
+            while (begin >= t0) { if (begin == 0) break; step_back(s, begin); }
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < PT; k++) {
@@ -588,11 +648,12 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(ScanArgs a)
             }
             const float2 v = sd[r][ch];
             const float ys = sg[r][ch], g = s_gB[r][ch];
-            const float dd = fmaf(u[k], g, s_qA[r][ch] * 0.69314718055994530942f) * dsp[k];
+            const float u = s_own[0][k][threadIdx.x];
+            const float dd = fmaf(u, g, s_qA[r][ch] * 0.69314718055994530942f) * s_own[1][k][threadIdx.x];
             ((T*)a.du)[at] = from_f32<T>(a.D ? fmaf(v.x, g, Dd * ys) : v.x * g);
             ((T*)a.ddelta)[at] = from_f32<T>(dd);
-            if (a.z) ((T*)a.dz)[at] = from_f32<T>(dgate[k] * (a.D ? fmaf(Dd, u[k], s_in[r][ch]) : s_in[r][ch]));
-            dD = fmaf(ys, u[k], dD);
+            if (a.z) ((T*)a.dz)[at] = from_f32<T>(s_own[2][k][threadIdx.x] * (a.D ? fmaf(Dd, u, s_in[r][ch]) : s_in[r][ch]));
+            dD = fmaf(ys, u, dD);
             dbias += dd;
         }
         // dB and dC of the block's channels: the four wavefronts in order
@@ -625,18 +686,22 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(ScanArgs a)
     }
 }
 
-// dB and dC where a group's channels are spread over blocks
+// dB and dC where a group's channels are spread over blocks: 32 rows a block, a row's values on neighbouring threads
+constexpr int SUM_ROWS = 32;
 template <class T>
 __global__ __launch_bounds__(256) void scan_sum_groups_kernel(ScanArgs a)
 {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per_row = (int64_t)a.groups * 2 * a.states, n = a.rows * per_row;
-    if (i >= n) return;
-    const int64_t row = i / per_row;
-    if ((row < a.off[0] || row >= a.off[a.n_seq]) && !a.zero_rest) return;
-    float v = 0.0f;
-    for (int k = 0; k < a.tiles_per_group; k++) v += a.part_bc[k * n + i];
-    const int64_t at = (i / (2 * a.states)) * a.states + i % a.states;
-    ((T*)(i / a.states % 2 ? a.dC : a.dB))[at] = from_f32<T>(v);
+    const int per_row = a.groups * 2 * a.states, n = per_row * SUM_ROWS;
+    const int64_t row0 = (int64_t)blockIdx.x * SUM_ROWS, lo = a.off[0], hi = a.off[a.n_seq];
+    const float* part = a.part_bc + row0 * per_row;
+    for (int i = threadIdx.x; i < n; i += 256) {
+        const int r = i / per_row, at = i - r * per_row, pair = at / a.states, v = at - pair * a.states;   // pair: group * 2 + (B or C)
+        const int64_t row = row0 + r;
+        if (row >= a.rows || ((row < lo || row >= hi) && !a.zero_rest)) continue;
+        float sum = 0.0f;
+        for (int k = 0; k < a.tiles_per_group; k++) sum += part[k * (a.rows * per_row) + i];
+        ((T*)(pair & 1 ? a.dC : a.dB))[(row * a.groups + pair / 2) * a.states + v] = from_f32<T>(sum);
+    }
 }
 
 // ---- single clicks: a block per row; bound by the state, which is read and written once (4 bytes a value each way), and by
@@ -810,7 +875,7 @@ int lanes_of(int states) { return states <= 4 ? 1 : states <= 8 ? 2 : states <= 
 // handed over, so chunks are as long as they can be while the launch still fills the chip: `blocks` of them, between 16 and
 // 512 rows.
 struct Cut { int tiles_per_group, tiles, chunk, chunks; };
-constexpr int kForwardBlocks = 2048, kBackwardBlocks = 2048;
+constexpr int kForwardBlocks = 2048, kBackwardBlocks = 3072;
 Cut cut_of(const rec_scan_desc* d, int blocks)
 {
     Cut c;
@@ -942,7 +1007,7 @@ extern "C" int rec_history_scan_backward(const rec_scan_desc* d, const void* dy,
         const Cut c = cut_of(d, kBackwardBlocks);
         const int64_t blocks = (int64_t)c.chunks * c.tiles, n = (int64_t)d->channels * d->states;
         const int64_t empty_blocks = out->dinitial ? (n * d->n_seq + 255) / 256 : 0;
-        const int64_t sum_blocks = c.tiles_per_group > 1 ? (d->rows * d->groups * 2 * d->states + 255) / 256 : 0;
+        const int64_t sum_blocks = c.tiles_per_group > 1 ? (d->rows + SUM_ROWS - 1) / SUM_ROWS : 0;
         if (int rc = check_blocks(blocks + empty_blocks > sum_blocks ? blocks + empty_blocks : sum_blocks)) return rc;
         const bool params = out->dA || out->dD || out->ddelta_bias;
         ScanArgs a = {};
@@ -967,9 +1032,16 @@ extern "C" int rec_history_scan_backward(const rec_scan_desc* d, const void* dy,
             scan_link_kernel<true><<<(unsigned)((n + LINK_COLS - 1) / LINK_COLS), LINK_COLS * LINK_RUNS, 0, st>>>(a);
         }
         if (blocks + empty_blocks > 0) {
-#define CALL(T, LN) scan_backward_kernel<T, LN><<<(unsigned)(blocks + empty_blocks), 256, 0, st>>>(a)
-            SCAN_DISPATCH(CALL)
+            // without states handed in or out, a history's beginning is a zero
+            if (in->initial || dfinal || out->dinitial) {
+#define CALL(T, LN) scan_backward_kernel<T, LN, true><<<(unsigned)(blocks + empty_blocks), 256, 0, st>>>(a)
+                SCAN_DISPATCH(CALL)
 #undef CALL
+            } else {
+#define CALL(T, LN) scan_backward_kernel<T, LN, false><<<(unsigned)(blocks + empty_blocks), 256, 0, st>>>(a)
+                SCAN_DISPATCH(CALL)
+#undef CALL
+            }
         }
         if (sum_blocks > 0) {
             if (d->type == REC_TYPE_F32) scan_sum_groups_kernel<float><<<(unsigned)sum_blocks, 256, 0, st>>>(a);

@@ -201,6 +201,10 @@ SCAN = [  # type, channels, groups, states, offsets, rows, gate, D, bias, softpl
     ("f16", 18, 1, 61, [0, 47, 48], 48, True, True, False, True, False),
     ("f32", 300, 1, 3, [0, 17, 90], 90, True, True, True, True, True),
     ("f32", 12, 2, 7, [0, 0, 0], 4, True, True, True, True, True),
+    ("f32", 48, 2, 16, [1, 4, 4, 20, 21, 22, 23, 40, 56, 72, 150], 160, True, True, True, True, False),
+    ("bf16", 20, 1, 32, [0, 16, 31, 64, 65, 96], 96, True, True, True, True, False),
+    ("f16", 40, 1, 2, [0, 1, 2, 3, 4, 5, 6, 7, 8, 60], 60, True, False, True, True, False),
+    ("bf16", 33, 1, 8, [0, 40, 48, 100], 100, False, True, True, True, False),
 ]
 
 
@@ -246,7 +250,7 @@ def test_scan_and_gradient(case, layout):
     tn, ch, G, N, off, rows, gate, has_D, has_bias, sp, has_init = case
     src, x, six, init = scan_inputs(case, layout)
     S = len(off) - 1
-    (dy, dy6), (df, df6) = src(rows, ch), src.f32(S, ch, N)
+    (dy, dy6), (df, df6) = src(rows, ch), src.f32(S, ch, N) if has_init else (None, None)   # (states in and out go together or not at all)
     if layout == "strided":
         dy = strided(dy, 7, 1)
     y, fin, kept = ops.history_scan(*x, seq_off=offsets(off), initial=init, softplus=sp, want_final=True, want_checkpoints=True)
@@ -273,15 +277,15 @@ def test_scan_and_gradient(case, layout):
         assert not t[:off[0]].any() and not t[off[-1]:].any()
 
 
-@pytest.mark.parametrize("tn,ch,G,N,longest", [("f32", 512, 2, 16, 2100), ("bf16", 96, 1, 16, 9000)])
-def test_scan_over_many_chunks_equals_one_row_after_the_other(tn, ch, G, N, longest):
+@pytest.mark.parametrize("tn,ch,G,N,longest,states", [("f32", 512, 2, 16, 2100, True), ("bf16", 96, 1, 16, 9000, True), ("f32", 200, 1, 16, 5000, False)])
+def test_scan_over_many_chunks_equals_one_row_after_the_other(tn, ch, G, N, longest, states):
     """Histories that cross from chunk to chunk, against a float64 recurrence on the GPU, gradients included."""
     off = [0, 7, longest, longest, longest + 400]
     rows = off[-1]
-    case = (tn, ch, G, N, off, rows, True, True, True, True, True)
+    case = (tn, ch, G, N, off, rows, True, True, True, True, states)
     src, x, six, init = scan_inputs(case)
-    (dy, dy6), (df, df6) = src(rows, ch), src.f32(4, ch, N)
-    on = {k: t.to(DEV) for k, t in six.items()}
+    (dy, dy6), (df, df6) = src(rows, ch), src.f32(4, ch, N) if states else (None, None)
+    on = {k: t.to(DEV) if t is not None else None for k, t in six.items()}
     y6, fin6 = ref.scan(**on, off=off)
     ya, _ = ref.scan(**on, off=off, absolute=True)
     y, fin, kept = ops.history_scan(*x, seq_off=offsets(off), initial=init, want_final=True, want_checkpoints=True)
@@ -289,10 +293,12 @@ def test_scan_over_many_chunks_equals_one_row_after_the_other(tn, ch, G, N, long
     few = U * (300 * 12 + N + 64)
     close(y, y6.cpu(), few * ya.cpu(), "y")
     g = ops.history_scan_backward(dy, *x, seq_off=offsets(off), checkpoints=kept, initial=init, dfinal=df)
-    want = ref.scan_gradient(dy6.to(DEV), **on, off=off, dfinal=df6.to(DEV))
-    size = ref.scan_gradient(dy6.to(DEV), **on, off=off, dfinal=df6.to(DEV), absolute=True)
+    df6 = df6.to(DEV) if states else None
+    want = ref.scan_gradient(dy6.to(DEV), **on, off=off, dfinal=df6)
+    size = ref.scan_gradient(dy6.to(DEV), **on, off=off, dfinal=df6, absolute=True)
     for name, got in (("u", g.du), ("delta", g.ddelta), ("B", g.dB), ("C", g.dC), ("z", g.dz), ("initial", g.dinitial)):
-        close(got, want[name].cpu(), 2 * few * size[name].cpu(), name)
+        if got is not None:
+            close(got, want[name].cpu(), 2 * few * size[name].cpu(), name)
     for name, got in (("A", g.dA), ("D", g.dD), ("bias", g.ddelta_bias)):
         close(got, want[name].cpu(), (2 * few + U * rows) * size[name].cpu(), name)
 
