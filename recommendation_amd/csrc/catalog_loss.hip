@@ -46,11 +46,11 @@ __device__ __forceinline__ Stat join(Stat a, Stat b, float c)
     return {m, a.l * fa + b.l * fb, a.ls * fa + b.ls * fb, (fa > 0.0f ? fmaf(da, a.ls, a.qs) * fa : 0.0f) + (fb > 0.0f ? fmaf(db, b.ls, b.qs) * fb : 0.0f)};
 }
 
+// over a wavefront, in every lane: everyone moves to the common maximum first, so that plain sums are left
 __device__ __forceinline__ Stat join_lanes(Stat st, float c)
 {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) st = join(st, {__shfl_xor(st.m, o, 64), __shfl_xor(st.l, o, 64), __shfl_xor(st.ls, o, 64), __shfl_xor(st.qs, o, 64)}, c);
-    return st;
+    const float m = wave_max(st.m), base = m == -INFINITY ? 0.0f : m, d = st.m == -INFINITY ? 0.0f : st.m - base, f = fast_exp2(d * c);
+    return {m, group_sum_dpp<64>(st.l * f), group_sum_dpp<64>(st.ls * f), group_sum_dpp<64>(f > 0.0f ? fmaf(d, st.ls, st.qs) * f : 0.0f)};
 }
 
 // N vectors of V scores into a thread's statistics
@@ -105,16 +105,15 @@ template <class T> __device__ __forceinline__ Vectors vectors_of(const T* row, i
     return r;
 }
 
-// the statistics of the scores [j0, j1) of a row, over the block; valid in every thread.  NaN scores give a NaN sum.
+// what thread `tid` of `step` finds in the scores [j0, j1) of a row.  NaN scores give a NaN sum.
 template <class T>
-__device__ __forceinline__ Stat row_statistics(const T* __restrict__ row, int64_t j0, int64_t j1, float c, Stat* red)
+__device__ __forceinline__ Stat thread_statistics(const T* __restrict__ row, int64_t j0, int64_t j1, float c, int tid, int step)
 {
     constexpr int V = 16 / sizeof(T), N = 4;   // four loads in flight per thread
     Stat st = {-INFINITY, 0.0f, 0.0f, 0.0f};
     const Vectors w = vectors_of(row, j0, j1);
     const Pack<T, V>* p = reinterpret_cast<const Pack<T, V>*>(row + w.lead);
-    const int step = blockDim.x;
-    int64_t i = threadIdx.x;
+    int64_t i = tid;
     for (; i + (N - 1) * step < w.n; i += N * step) {
         Pack<T, V> raw[N];
 #pragma unroll
@@ -130,18 +129,25 @@ __device__ __forceinline__ Stat row_statistics(const T* __restrict__ row, int64_
         add_scores<V, 1>(st, x, c);
     }
     const int64_t n = (w.lead - j0) + (j1 - w.tail);   // at most 2 V - 2
-    if ((int64_t)threadIdx.x < n) {
-        const int64_t j = (int64_t)threadIdx.x < w.lead - j0 ? j0 + threadIdx.x : w.tail + (threadIdx.x - (w.lead - j0));
+    if (tid < n) {
+        const int64_t j = tid < w.lead - j0 ? j0 + tid : w.tail + (tid - (w.lead - j0));
         const float x[1][1] = {{to_f32(row[j])}};
         add_scores<1, 1>(st, x, c);
     }
-    st = join_lanes(st, c);
+    return st;
+}
+
+// over the block, valid in every thread
+template <class T>
+__device__ __forceinline__ Stat row_statistics(const T* __restrict__ row, int64_t j0, int64_t j1, float c, Stat* red)
+{
+    Stat st = join_lanes(thread_statistics(row, j0, j1, c, threadIdx.x, blockDim.x), c);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = st;
     __syncthreads();
-    st = red[0];
-    for (int k = 1; k < (int)blockDim.x / 64; k++) st = join(st, red[k], c);
-    return st;
+    const int waves = blockDim.x / 64, lane = threadIdx.x & 63;   // at most 16: every wavefront joins them for itself
+    st = lane < waves ? red[lane] : Stat{-INFINITY, 0.0f, 0.0f, 0.0f};
+    return join_lanes(st, c);
 }
 
 __device__ __forceinline__ bool row_counts(const LossArgs& a, int64_t row)
@@ -180,6 +186,20 @@ __device__ __forceinline__ bool row_log_probability(const LossArgs& a, int64_t r
 }
 
 __device__ __forceinline__ double softplus64(double v) { return fmax(v, 0.0) + log1p(exp(-fabs(v))); }
+
+__device__ __forceinline__ void pair_loss(const LossArgs& a, int64_t p, double m)
+{
+    a.margin[p] = (float)m;
+    double loss = 0.0;   // a term with weight 0 adds nothing, be it infinite
+    if (a.smoothing < 1.0) loss += (1.0 - a.smoothing) * softplus64(-m);
+    if (a.smoothing > 0.0) loss += a.smoothing * softplus64(m);
+    a.loss[p] = (float)loss;
+}
+// d(weighted loss) / d(log p) of the preferred list's rows; the other list's have the opposite
+__device__ __forceinline__ float pair_coef(const LossArgs& a, int64_t p, double m)
+{
+    return (float)(a.beta * (a.smoothing - 1.0 / (1.0 + exp(m))) * (double)a.grad_weight[p]);
+}
 
 // A block per pair adds up its two lists' rows in a fixed order: a thread per row, or a wavefront where a row has several parts.
 template <class T>
@@ -225,15 +245,9 @@ __global__ __launch_bounds__(256) void preference_kernel(LossArgs a)
         __syncthreads();
     }
     const double m = a.beta * red[0];
-    if (threadIdx.x == 0) {
-        a.margin[p] = (float)m;
-        double loss = 0.0;   // a term with weight 0 adds nothing, be it infinite
-        if (a.smoothing < 1.0) loss += (1.0 - a.smoothing) * softplus64(-m);
-        if (a.smoothing > 0.0) loss += a.smoothing * softplus64(m);
-        a.loss[p] = (float)loss;
-    }
+    if (threadIdx.x == 0) pair_loss(a, p, m);
     if (!a.grad_weight) return;
-    const float c = (float)(a.beta * (a.smoothing - 1.0 / (1.0 + exp(m))) * (double)a.grad_weight[p]);
+    const float c = pair_coef(a, p, m);
     for (int64_t row = begin[0] + threadIdx.x; row < begin[2]; row += 256) a.coef[row] = a.coef[row] == 0.0f ? 0.0f : a.coef[row] * c;
 }
 
@@ -283,7 +297,7 @@ __global__ __launch_bounds__(256) void policy_kernel(LossArgs a)
 // The gradient's elements [j0, j1) of a row, from its end to its beginning: where the same block has just read the row, what it
 // read last is still in the cache.
 template <class T>
-__device__ __forceinline__ void write_gradient(const LossArgs& a, int64_t row, int64_t j0, int64_t j1, float coef, float m, float l)
+__device__ __forceinline__ void write_gradient(const LossArgs& a, int64_t row, int64_t j0, int64_t j1, float coef, float m, float l, int tid, int step)
 {
     constexpr int V = 16 / sizeof(T), N = 4;
     const T* in = (const T*)a.scores + row * a.scores_stride;
@@ -313,22 +327,21 @@ __device__ __forceinline__ void write_gradient(const LossArgs& a, int64_t row, i
         }
         return o;
     };
-    const int step = blockDim.x;
     const int64_t whole = w.n / (N * step) * (N * step);
-    for (int64_t i = whole + threadIdx.x; i < w.n; i += step) q[i] = vector_of(p[i], i);
-    for (int64_t i = whole - N * step + threadIdx.x; i >= 0; i -= N * step) {
+    for (int64_t i = whole + tid; i < w.n; i += step) q[i] = vector_of(p[i], i);
+    for (int64_t i = whole - N * step + tid; i >= 0; i -= N * step) {
         Pack<T, V> raw[N];
 #pragma unroll
         for (int n = 0; n < N; n++) raw[n] = p[i + n * step];
 #pragma unroll
         for (int n = 0; n < N; n++) q[i + n * step] = vector_of(raw[n], i + n * step);
     }
-    for (int64_t j = j0 + threadIdx.x; j < w.lead; j += step) out[j] = from_f32<T>(of(to_f32(in[j]), j));
-    for (int64_t j = w.tail + threadIdx.x; j < j1; j += step) out[j] = from_f32<T>(of(to_f32(in[j]), j));
+    for (int64_t j = j0 + tid; j < w.lead; j += step) out[j] = from_f32<T>(of(to_f32(in[j]), j));
+    for (int64_t j = w.tail + tid; j < j1; j += step) out[j] = from_f32<T>(of(to_f32(in[j]), j));
 }
 
 template <class T>
-__device__ __forceinline__ void write_zeros(const LossArgs& a, int64_t row, int64_t j0, int64_t j1)
+__device__ __forceinline__ void write_zeros(const LossArgs& a, int64_t row, int64_t j0, int64_t j1, int tid, int step)
 {
     constexpr int V = 16 / sizeof(T);
     T* out = (T*)a.dscores + row * a.dscores_stride;
@@ -336,9 +349,9 @@ __device__ __forceinline__ void write_zeros(const LossArgs& a, int64_t row, int6
     Pack<T, V> zero;
 #pragma unroll
     for (int v = 0; v < V; v++) zero.v[v] = from_f32<T>(0.0f);
-    for (int64_t i = threadIdx.x; i < w.n; i += blockDim.x) reinterpret_cast<Pack<T, V>*>(out + w.lead)[i] = zero;
-    for (int64_t j = j0 + threadIdx.x; j < w.lead; j += blockDim.x) out[j] = zero.v[0];
-    for (int64_t j = w.tail + threadIdx.x; j < j1; j += blockDim.x) out[j] = zero.v[0];
+    for (int64_t i = tid; i < w.n; i += step) reinterpret_cast<Pack<T, V>*>(out + w.lead)[i] = zero;
+    for (int64_t j = j0 + tid; j < w.lead; j += step) out[j] = zero.v[0];
+    for (int64_t j = w.tail + tid; j < j1; j += step) out[j] = zero.v[0];
 }
 
 // Rows in falling order: the last ones that the statistics read are the ones still in the Infinity Cache.
@@ -350,13 +363,13 @@ __global__ __launch_bounds__(512) void gradient_kernel(LossArgs a)
     const int64_t per = (a.n_items + a.splits - 1) / a.splits, j1 = (split + 1) * per < a.n_items ? (split + 1) * per : a.n_items, j0 = split * per < j1 ? split * per : j1;
     if (a.off && (row < a.off[0] || row >= a.off[a.n_seq])) {
         if (!a.zero_rest) return;
-        write_zeros<T>(a, row, j0, j1);
+        write_zeros<T>(a, row, j0, j1, threadIdx.x, blockDim.x);
         if (split == 0 && threadIdx.x == 0) a.logp[row] = 0.0f;
         return;
     }
     const float coef = a.coef[row];
-    if (coef == 0.0f) write_zeros<T>(a, row, j0, j1);   // p is finite or the row's coefficient is NaN: nothing to read
-    else write_gradient<T>(a, row, j0, j1, coef, a.stat[row].x, a.stat[row].y);
+    if (coef == 0.0f) write_zeros<T>(a, row, j0, j1, threadIdx.x, blockDim.x);   // p is finite or the row's coefficient is NaN: nothing to read
+    else write_gradient<T>(a, row, j0, j1, coef, a.stat[row].x, a.stat[row].y, threadIdx.x, blockDim.x);
 }
 
 // The policy loss where a block takes whole rows: it reads a row twice, but the second time from the cache (two blocks of a
@@ -379,8 +392,64 @@ __global__ __launch_bounds__(1024) void policy_fused_kernel(LossArgs a)
     if (!a.dscores) return;
     __syncthreads();
     const float coef = coef_s;
-    if (coef == 0.0f) write_zeros<T>(a, row, 0, a.n_items);
-    else write_gradient<T>(a, row, 0, a.n_items, coef, st.m, st.l);
+    if (coef == 0.0f) write_zeros<T>(a, row, 0, a.n_items, threadIdx.x, blockDim.x);
+    else write_gradient<T>(a, row, 0, a.n_items, coef, st.m, st.l, threadIdx.x, blockDim.x);
+}
+
+// Few rows of few items: one launch, a block per pair, a wavefront per row (at most kSmallRows rows in the call, so in a pair).
+constexpr int kSmallRows = 64;
+template <class T>
+__global__ __launch_bounds__(1024) void preference_small_kernel(LossArgs a)
+{
+    __shared__ double gain[kSmallRows];
+    __shared__ float m_s[kSmallRows], l_s[kSmallRows];
+    __shared__ bool on_s[kSmallRows];
+    __shared__ float coef_s;
+    const int64_t p = blockIdx.x;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, rows = (int)a.rows;
+    int begin[3];
+#pragma unroll
+    for (int k = 0; k < 3; k++) {   // offsets that break the rules stay within the rows
+        const int64_t o = a.n_seq ? a.off[2 * p + k] : rows;
+        begin[k] = o < 0 ? 0 : o > rows ? rows : (int)o;
+    }
+    if (threadIdx.x < kSmallRows) gain[threadIdx.x] = 0.0;
+    __syncthreads();
+    for (int row = begin[0] + wave; row < begin[2]; row += 16) {
+        bool on = row_counts(a, row);
+        Stat st = {-INFINITY, 0.0f, 0.0f, 0.0f};
+        if (on) st = join_lanes(thread_statistics((const T*)a.scores + row * a.scores_stride, 0, a.n_items, a.scale2, lane, 64), a.scale2);
+        if (lane) continue;
+        double logp = 0.0;
+        on = on && row_log_probability<T>(a, row, st, logp);
+        a.logp[row] = (float)logp;
+        if (on && a.ref_logp) logp -= (double)a.ref_logp[row];
+        gain[row] = row < begin[1] ? logp : -logp;
+        m_s[row] = st.m;
+        l_s[row] = st.l;
+        on_s[row] = on;
+    }
+    __syncthreads();
+    if (wave == 0 && a.n_seq) {
+        const double m = a.beta * group_sum<64>(gain[lane]);
+        if (lane == 0) {
+            pair_loss(a, p, m);
+            coef_s = a.grad_weight ? pair_coef(a, p, m) : 0.0f;
+        }
+    }
+    if (blockIdx.x == 0 && a.zero_rest)   // rows of no list
+        for (int row = wave; row < rows; row += 16)
+            if (row < a.off[0] || row >= a.off[a.n_seq]) {
+                if (lane == 0) a.logp[row] = 0.0f;
+                if (a.dscores) write_zeros<T>(a, row, 0, a.n_items, lane, 64);
+            }
+    __syncthreads();
+    if (!a.dscores) return;
+    for (int row = begin[0] + wave; row < begin[2]; row += 16) {
+        const float coef = !on_s[row] ? 0.0f : row < begin[1] ? coef_s : -coef_s;
+        if (coef == 0.0f) write_zeros<T>(a, row, 0, a.n_items, lane, 64);
+        else write_gradient<T>(a, row, 0, a.n_items, coef, m_s[row], l_s[row], lane, 64);
+    }
 }
 
 // rows of no list, where no gradient pass comes by
@@ -475,6 +544,14 @@ extern "C" int rec_preference_loss(const rec_loss_desc* d, const void* scores, i
         DeviceScope scope;
         HIP_TRY(scope.enter(d->device));
         hipStream_t st = (hipStream_t)stream;
+        // (one pair of 6 x 2848 f32: three launches of 4.8, 4.0 and 3.4 us; 16 rows at a time pay for that up to some thousand items)
+        if (d->rows > 0 && d->rows <= kSmallRows && d->rows * d->n_items <= 131072) {
+#define CALL(T) preference_small_kernel<T><<<n_pairs ? (unsigned)n_pairs : 1u, 1024, 0, st>>>(a)
+            LOSS_DISPATCH(CALL)
+#undef CALL
+            HIP_TRY(hipGetLastError());
+            return 0;
+        }
         const unsigned blocks = (unsigned)(d->rows * a.splits);
 #define CALL(T)                                                                                     \
         if (blocks) row_statistics_kernel<T><<<blocks, kThreads, 0, st>>>(a);                       \

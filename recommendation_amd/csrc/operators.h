@@ -29,8 +29,7 @@ template <class F> int rec_guarded(F&& f)
 
 inline int rec_check_device(int device)
 {
-    int n = 0;
-    if (hipGetDeviceCount(&n) != hipSuccess) n = 0;
+    static const int n = [] { int c = 0; return hipGetDeviceCount(&c) == hipSuccess ? c : 0; }();
     REC_REFUSE(device < 0 || device >= n, "no such HIP device");
     return 0;
 }
@@ -121,6 +120,17 @@ __device__ __forceinline__ float softplus_f32(float v)
     p = fmaf(p, e, -0.4999990463256836f);
     p = fmaf(p, e, 1.0f);
     return fmaf(p, e, fmaxf(v, 0.0f));
+}
+
+// the largest of a wavefront's values, in every lane
+__device__ __forceinline__ float wave_max(float v)
+{
+    v = fmaxf(v, dpp_move<0xB1>(v));
+    v = fmaxf(v, dpp_move<0x4E>(v));
+    v = fmaxf(v, dpp_move<0x141>(v));
+    v = fmaxf(v, dpp_move<0x140>(v));
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return fmaxf(v, __shfl_xor(v, 32, 64));
 }
 
 // sums over lanes in pieces: lanes below 32 end up with a of both halves added, lanes from 32 on with b of both halves
