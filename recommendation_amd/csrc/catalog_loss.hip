@@ -480,6 +480,9 @@ int splits_of(const rec_loss_desc* d)
 }
 
 int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
+// one launch does it all, and nothing passes between launches
+bool small_preference(const rec_loss_desc* d) { return d->rows <= kSmallRows && d->rows * d->n_items <= 131072; }
+bool whole_policy(const rec_loss_desc* d) { return splits_of(d) == 1; }
 int64_t workspace_of(const rec_loss_desc* d) { return d->rows * splits_of(d) * 16 + round16(d->rows * 8) + round16(d->rows * 4); }
 
 int check_call(const rec_loss_desc* d, const void* scores, int64_t scores_stride, const float* grad_weight, int64_t weights, const void* dscores,
@@ -522,8 +525,8 @@ void fill(LossArgs& a, const rec_loss_desc* d, const void* scores, int64_t score
 extern "C" int64_t rec_preference_loss_workspace(const rec_loss_desc* d, int32_t n_pairs)
 {
     if (check_desc(d)) return -1;
-    if (n_pairs < 0) { rec_set_error("n_pairs must be in 0..2^22-1"); return -1; }
-    return workspace_of(d);
+    if (n_pairs < 0 || n_pairs > (1 << 22) - 1) { rec_set_error("n_pairs must be in 0..2^22-1"); return -1; }
+    return small_preference(d) ? 0 : workspace_of(d);
 }
 
 extern "C" int rec_preference_loss(const rec_loss_desc* d, const void* scores, int64_t scores_stride, const int32_t* item,
@@ -537,7 +540,7 @@ extern "C" int rec_preference_loss(const rec_loss_desc* d, const void* scores, i
         REC_REFUSE(!seq_off || (d->rows > 0 && (!scores || !item || !logp)) || (n_pairs > 0 && (!loss || !margin)), "null argument");
         REC_REFUSE(!isfinite(beta), "beta must be finite");
         REC_REFUSE(!(smoothing >= 0.0f && smoothing <= 1.0f), "smoothing must be in 0..1");
-        if (int rc = check_call(d, scores, scores_stride, grad_weight, n_pairs, dscores, dscores_stride, workspace, workspace_bytes, workspace_of(d))) return rc;
+        if (int rc = check_call(d, scores, scores_stride, grad_weight, n_pairs, dscores, dscores_stride, workspace, workspace_bytes, small_preference(d) ? 0 : workspace_of(d))) return rc;
         LossArgs a = {};
         fill(a, d, scores, scores_stride, item, ref_logp, grad_weight, loss, logp, dscores, dscores_stride, workspace);
         a.off = seq_off; a.n_seq = 2 * n_pairs; a.margin = margin; a.beta = beta; a.smoothing = smoothing;
@@ -545,7 +548,7 @@ extern "C" int rec_preference_loss(const rec_loss_desc* d, const void* scores, i
         HIP_TRY(scope.enter(d->device));
         hipStream_t st = (hipStream_t)stream;
         // (one pair of 6 x 2848 f32: three launches of 4.8, 4.0 and 3.4 us; 16 rows at a time pay for that up to some thousand items)
-        if (d->rows > 0 && d->rows <= kSmallRows && d->rows * d->n_items <= 131072) {
+        if (d->rows > 0 && small_preference(d)) {
 #define CALL(T) preference_small_kernel<T><<<n_pairs ? (unsigned)n_pairs : 1u, 1024, 0, st>>>(a)
             LOSS_DISPATCH(CALL)
 #undef CALL
@@ -568,7 +571,7 @@ extern "C" int rec_preference_loss(const rec_loss_desc* d, const void* scores, i
 extern "C" int64_t rec_policy_loss_workspace(const rec_loss_desc* d)
 {
     if (check_desc(d)) return -1;
-    return workspace_of(d);
+    return whole_policy(d) ? 0 : workspace_of(d);
 }
 
 extern "C" int rec_policy_loss(const rec_loss_desc* d, const void* scores, int64_t scores_stride, const int32_t* item,
@@ -581,7 +584,7 @@ extern "C" int rec_policy_loss(const rec_loss_desc* d, const void* scores, int64
         REC_REFUSE(d->rows > 0 && (!scores || !item || !old_logp || !advantage || !loss || !logp), "null argument");
         REC_REFUSE(!(clip_low >= 0.0f && clip_low <= 1.0f) || !(clip_high >= 0.0f) || !isfinite(clip_high), "clip_low must be in 0..1 and clip_high at least 0");
         REC_REFUSE(!isfinite(kl_coef) || (!ref_logp && kl_coef != 0.0f), "kl_coef must be finite, and 0 without ref_logp");
-        if (int rc = check_call(d, scores, scores_stride, grad_weight, d->rows, dscores, dscores_stride, workspace, workspace_bytes, workspace_of(d))) return rc;
+        if (int rc = check_call(d, scores, scores_stride, grad_weight, d->rows, dscores, dscores_stride, workspace, workspace_bytes, whole_policy(d) ? 0 : workspace_of(d))) return rc;
         LossArgs a = {};
         fill(a, d, scores, scores_stride, item, ref_logp, grad_weight, loss, logp, dscores, dscores_stride, workspace);
         a.old_logp = old_logp; a.advantage = advantage; a.kl = kl;
@@ -590,7 +593,7 @@ extern "C" int rec_policy_loss(const rec_loss_desc* d, const void* scores, int64
         DeviceScope scope;
         HIP_TRY(scope.enter(d->device));
         hipStream_t st = (hipStream_t)stream;
-        if (a.splits == 1) {
+        if (whole_policy(d)) {
             // rows of few items take smaller blocks: two 16-byte loads for each thread at least
             const int64_t vectors = d->n_items * rec_type_size(d->type) / 16 / 2;
             const int threads = vectors >= 1024 ? 1024 : vectors < 64 ? 64 : (int)(vectors + 63) / 64 * 64;

@@ -449,9 +449,10 @@ __device__ __forceinline__ void clear_if(float (&h)[4], bool clear)
     } while (0)
 
 // third pass: per 16 rows, the states again from the checkpoint in front of them, then the gradient backwards.  A lane keeps the
-// tile's states in registers (64 of them).  Keeping the decays as well left room for one wavefront per SIMD instead of three.
+// tile's states in registers (64 of them).  Keeping the decays as well left room for one wavefront per SIMD instead of three.  Up to 8
+// states the LDS of 128 or 256 channels allows two blocks or one.
 template <class T, int LN, bool STATES>
-__global__ __launch_bounds__(256, STATES ? 2 : 3) void scan_backward_kernel(ScanArgs a)
+__global__ __launch_bounds__(256, LN == 1 ? 1 : STATES || LN == 2 ? 2 : 3) void scan_backward_kernel(ScanArgs a)
 {
     if ((int)blockIdx.x >= a.main_blocks) {
         pass_empty(a, a.dfinal, a.dinitial);
@@ -875,7 +876,7 @@ int lanes_of(int states) { return states <= 4 ? 1 : states <= 8 ? 2 : states <= 
 // handed over, so chunks are as long as they can be while the launch still fills the chip: `blocks` of them, between 16 and
 // 512 rows.
 struct Cut { int tiles_per_group, tiles, chunk, chunks; };
-constexpr int kForwardBlocks = 2048, kBackwardBlocks = 3072;
+constexpr int kForwardBlocks = 2048, kBackwardBlocks = 3000;
 Cut cut_of(const rec_scan_desc* d, int blocks)
 {
     Cut c;

@@ -34,7 +34,7 @@ def scan(entry="rec_history_scan", in_kw={}, out=AT + 8192, y_stride=8, ws=1 << 
         return call(entry, C.byref(d), C.byref(i), AT, out, y_stride, None, None, AT, ws, None)
     if entry == "rec_history_scan_step":
         return call(entry, C.byref(d), C.byref(i), AT, AT + 16384, out, y_stride, None)
-    o = ops._ScanGradientPointers(du=out, ddelta=out + 1024, dB=out + 2048, dC=out + 3072, dA=out + 4096)
+    o = ops._ScanGradientPointers(du=out, ddelta=out + 1024, dB=out + 2048, dC=out + 3200, dA=out + 4096)
     return call(entry, C.byref(d), AT + 2048, y_stride, C.byref(i), AT, AT, None, C.byref(o), AT + 32768, ws, None)
 
 
@@ -43,9 +43,9 @@ def preference(out=None, weight=None, stride=16, ws=1 << 20, n_pairs=1, beta=0.1
     return call("rec_preference_loss", C.byref(d), AT, stride, AT, AT, n_pairs, None, beta, smoothing, weight, AT, AT, AT, out, out_stride, AT + 16384, ws, None)
 
 
-def policy(out=None, weight=None, clip=(0.2, 0.2), kl=0.0, refs=None, ws=1 << 20, **kw):
+def policy(out=None, weight=None, clip=(0.2, 0.2), kl=0.0, refs=None, ws=1 << 20, stride=16, **kw):
     d = ops._LossDesc(**{**dict(device=0, type=0, rows=4, n_items=16, scale=1.0, zero_rest=0), **kw})
-    return call("rec_policy_loss", C.byref(d), AT, 16, AT, AT, AT, refs, *clip, kl, weight, AT, None, AT, out, 16, AT + 16384, ws, None)
+    return call("rec_policy_loss", C.byref(d), AT, stride, AT, AT, AT, refs, *clip, kl, weight, AT, None, AT, out, 16, AT + 16384, ws, None)
 
 
 REFUSED = [
@@ -68,9 +68,9 @@ REFUSED = [
     (lambda: preference(stride=15), "row stride"), (lambda: preference(beta=float("inf")), "beta"), (lambda: preference(smoothing=1.5), "smoothing"),
     (lambda: preference(smoothing=float("nan")), "smoothing"), (lambda: preference(weight=AT), "come together"), (lambda: preference(out=AT + 8192), "come together"),
     (lambda: preference(out=AT, weight=AT, out_stride=15), "row stride"), (lambda: preference(out=AT + 64, weight=AT), "dscores overlaps"),
-    (lambda: preference(out=AT, weight=AT, out_stride=17), "dscores overlaps"), (lambda: preference(ws=0), "workspace is too small"), (lambda: preference(device=77), "no such HIP device"),
+    (lambda: preference(out=AT, weight=AT, out_stride=17), "dscores overlaps"), (lambda: preference(ws=0, rows=65, n_items=16), "workspace is too small"), (lambda: preference(device=77), "no such HIP device"),
     (lambda: policy(clip=(-0.1, 0.2)), "clip_low"), (lambda: policy(clip=(0.2, float("nan"))), "clip_low"), (lambda: policy(clip=(1.1, 0.2)), "clip_low"),
-    (lambda: policy(kl=0.1), "kl_coef"), (lambda: policy(kl=float("inf"), refs=AT), "kl_coef"), (lambda: policy(out=AT + 8192), "come together"), (lambda: policy(ws=1), "workspace is too small"),
+    (lambda: policy(kl=0.1), "kl_coef"), (lambda: policy(kl=float("inf"), refs=AT), "kl_coef"), (lambda: policy(out=AT + 8192), "come together"), (lambda: policy(ws=1, rows=2, n_items=16384, stride=16384), "workspace is too small"),
     (lambda: policy(type=4), "unknown type"),
 ]
 
