@@ -352,19 +352,19 @@ template <class T, int W, int V>
 __global__ __launch_bounds__(256) void conv_step_kernel(ConvArgs a, const int32_t* __restrict__ slots, T* window)
 {
     const int64_t row = blockIdx.x / a.tiles;
-    const int cv = (int)(blockIdx.x % a.tiles) * (int)blockDim.x + threadIdx.x, d = cv * V;
-    const int slot = slots[row];
+    const int cv = (int)(blockIdx.x % a.tiles) * (int)blockDim.x + threadIdx.x;
+    const bool on = cv < a.nvec;
+    const int d = on ? cv * V : 0, slot = slots[row];
     __shared__ unsigned seen[4];
     look_for_slot(slots, a.rows, row, slot, seen);
     __syncthreads();
     const unsigned shared = slots_seen(seen);
     const bool earlier = shared & 1, later = shared & 2;
-    if (cv >= a.nvec) return;
     float y[V];
     if (slot < 0 || slot >= a.n_seq) {
 #pragma unroll
         for (int v = 0; v < V; v++) y[v] = 0.0f;
-        store_row<T, V>(a.y, row * a.y_stride + d, y);
+        if (on) store_row<T, V>(a.y, row * a.y_stride + d, y);
         return;
     }
     if (earlier) return;
@@ -373,6 +373,7 @@ __global__ __launch_bounds__(256) void conv_step_kernel(ConvArgs a, const int32_
     const int64_t at = (int64_t)slot * (W - 1) * a.channels + d;
     auto click = [&](int64_t r) {   // the window goes through memory, so that rows of a shared slot are steps like any other
         float win[W][V];
+        if (!on) return;
 #pragma unroll
         for (int j = 0; j < W - 1; j++) load_row<T, V>(window, at + (int64_t)j * a.channels, win[j]);
         load_row<T, V>(a.x, r * a.x_stride + d, win[W - 1]);
@@ -389,8 +390,7 @@ __global__ __launch_bounds__(256) void conv_step_kernel(ConvArgs a, const int32_
     };
     click(row);
     if (later)
-        for (int64_t r = row + 1; r < a.rows; r++)
-            if (slots[r] == slot) click(r);
+        for (int r = next_row_of(slots, (int)a.rows, (int)row, slot); r < (int)a.rows; r = next_row_of(slots, (int)a.rows, r, slot)) click(r);
 }
 
 // Rows of a strip: long strips read fewer rows twice (gradient above: 163, 142, 134 us at 32, 64, 128 rows), short ones give a small
@@ -426,6 +426,8 @@ RowsOf rows_of(const rec_conv_desc* d, const void* p, int64_t stride)
     const int size = rec_type_size(d->type);
     return {p, d->rows, stride * size, (int64_t)d->channels * size};
 }
+
+int64_t window_bytes(const rec_conv_desc* d) { return (int64_t)d->n_seq * (d->taps - 1) * d->channels * rec_type_size(d->type); }
 
 struct Layout { int vec, nvec; };
 
@@ -491,6 +493,7 @@ extern "C" int rec_history_conv(const rec_conv_desc* d, const void* x, int64_t x
         if (int rc = check_stride(y_stride, d)) return rc;
         const int wide = kForwardVec;
         REC_REFUSE(rec_overlap(rows_of(d, x, x_stride), rows_of(d, y, y_stride)), "the output overlaps the input");
+        REC_REFUSE(rec_overlap(initial, window_bytes(d), final_window, window_bytes(d)), "final_window overlaps initial");
         if (int rc = rec_check_device(d->device)) return rc;
         const Layout l = layout_of(d, wide, {x, y, initial, final_window}, {x_stride, y_stride});
         const Grid g = grid_of(d, l.nvec, kForwardStrip, INT32_MAX);
@@ -536,6 +539,8 @@ extern "C" int rec_history_conv_backward(const rec_conv_desc* d, const void* dy,
         if (int rc = check_stride(dx_stride, d)) return rc;
         REC_REFUSE(rec_overlap(rows_of(d, x, x_stride), rows_of(d, dx, dx_stride)) || rec_overlap(rows_of(d, dy, dy_stride), rows_of(d, dx, dx_stride)),
                    "the output overlaps the input");
+        REC_REFUSE(rec_overlap(initial, window_bytes(d), dinitial, window_bytes(d)) || rec_overlap(dfinal, window_bytes(d), dinitial, window_bytes(d)),
+                   "dinitial overlaps initial or dfinal");
         const bool sums = dweight || dbias;
         REC_REFUSE(sums && workspace_bytes < rec_history_conv_backward_workspace(d), "the workspace is too small");
         REC_REFUSE(sums && rec_history_conv_backward_workspace(d) > 0 && (!workspace || !rec_aligned(workspace, 16)), "the workspace is null or not aligned to 16 bytes");
@@ -577,7 +582,7 @@ extern "C" int rec_history_conv_step(const rec_conv_desc* d, const void* x, int6
         if (int rc = check_stride(y_stride, d)) return rc;
         const int size = rec_type_size(d->type), wide = 16 / size;
         const RowsOf xr = rows_of(d, x, x_stride), yr = rows_of(d, y, y_stride);
-        const RowsOf pool = {window, 1, INT64_MAX, (int64_t)d->n_seq * (d->taps - 1) * d->channels * size};
+        const RowsOf pool = {window, 1, INT64_MAX, window_bytes(d)};
         REC_REFUSE(rec_overlap(xr, yr) || rec_overlap(pool, yr) || rec_overlap(pool, xr), "x, y and the window must not overlap");
         if (int rc = rec_check_device(d->device)) return rc;
         if (d->rows == 0) return 0;
@@ -587,13 +592,17 @@ extern "C" int rec_history_conv_step(const rec_conv_desc* d, const void* x, int6
         a.n_seq = d->n_seq; a.channels = d->channels; a.nvec = l.nvec; a.silu = d->silu;
         const int threads = l.nvec >= 256 ? 256 : (l.nvec + 63) / 64 * 64;
         a.tiles = (l.nvec + threads - 1) / threads;
-        const int64_t blocks = d->rows * a.tiles;
-        if (int rc = check_blocks(blocks)) return rc;
+        if (int rc = check_blocks((d->rows < kStepRows ? d->rows : kStepRows) * a.tiles)) return rc;
         DeviceScope scope;
         HIP_TRY(scope.enter(d->device));
-#define CALL(T, W, V, ONE) conv_step_kernel<T, W, V><<<(unsigned)blocks, threads, 0, (hipStream_t)stream>>>(a, slots, (T*)window)
-        CONV_DISPATCH(4, 8, l.vec, false, CALL)
+        for (int64_t r = 0; r < d->rows; r += kStepRows) {
+            a.rows = d->rows - r < kStepRows ? d->rows - r : kStepRows;
+            a.x = (const char*)x + r * x_stride * size;
+            a.y = (char*)y + r * y_stride * size;
+#define CALL(T, W, V, ONE) conv_step_kernel<T, W, V><<<(unsigned)(a.rows * a.tiles), threads, 0, (hipStream_t)stream>>>(a, slots + r, (T*)window)
+            CONV_DISPATCH(4, 8, l.vec, false, CALL)
 #undef CALL
+        }
         HIP_TRY(hipGetLastError());
         return 0;
     });

@@ -482,7 +482,15 @@ __global__ __launch_bounds__(256, LN == 1 ? 1 : STATES || LN == 2 ? 2 : 3) void 
     }
     auto step_back = [&](int& q, int64_t& b) {   // to the sequence in front, past empty ones
         const int64_t at = b;
-        do q--; while (q >= 0 && a.off[q] >= at);
+        q--;
+        if (q >= 0 && a.off[q] >= at) {
+            int low = -1, high = q - 1;
+            while (low < high) {
+                const int mid = low + ((high - low + 1) >> 1);
+                if (a.off[mid] < at) low = mid; else high = mid - 1;
+            }
+            q = low;
+        }
         b = q >= 0 ? a.off[q] : -1;
     };
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -824,7 +832,7 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a, const int32_
                 ((T*)a.y)[r * a.y_stride + mine[k]] = from_f32<T>(valid ? y : 0.0f);
             }
             if (!valid || !(shared & 2)) break;
-            do r++; while (r < rows && slots[r] != slot);
+            r = next_row_of(slots, rows, r, slot);
             if (r >= rows) break;
         }
     }
@@ -869,6 +877,8 @@ RowsOf channel_rows(const rec_scan_desc* d, const void* p, int64_t stride)
     const int64_t e = rec_type_size(d->type);
     return {p, d->rows, stride * e, d->channels * e};
 }
+
+int64_t state_bytes(const rec_scan_desc* d) { return (int64_t)d->n_seq * d->channels * d->states * 4; }
 
 int lanes_of(int states) { return states <= 4 ? 1 : states <= 8 ? 2 : states <= 16 ? 4 : states <= 32 ? 8 : 16; }
 
@@ -944,6 +954,7 @@ extern "C" int rec_history_scan(const rec_scan_desc* d, const rec_scan_inputs* i
         REC_REFUSE(!seq_off || (d->rows > 0 && !y), "null argument");
         REC_REFUSE(y_stride < d->channels || y_stride > INT32_MAX, "a row stride is smaller than the channels, or beyond 2^31-1");
         REC_REFUSE(overlaps_inputs(d, in, channel_rows(d, y, y_stride)), "the output overlaps an input");
+        REC_REFUSE(rec_overlap(in->initial, state_bytes(d), final_state, state_bytes(d)), "final_state overlaps initial");
         const Cut c = cut_of(d, kForwardBlocks);
         if (int rc = check_workspace(workspace, workspace_bytes, link_bytes(d, c))) return rc;
         if (int rc = rec_check_device(d->device)) return rc;
@@ -1003,6 +1014,8 @@ extern "C" int rec_history_scan_backward(const rec_scan_desc* d, const void* dy,
             REC_REFUSE(overlaps_inputs(d, in, outs[k]) || rec_overlap(channel_rows(d, dy, dy_stride), outs[k]), "an output overlaps an input");
             for (int j = 0; j < k; j++) REC_REFUSE(rec_overlap(outs[j], outs[k]), "two outputs overlap");
         }
+        REC_REFUSE(rec_overlap(in->initial, state_bytes(d), out->dinitial, state_bytes(d)) || rec_overlap(dfinal, state_bytes(d), out->dinitial, state_bytes(d)),
+                   "dinitial overlaps initial or dfinal");
         if (int rc = check_workspace(workspace, workspace_bytes, rec_history_scan_backward_workspace(d))) return rc;
         if (int rc = rec_check_device(d->device)) return rc;
         const Cut c = cut_of(d, kBackwardBlocks);
@@ -1064,7 +1077,7 @@ extern "C" int rec_history_scan_step(const rec_scan_desc* d, const rec_scan_inpu
         REC_REFUSE(d->rows > 65536, "a step takes at most 65536 rows");
         REC_REFUSE((d->rows > 0 && (!y || !slots)) || (d->n_seq > 0 && !state), "null argument");
         REC_REFUSE(y_stride < d->channels || y_stride > INT32_MAX, "a row stride is smaller than the channels, or beyond 2^31-1");
-        const RowsOf yr = channel_rows(d, y, y_stride), pool = {state, 1, INT64_MAX, (int64_t)d->n_seq * d->channels * d->states * 4};
+        const RowsOf yr = channel_rows(d, y, y_stride), pool = {state, 1, INT64_MAX, state_bytes(d)};
         REC_REFUSE(overlaps_inputs(d, in, yr) || overlaps_inputs(d, in, pool) || rec_overlap(pool, yr), "the inputs, y and the state must not overlap");
         if (int rc = rec_check_device(d->device)) return rc;
         if (d->rows == 0) return 0;
@@ -1078,14 +1091,21 @@ extern "C" int rec_history_scan_step(const rec_scan_desc* d, const rec_scan_inpu
         const bool whole = d->states == 4 * lanes_of(d->states) && rec_aligned(in->B, four) && rec_aligned(in->C, four) && in->B_stride % 4 == 0 && in->C_stride % 4 == 0;
         DeviceScope scope;
         HIP_TRY(scope.enter(d->device));
-        if (whole) {
-#define CALL(T, LN) scan_step_kernel<T, LN, true><<<(unsigned)d->rows, 256, 0, (hipStream_t)stream>>>(a, slots, state)
-            SCAN_DISPATCH(CALL)
+        const int64_t e = rec_type_size(d->type);
+        auto behind = [&](const void* p, int64_t r, int64_t stride) -> const void* { return p ? (const char*)p + r * stride * e : nullptr; };
+        for (int64_t r = 0; r < d->rows; r += kStepRows) {
+            a.rows = d->rows - r < kStepRows ? d->rows - r : kStepRows;
+            a.u = behind(in->u, r, a.u_stride); a.delta = behind(in->delta, r, a.delta_stride); a.z = behind(in->z, r, a.z_stride);
+            a.B = behind(in->B, r, a.B_stride); a.C = behind(in->C, r, a.C_stride); a.y = (char*)y + r * y_stride * e;
+            if (whole) {
+#define CALL(T, LN) scan_step_kernel<T, LN, true><<<(unsigned)a.rows, 256, 0, (hipStream_t)stream>>>(a, slots + r, state)
+                SCAN_DISPATCH(CALL)
 #undef CALL
-        } else {
-#define CALL(T, LN) scan_step_kernel<T, LN, false><<<(unsigned)d->rows, 256, 0, (hipStream_t)stream>>>(a, slots, state)
-            SCAN_DISPATCH(CALL)
+            } else {
+#define CALL(T, LN) scan_step_kernel<T, LN, false><<<(unsigned)a.rows, 256, 0, (hipStream_t)stream>>>(a, slots + r, state)
+                SCAN_DISPATCH(CALL)
 #undef CALL
+            }
         }
         HIP_TRY(hipGetLastError());
         return 0;

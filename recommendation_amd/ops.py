@@ -322,7 +322,7 @@ def preference_loss(scores, items, seq_off, ref_logp=None, *, beta=0.1, label_sm
     w, ds, pd, sd = _gradient(scores, grad_weight, pairs, out, dtype, dev, rows, width)
     d = _LossDesc(dev, kind, rows, width, scale, 1 if out is None else 0)
     i, r = _whole(items, "items", (rows,), torch.int32, dev), _whole(ref_logp, "ref_logp", (rows,), F32, dev)
-    logp = scores.new_empty(rows, dtype=F32)
+    logp = scores.new_empty(rows, dtype=F32) if out is None else scores.new_zeros(rows, dtype=F32)   # rows of no list: 0
     loss, margin = scores.new_empty((2, pairs), dtype=F32).unbind()
     size = _fn("rec_preference_loss_workspace")(C.byref(d), pairs)
     ws, pw = _space(size, scores)

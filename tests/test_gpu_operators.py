@@ -593,6 +593,9 @@ def test_outputs_leave_other_rows_alone():
         else:
             ops.preference_loss(s, item, off, grad_weight=torch.ones(1, device=DEV), out=o)
         outs.append(o)
+    # what is allocated beside the caller's array has zeros there
+    r = ops.preference_loss(s, item, off, grad_weight=torch.ones(1, device=DEV), out=s.clone())
+    assert not r.logp[:3].any() and not r.logp[41:].any() and r.logp[3:41].all()
     o = torch.full(x.shape, 7.0, device=DEV)
     ops.history_conv_backward(x, x, w, seq_off=off, out=o)
     for o in outs + [o]:
@@ -652,6 +655,57 @@ def test_element_offsets_beyond_32_bits():
     a = ops.history_scan_step(x, x, A, B, B, state=pool, slots=torch.tensor([slots - 1], dtype=torch.int32, device=DEV))
     b = ops.history_scan_step(x, x, A, B, B, state=small, slots=torch.tensor([0], dtype=torch.int32, device=DEV))
     assert torch.equal(a, b) and torch.equal(pool[slots - 1], small[0])
+
+
+def test_long_runs_of_empty_histories():
+    """Hundreds of thousands of them between two clicks: what the other histories get is what they get without them."""
+    full = [0, 3, 40, 41, 200]
+    gaps = [0, 1, 200000, 70001, 1]   # empty histories behind each of the boundaries
+    off, at = [], []
+    for o, k in zip(full, gaps):
+        off += [o] * (1 + k)
+        at.append(len(off) - 1)
+    at = at[:-1]                      # the histories that have clicks
+    off, few, n = offsets(off), offsets(full), len(off) - 1
+    x, w = torch.randn(200, 8, device=DEV), torch.randn(8, 4, device=DEV)
+    i, df = torch.randn(n, 3, 8, device=DEV), torch.randn(n, 3, 8, device=DEV)
+    y, fin = ops.history_conv(x, w, seq_off=off, initial=i, want_final=True)
+    y1, fin1 = ops.history_conv(x, w, seq_off=few, initial=i[at], want_final=True)
+    assert torch.equal(y, y1) and torch.equal(fin[at], fin1)
+    empty = torch.ones(n, dtype=torch.bool, device=DEV)
+    empty[at] = False
+    assert torch.equal(fin[empty], i[empty])
+    g = ops.history_conv_backward(x, x, w, seq_off=off, initial=i, dfinal=df)
+    g1 = ops.history_conv_backward(x, x, w, seq_off=few, initial=i[at], dfinal=df[at])
+    assert torch.equal(g.dx, g1.dx) and torch.equal(g.dweight, g1.dweight) and torch.equal(g.dinitial[at], g1.dinitial) and torch.equal(g.dinitial[empty], df[empty])
+    A, B = -torch.rand(8, 4, device=DEV), torch.randn(200, 1, 4, device=DEV)
+    h, dh = torch.randn(n, 8, 4, device=DEV), torch.randn(n, 8, 4, device=DEV)
+    y, fin, kept = ops.history_scan(x, x, A, B, B, seq_off=off, initial=h, want_final=True, want_checkpoints=True)
+    y1, fin1, kept1 = ops.history_scan(x, x, A, B, B, seq_off=few, initial=h[at], want_final=True, want_checkpoints=True)
+    assert torch.equal(y, y1) and torch.equal(fin[at], fin1) and torch.equal(kept, kept1) and torch.equal(fin[empty], h[empty])
+    g = ops.history_scan_backward(x, x, x, A, B, B, seq_off=off, checkpoints=kept, initial=h, dfinal=dh)
+    g1 = ops.history_scan_backward(x, x, x, A, B, B, seq_off=few, checkpoints=kept, initial=h[at], dfinal=dh[at])
+    for name in ("du", "ddelta", "dA", "dB", "dC"):
+        assert torch.equal(getattr(g, name), getattr(g1, name)), name
+    assert torch.equal(g.dinitial[at], g1.dinitial) and torch.equal(g.dinitial[empty], dh[empty])
+
+
+def test_steps_of_many_rows_are_steps_one_after_the_other():
+    rows, slots = 9001, 5000   # more rows than slots: some name the same one, some none
+    slot = torch.randint(-1, slots + 1, (rows,), generator=torch.Generator().manual_seed(3)).to(DEV).int()
+    slot[100:4300] = torch.where(torch.arange(4200, device=DEV) % 3 == 0, 7, slot[100:4300])   # one of them 1400 times
+    x, w = torch.randn(rows, 12, device=DEV).half(), torch.randn(12, 3, device=DEV)
+    pool = torch.randn(slots, 2, 12, device=DEV).half()
+    mine = pool.clone()
+    y = ops.history_conv_step(x, w, state=pool, slots=slot)
+    part = [ops.history_conv_step(x[r:r + 700], w, state=mine, slots=slot[r:r + 700]) for r in range(0, rows, 700)]
+    assert torch.equal(y, torch.cat(part)) and torch.equal(pool, mine)
+    A, B = -torch.rand(12, 5, device=DEV), torch.randn(rows, 2, 5, device=DEV).half()
+    pool = torch.randn(slots, 12, 5, device=DEV)
+    mine = pool.clone()
+    y = ops.history_scan_step(x, x, A, B, B, z=x, state=pool, slots=slot)
+    part = [ops.history_scan_step(*(t[r:r + 700] for t in (x, x)), A, B[r:r + 700], B[r:r + 700], z=x[r:r + 700], state=mine, slots=slot[r:r + 700]) for r in range(0, rows, 700)]
+    assert torch.equal(y, torch.cat(part)) and torch.equal(pool, mine)
 
 
 def test_offsets_that_break_the_rules_touch_nothing_else():

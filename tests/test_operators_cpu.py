@@ -27,14 +27,17 @@ def conv(entry="rec_history_conv", at=AT, out=AT + 8192, stride=8, ws=0, **kw):
     return call(entry, C.byref(d), AT + 4096, stride, at, stride, AT, None, AT, None, None, out, stride, AT + 30000 // 256 * 256, None, None, AT + 40960, ws, None)
 
 
-def scan(entry="rec_history_scan", in_kw={}, out=AT + 8192, y_stride=8, ws=1 << 20, **kw):
+CONV_4X8 = ops._ConvDesc(device=0, type=0, rows=4, n_seq=1, channels=8, taps=4, silu=1, zero_rest=0)
+
+
+def scan(entry="rec_history_scan", in_kw={}, out=AT + 8192, y_stride=8, ws=1 << 20, final=None, **kw):
     d = ops._ScanDesc(**{**dict(device=0, type=0, rows=4, n_seq=1, channels=8, groups=2, states=4, softplus=1, zero_rest=0), **kw})
     i = ops._ScanInputs(**{**dict(u=AT, delta=AT + 256, z=None, B=AT + 512, C=AT + 1024, u_stride=8, delta_stride=8, z_stride=0, B_stride=8, C_stride=8, A=AT), **in_kw})
     if entry == "rec_history_scan":
-        return call(entry, C.byref(d), C.byref(i), AT, out, y_stride, None, None, AT, ws, None)
+        return call(entry, C.byref(d), C.byref(i), AT, out, y_stride, final, None, AT, ws, None)
     if entry == "rec_history_scan_step":
         return call(entry, C.byref(d), C.byref(i), AT, AT + 16384, out, y_stride, None)
-    o = ops._ScanGradientPointers(du=out, ddelta=out + 1024, dB=out + 2048, dC=out + 3200, dA=out + 4096)
+    o = ops._ScanGradientPointers(du=out, ddelta=out + 1024, dB=out + 2048, dC=out + 3200, dA=out + 4096, dinitial=final)
     return call(entry, C.byref(d), AT + 2048, y_stride, C.byref(i), AT, AT, None, C.byref(o), AT + 32768, ws, None)
 
 
@@ -72,6 +75,11 @@ REFUSED = [
     (lambda: policy(clip=(-0.1, 0.2)), "clip_low"), (lambda: policy(clip=(0.2, float("nan"))), "clip_low"), (lambda: policy(clip=(1.1, 0.2)), "clip_low"),
     (lambda: policy(kl=0.1), "kl_coef"), (lambda: policy(kl=float("inf"), refs=AT), "kl_coef"), (lambda: policy(out=AT + 8192), "come together"), (lambda: policy(ws=1, rows=2, n_items=16384, stride=16384), "workspace is too small"),
     (lambda: policy(type=4), "unknown type"),
+    # the state that a call starts from is not the one that it leaves
+    (lambda: call("rec_history_conv", C.byref(CONV_4X8), AT, 8, AT, None, AT, AT + 32768, AT + 8192, 8, AT + 32768 + 64, None), "final_window overlaps"),
+    (lambda: call("rec_history_conv_backward", C.byref(CONV_4X8), AT + 4096, 8, AT, 8, AT, None, AT, None, AT + 32768, AT + 8192, 8, AT, None, AT + 32768, AT + 40960, 1 << 20, None), "dinitial overlaps"),
+    (lambda: scan(in_kw={"initial": AT + 32768}, final=AT + 32768 + 64), "final_state overlaps"),
+    (lambda: scan("rec_history_scan_backward", in_kw={"initial": AT + 32768}, final=AT + 32768), "dinitial overlaps"),
 ]
 
 
