@@ -34,7 +34,8 @@ struct LossArgs {
 // sample of it ls = sum of 2^(c (x - m)) and qs = sum of (x - m) 2^(c (x - m)).  The rounding of c is the same for every score: it would
 // move log l of all rows the same way (by 6e-8 for scores of deviation 2), and the log-ratio of lists of different lengths by
 // that times their difference.  qs / ls, the derivative of log l by c, takes it out again; one score of each 16 bytes is
-// sample enough for a factor of a rounding.  m is -inf for a set with nothing in it.
+// sample enough for a factor of a rounding.  (Where a few scores that are not in the sample hold nearly all of l, the mean is near
+// 0 and the sample's own is not: it counts for no more than its share of l.)  m is -inf for a set with nothing in it.
 struct Stat { float m, l, ls, qs; };
 
 __device__ __forceinline__ Stat join(Stat a, Stat b, float c)
@@ -180,7 +181,8 @@ __device__ __forceinline__ bool row_log_probability(const LossArgs& a, int64_t r
 {
     logp = 0.0;
     if (st.m == -INFINITY && st.l == 0.0f) return false;
-    const double l = log((double)st.l), mean = st.ls > 0.0f ? (double)st.qs / (double)st.ls : 0.0;
+    const double of = fmax((double)st.ls, (double)st.l * (sizeof(T) / 16.0));   // a sample with less than its share speaks for its share
+    const double l = log((double)st.l), mean = of > 0.0 ? (double)st.qs / of : 0.0;
     logp = (double)a.scale * ((double)to_f32(((const T*)a.scores)[row * a.scores_stride + a.item[row]]) - (double)st.m) - l - a.scale_rest * mean;
     return true;
 }

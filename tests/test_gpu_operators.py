@@ -460,6 +460,23 @@ def test_rows_whose_mask_leaves_nothing_and_masked_choices():
     assert v.margin[0] == inf and v.loss[0] == 0 and not v.dscores.any()
 
 
+@pytest.mark.parametrize("tn", ["f32", "f16", "bf16"])
+def test_rows_that_one_score_decides(tn):
+    """The choice stands 32 above 4096 others, at every place within 16 bytes.  The others' part of the sum is below 4096 e^(4.5 - 32),
+    5e-9, so log p is between -5e-9 and 0; a sum that starts at 1 loses or gains no more than that part, and what is left
+    of the correction for log2(e)'s rounding is 2^-24 of (32 + 4.5) times it."""
+    rows, items = 16, 4096
+    s = torch.randn(rows, items, generator=torch.Generator().manual_seed(5)).clamp(-4.5, 4.5)
+    item = torch.arange(rows) + 1000
+    s[torch.arange(rows), item] = 32.0
+    s = s.to(TYPES[tn]).to(DEV)
+    zero = torch.zeros(rows, device=DEV)
+    r = ops.policy_loss(s, item.int().to(DEV), zero, zero + 1)
+    assert float(r.logp.abs().max()) <= 1.1e-8 and float((r.loss + 1).abs().max()) <= 2 ** -24
+    p = ops.preference_loss(s, item.int().to(DEV), offsets([0, 12, 16]))
+    assert float(p.logp.abs().max()) <= 1.1e-8 and float(p.margin.abs().max()) <= 0.1 * 16 * 1.1e-8
+
+
 def test_values_that_are_not_finite_stay_in_their_rows():
     s = torch.randn(6, 3000, device=DEV)
     s[1, 7], s[3, 2999], s[4, 0] = float("nan"), float("inf"), torch.finfo(torch.float32).min
