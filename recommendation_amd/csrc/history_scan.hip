@@ -449,10 +449,10 @@ __device__ __forceinline__ void clear_if(float (&h)[4], bool clear)
     } while (0)
 
 // third pass: per 16 rows, the states again from the checkpoint in front of them, then the gradient backwards.  A lane keeps the
-// tile's states in registers (64 of them).  Keeping the decays as well left room for one wavefront per SIMD instead of three.  Up to 8
-// states the LDS of 128 or 256 channels allows two blocks or one.
+// tile's states in registers (64 of them).  Keeping the decays as well left room for one wavefront per SIMD instead of three.  (Two
+// with 128 channels: their LDS leaves room for two blocks.)
 template <class T, int LN, bool STATES>
-__global__ __launch_bounds__(256, LN == 1 ? 1 : STATES || LN == 2 ? 2 : 3) void scan_backward_kernel(ScanArgs a)
+__global__ __launch_bounds__(256, STATES || LN == 2 ? 2 : 3) void scan_backward_kernel(ScanArgs a)
 {
     if ((int)blockIdx.x >= a.main_blocks) {
         pass_empty(a, a.dfinal, a.dinitial);
@@ -880,17 +880,27 @@ RowsOf channel_rows(const rec_scan_desc* d, const void* p, int64_t stride)
 
 int64_t state_bytes(const rec_scan_desc* d) { return (int64_t)d->n_seq * d->channels * d->states * 4; }
 
-int lanes_of(int states) { return states <= 4 ? 1 : states <= 8 ? 2 : states <= 16 ? 4 : states <= 32 ? 8 : 16; }
+int lanes_of(const rec_scan_desc* d) { return d->states <= 4 ? 1 : d->states <= 8 ? 2 : d->states <= 16 ? 4 : d->states <= 32 ? 8 : 16; }
+// The passes over histories take two lanes at least, and more, idle ones too, where the group's channels fill half a block or less: a
+// block with fewer channels stages and keeps less.  (The gradient's last pass, bf16, 4 states: 50 000 rows of 256 channels 230 us with
+// one lane, whose LDS leaves room for one block on a compute unit, 187 with two, 240 with four; 100 000 rows of 100 channels 404 and
+// 186 us with one and two; f32, 16 575 rows of 31 channels 86 and 32 us with one and eight.)
+int pass_lanes(const rec_scan_desc* d)
+{
+    int lanes = d->states <= 4 ? 2 : lanes_of(d);
+    while (lanes < 16 && 256 / (2 * lanes) >= d->channels / d->groups) lanes *= 2;
+    return lanes;
+}
 
 // How the rows are cut.  A chunk more costs its first pass (two thirds of the third, over the chunk's last history) and a state
 // handed over, so chunks are as long as they can be while the launch still fills the chip: `blocks` of them, between 16 and
 // 512 rows.
 struct Cut { int tiles_per_group, tiles, chunk, chunks; };
 constexpr int kForwardBlocks = 2048, kBackwardBlocks = 3000;
-Cut cut_of(const rec_scan_desc* d, int blocks)
+Cut cut_of(const rec_scan_desc* d, int blocks, int lanes)
 {
     Cut c;
-    const int ch = 256 / lanes_of(d->states), per = d->channels / d->groups;
+    const int ch = 256 / lanes, per = d->channels / d->groups;
     c.tiles_per_group = (per + ch - 1) / ch;
     c.tiles = c.tiles_per_group * d->groups;
     int64_t rows = d->rows * c.tiles / blocks / TT * TT;
@@ -927,22 +937,26 @@ int check_workspace(const void* p, int64_t has, int64_t needs)
     return 0;
 }
 
-#define SCAN_LANES(T, CALL)                                                                                 \
-    switch (lanes_of(d->states)) {                                                                          \
+#define SCAN_TYPES(LANES, CALL)                                                                             \
+    if (d->type == REC_TYPE_F32) { LANES(float, CALL) }                                                     \
+    else if (d->type == REC_TYPE_F16) { LANES(_Float16, CALL) }                                             \
+    else { LANES(__bf16, CALL) }
+#define SCAN_PASS_LANES(T, CALL)                                                                            \
+    switch (pass_lanes(d)) {                                                                                \
+    case 2: CALL(T, 2); break; case 4: CALL(T, 4); break; case 8: CALL(T, 8); break; default: CALL(T, 16); break; \
+    }
+#define SCAN_STEP_LANES(T, CALL)                                                                            \
+    switch (lanes_of(d)) {                                                                                  \
     case 1: CALL(T, 1); break; case 2: CALL(T, 2); break; case 4: CALL(T, 4); break;                        \
     case 8: CALL(T, 8); break; default: CALL(T, 16); break;                                                 \
     }
-#define SCAN_DISPATCH(CALL)                                                                                 \
-    if (d->type == REC_TYPE_F32) { SCAN_LANES(float, CALL) }                                                \
-    else if (d->type == REC_TYPE_F16) { SCAN_LANES(_Float16, CALL) }                                        \
-    else { SCAN_LANES(__bf16, CALL) }
 
 }  // namespace
 
 extern "C" int64_t rec_history_scan_workspace(const rec_scan_desc* d)
 {
     if (check_desc(d)) return -1;
-    return link_bytes(d, cut_of(d, kForwardBlocks));
+    return link_bytes(d, cut_of(d, kForwardBlocks, pass_lanes(d)));
 }
 
 extern "C" int rec_history_scan(const rec_scan_desc* d, const rec_scan_inputs* in, const int64_t* seq_off, void* y, int64_t y_stride,
@@ -955,7 +969,7 @@ extern "C" int rec_history_scan(const rec_scan_desc* d, const rec_scan_inputs* i
         REC_REFUSE(y_stride < d->channels || y_stride > INT32_MAX, "a row stride is smaller than the channels, or beyond 2^31-1");
         REC_REFUSE(overlaps_inputs(d, in, channel_rows(d, y, y_stride)), "the output overlaps an input");
         REC_REFUSE(rec_overlap(in->initial, state_bytes(d), final_state, state_bytes(d)), "final_state overlaps initial");
-        const Cut c = cut_of(d, kForwardBlocks);
+        const Cut c = cut_of(d, kForwardBlocks, pass_lanes(d));
         if (int rc = check_workspace(workspace, workspace_bytes, link_bytes(d, c))) return rc;
         if (int rc = rec_check_device(d->device)) return rc;
         const int64_t blocks = (int64_t)c.chunks * c.tiles, n = (int64_t)d->channels * d->states;
@@ -973,13 +987,13 @@ extern "C" int rec_history_scan(const rec_scan_desc* d, const rec_scan_inputs* i
         hipStream_t st = (hipStream_t)stream;
         if (c.chunks > 1) {
 #define CALL(T, LN) scan_local_kernel<T, LN><<<(unsigned)blocks, 256, 0, st>>>(a)
-            SCAN_DISPATCH(CALL)
+            SCAN_TYPES(SCAN_PASS_LANES, CALL)
 #undef CALL
             scan_link_kernel<false><<<(unsigned)((n + LINK_COLS - 1) / LINK_COLS), LINK_COLS * LINK_RUNS, 0, st>>>(a);
         }
         if (blocks + empty_blocks > 0) {
 #define CALL(T, LN) scan_forward_kernel<T, LN><<<(unsigned)(blocks + empty_blocks), 256, 0, st>>>(a)
-            SCAN_DISPATCH(CALL)
+            SCAN_TYPES(SCAN_PASS_LANES, CALL)
 #undef CALL
         }
         HIP_TRY(hipGetLastError());
@@ -994,7 +1008,7 @@ static int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 extern "C" int64_t rec_history_scan_backward_workspace(const rec_scan_desc* d)
 {
     if (check_desc(d)) return -1;
-    const Cut c = cut_of(d, kBackwardBlocks);
+    const Cut c = cut_of(d, kBackwardBlocks, pass_lanes(d));
     return round16(link_bytes(d, c)) + round16(backward_part_a(d, c)) + backward_part_bc(d, c);
 }
 
@@ -1018,7 +1032,7 @@ extern "C" int rec_history_scan_backward(const rec_scan_desc* d, const void* dy,
                    "dinitial overlaps initial or dfinal");
         if (int rc = check_workspace(workspace, workspace_bytes, rec_history_scan_backward_workspace(d))) return rc;
         if (int rc = rec_check_device(d->device)) return rc;
-        const Cut c = cut_of(d, kBackwardBlocks);
+        const Cut c = cut_of(d, kBackwardBlocks, pass_lanes(d));
         const int64_t blocks = (int64_t)c.chunks * c.tiles, n = (int64_t)d->channels * d->states;
         const int64_t empty_blocks = out->dinitial ? (n * d->n_seq + 255) / 256 : 0;
         const int64_t sum_blocks = c.tiles_per_group > 1 ? (d->rows + SUM_ROWS - 1) / SUM_ROWS : 0;
@@ -1041,7 +1055,7 @@ extern "C" int rec_history_scan_backward(const rec_scan_desc* d, const void* dy,
         hipStream_t st = (hipStream_t)stream;
         if (c.chunks > 1) {
 #define CALL(T, LN) scan_local_backward_kernel<T, LN><<<(unsigned)blocks, 256, 0, st>>>(a)
-            SCAN_DISPATCH(CALL)
+            SCAN_TYPES(SCAN_PASS_LANES, CALL)
 #undef CALL
             scan_link_kernel<true><<<(unsigned)((n + LINK_COLS - 1) / LINK_COLS), LINK_COLS * LINK_RUNS, 0, st>>>(a);
         }
@@ -1049,11 +1063,11 @@ extern "C" int rec_history_scan_backward(const rec_scan_desc* d, const void* dy,
             // without states handed in or out, a history's beginning is a zero
             if (in->initial || dfinal || out->dinitial) {
 #define CALL(T, LN) scan_backward_kernel<T, LN, true><<<(unsigned)(blocks + empty_blocks), 256, 0, st>>>(a)
-                SCAN_DISPATCH(CALL)
+                SCAN_TYPES(SCAN_PASS_LANES, CALL)
 #undef CALL
             } else {
 #define CALL(T, LN) scan_backward_kernel<T, LN, false><<<(unsigned)(blocks + empty_blocks), 256, 0, st>>>(a)
-                SCAN_DISPATCH(CALL)
+                SCAN_TYPES(SCAN_PASS_LANES, CALL)
 #undef CALL
             }
         }
@@ -1081,14 +1095,14 @@ extern "C" int rec_history_scan_step(const rec_scan_desc* d, const rec_scan_inpu
         REC_REFUSE(overlaps_inputs(d, in, yr) || overlaps_inputs(d, in, pool) || rec_overlap(pool, yr), "the inputs, y and the state must not overlap");
         if (int rc = rec_check_device(d->device)) return rc;
         if (d->rows == 0) return 0;
-        Cut c = cut_of(d, kForwardBlocks);
+        Cut c = cut_of(d, kForwardBlocks, lanes_of(d));
         c.chunk = 0; c.chunks = 0;
         ScanArgs a = {};
         fill(a, d, in, c);
         a.y = y; a.y_stride = y_stride;
         // four states of B and C in one load: no group's last four reach into the next, and all begin on a multiple of four
         const size_t four = 4 * (size_t)rec_type_size(d->type);
-        const bool whole = d->states == 4 * lanes_of(d->states) && rec_aligned(in->B, four) && rec_aligned(in->C, four) && in->B_stride % 4 == 0 && in->C_stride % 4 == 0;
+        const bool whole = d->states == 4 * lanes_of(d) && rec_aligned(in->B, four) && rec_aligned(in->C, four) && in->B_stride % 4 == 0 && in->C_stride % 4 == 0;
         DeviceScope scope;
         HIP_TRY(scope.enter(d->device));
         const int64_t e = rec_type_size(d->type);
@@ -1099,11 +1113,11 @@ extern "C" int rec_history_scan_step(const rec_scan_desc* d, const rec_scan_inpu
             a.B = behind(in->B, r, a.B_stride); a.C = behind(in->C, r, a.C_stride); a.y = (char*)y + r * y_stride * e;
             if (whole) {
 #define CALL(T, LN) scan_step_kernel<T, LN, true><<<(unsigned)a.rows, 256, 0, (hipStream_t)stream>>>(a, slots + r, state)
-                SCAN_DISPATCH(CALL)
+                SCAN_TYPES(SCAN_STEP_LANES, CALL)
 #undef CALL
             } else {
 #define CALL(T, LN) scan_step_kernel<T, LN, false><<<(unsigned)a.rows, 256, 0, (hipStream_t)stream>>>(a, slots + r, state)
-                SCAN_DISPATCH(CALL)
+                SCAN_TYPES(SCAN_STEP_LANES, CALL)
 #undef CALL
             }
         }

@@ -155,13 +155,12 @@ __device__ __forceinline__ float fold16(float a, float b)
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-// sum over the lanes of a row of 16 that are equal modulo LN, in every one of them
+// sum over the lanes of a row of 16 that are equal modulo LN (2 .. 16), in every one of them
 template <int LN> __device__ __forceinline__ float row_sum_strided(float v)
 {
     if constexpr (LN <= 8) v += dpp_move<0x128>(v);   // row_ror:8
     if constexpr (LN <= 4) v += dpp_move<0x124>(v);
     if constexpr (LN <= 2) v += dpp_move<0x122>(v);
-    if constexpr (LN <= 1) v += dpp_move<0x121>(v);
     return v;
 }
 
