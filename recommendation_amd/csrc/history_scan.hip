@@ -10,6 +10,10 @@
 // crosses from one chunk into the next hands its state over: the first pass computes what each chunk adds on its own
 // (only from the last history's beginning on, and only if it goes on), the second links the chunks of each history, the third
 // walks again from the linked states and writes y.  With one chunk the first two are not launched.
+//
+// Bound by vector instructions: per row and state one exp and three multiply-adds forwards, one exp and some ten backwards, and
+// the sums over states and channels.  100 000 rows of 128 bf16 channels with 16 states (1000 histories): 45 + 16 + 80 us for
+// the three passes, 48 + 21 + 243 and 12 + 9 for sums backwards, where the arrays alone would take 45 us in all at the rate of a copy.
 #include "operators.h"
 #include <type_traits>
 
@@ -146,7 +150,8 @@ template <class T, int LN, bool U, bool Z, bool DY, bool GB, bool GC> struct Til
     }
 };
 
-// first pass: the state a chunk's last history has at the chunk's end, for a state of zero in front of the chunk
+// first pass: the state a chunk's last history has at the chunk's end, for a state of zero in front of the chunk.  (One history of
+// 20 000 rows x 256 f16 channels: 22 us, the link 14, the third pass 32.)
 template <class T, int LN>
 __global__ __launch_bounds__(256) void scan_local_kernel(ScanArgs a)
 {
@@ -197,7 +202,7 @@ __global__ __launch_bounds__(256) void scan_local_kernel(ScanArgs a)
 
 // second pass: the state handed into chunk c + 1 is exp(A span) of what was handed into c (where c's history came from there), plus
 // what c adds.  Such steps compose, so 64 threads share the chunks of a channel's state: each composes a run of them, then
-// walks it again from what the runs in front of it lead to.  (One thread after the other's loads took 0.3 us per chunk.)
+// walks it again from what the runs in front of it lead to.
 // The gradient takes the same steps from the back.
 constexpr int LINK_COLS = 16, LINK_RUNS = 64;
 template <bool BACK>
@@ -273,7 +278,6 @@ template <int LN, int GR> __device__ __forceinline__ void write_sums(float (*to)
     if (GR == LN || j < GR) to[r + j][ch] = mine;
 }
 
-// third pass
 // Empty histories: their state passes through (forwards initial -> final_state, backwards dfinal -> dinitial).  Blocks behind
 // the walk's take them, a value per thread.
 __device__ __forceinline__ void pass_empty(const ScanArgs& a, const float* from, float* to)
@@ -284,6 +288,7 @@ __device__ __forceinline__ void pass_empty(const ScanArgs& a, const float* from,
     if (a.off[s + 1] <= a.off[s]) to[i] = from ? from[i] : 0.0f;
 }
 
+// third pass: y, the states that histories end with, and the checkpoints
 template <class T, int LN>
 __global__ __launch_bounds__(256) void scan_forward_kernel(ScanArgs a)
 {
@@ -448,7 +453,7 @@ __device__ __forceinline__ void clear_if(float (&h)[4], bool clear)
         __builtin_amdgcn_sched_barrier(0);        \
     } while (0)
 
-// third pass: per 16 rows, the states again from the checkpoint in front of them, then the gradient backwards.  A lane keeps the
+// third pass of the gradient: per 16 rows, the states again from the checkpoint in front of them, then the gradient backwards.  A lane keeps the
 // tile's states in registers (64 of them).  Keeping the decays as well left room for one wavefront per SIMD instead of three.  (Two
 // with 128 channels: their LDS leaves room for two blocks.)
 template <class T, int LN, bool STATES>
@@ -714,7 +719,7 @@ __global__ __launch_bounds__(256) void scan_sum_groups_kernel(ScanArgs a)
 }
 
 // ---- single clicks: a block per row; bound by the state, which is read and written once (4 bytes a value each way), and by
-// the waits in between.  Four pieces of 256 / LN channels at a time: a thread prepares whole channels (delta, delta * u, the gate), then
+// the waits in between (1000 rows of 256 channels with 16 states: 10 us, 3.4 TB/s).  Four pieces of 256 / LN channels at a time: a thread prepares whole channels (delta, delta * u, the gate), then
 // takes four states of one channel of each piece, and everything a row needs is asked for at once, before the block looks for
 // other rows of its slot.
 // The code is kept short (one copy of everything; WHOLE: all 4 LN states of a lane group exist and lie on boundaries of four): a
