@@ -12,6 +12,7 @@ tensors' GPU, waits for nothing and can be captured into a graph.  Outputs are a
 to no history are 0 in an allocated output and left as they were in `out`.  Gradients are explicit calls, as the engine's own
 updates are: nothing is recorded for autograd.  Offsets, items and slots are read on the GPU and not checked on the host."""
 import ctypes as C
+import struct
 from collections import namedtuple
 
 import torch
@@ -27,30 +28,12 @@ PreferenceLoss = namedtuple("PreferenceLoss", "loss margin logp dscores")
 PolicyLoss = namedtuple("PolicyLoss", "loss kl logp dscores")
 
 
-class _ConvDesc(C.Structure):
-    _fields_ = [("device", C.c_int32), ("type", C.c_int32), ("rows", C.c_int64), ("n_seq", C.c_int32), ("channels", C.c_int32),
-                ("taps", C.c_int32), ("silu", C.c_int32), ("zero_rest", C.c_int32)]
-
-
-class _ScanDesc(C.Structure):
-    _fields_ = [("device", C.c_int32), ("type", C.c_int32), ("rows", C.c_int64), ("n_seq", C.c_int32), ("channels", C.c_int32),
-                ("groups", C.c_int32), ("states", C.c_int32), ("softplus", C.c_int32), ("zero_rest", C.c_int32)]
-
-
-class _ScanInputs(C.Structure):
-    _fields_ = [(n, C.c_void_p) for n in ("u", "delta", "z", "B", "C")] + \
-               [(n + "_stride", C.c_int64) for n in ("u", "delta", "z", "B", "C")] + \
-               [(n, C.c_void_p) for n in ("A", "D", "delta_bias", "initial")]
-
-
-class _ScanGradientPointers(C.Structure):
-    _fields_ = [(n, C.c_void_p) for n in ("du", "ddelta", "dz", "dB", "dC", "dA", "dD", "ddelta_bias", "dinitial")]
-
-
-class _LossDesc(C.Structure):
-    _fields_ = [("device", C.c_int32), ("type", C.c_int32), ("rows", C.c_int64), ("n_items", C.c_int64), ("scale", C.c_float),
-                ("zero_rest", C.c_int32)]
-
+# The structs of the header, packed from their fields (0q: up to the next multiple of 8 bytes).
+_conv_desc = struct.Struct("@iiqiiiii0q").pack          # rec_conv_desc
+_scan_desc = struct.Struct("@iiqiiiiii0q").pack         # rec_scan_desc
+_scan_inputs = struct.Struct("@5P5q4P").pack            # rec_scan_inputs
+_scan_gradients = struct.Struct("@9P").pack             # rec_scan_gradients
+_loss_desc = struct.Struct("@iiqqfi").pack              # rec_loss_desc
 
 _P, _L, _I, _F = C.c_void_p, C.c_int64, C.c_int32, C.c_float
 _SIGNATURES = {
@@ -181,7 +164,7 @@ def _conv(x, weight, bias, n_seq, silu, zero_rest):
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
         _bad("weight must have the shape [channels, taps]")
     taps = weight.shape[1]
-    d = _ConvDesc(dev, kind, rows, n_seq, ch, taps, 1 if silu else 0, zero_rest)
+    d = _conv_desc(dev, kind, rows, n_seq, ch, taps, 1 if silu else 0, zero_rest)
     return d, px, sx, dtype, dev, rows, ch, taps, _whole(weight, "weight", (ch, taps), F32, dev), _whole(bias, "bias", (ch,), F32, dev)
 
 
@@ -191,10 +174,10 @@ def history_conv(x, weight, bias=None, *, seq_off, initial=None, silu=True, want
     d, px, sx, dtype, dev, rows, ch, taps, w, b = _conv(x, weight, bias, n, silu, 1 if out is None else 0)
     window = (n, max(0, taps - 1), ch)
     i = _whole(initial, "initial", window, dtype, dev)
-    y = x.new_empty((rows, ch)) if out is None else out
+    y = torch.empty_like(x) if out is None else out
     py, sy = _rows(y, "out", dtype, dev, rows, ch)
     final = x.new_empty(window) if want_final else None
-    capi._check(_fn("rec_history_conv")(C.byref(d), px, sx, w, b, off, i, py, sy, _ptr(final), _raw_stream(dev)))
+    capi._check(_fn("rec_history_conv")(d, px, sx, w, b, off, i, py, sy, _ptr(final), _raw_stream(dev)))
     return y, final
 
 
@@ -205,14 +188,14 @@ def history_conv_backward(dy, x, weight, bias=None, *, seq_off, initial=None, si
     pg, sg = _rows(dy, "dy", dtype, dev, rows, ch)
     window = (n, max(0, taps - 1), ch)
     i, df = _whole(initial, "initial", window, dtype, dev), _whole(dfinal, "dfinal", window, dtype, dev)
-    dx = x.new_empty((rows, ch)) if out is None else out
+    dx = torch.empty_like(x) if out is None else out
     pd, sd = _rows(dx, "out", dtype, dev, rows, ch)
     dweight = torch.empty_like(weight)
     dbias = torch.empty_like(bias) if bias is not None else None
     dinitial = torch.empty_like(initial) if initial is not None else None
-    size = _fn("rec_history_conv_backward_workspace")(C.byref(d))
+    size = _fn("rec_history_conv_backward_workspace")(d)
     ws, pw = _space(size, x)
-    capi._check(_fn("rec_history_conv_backward")(C.byref(d), pg, sg, px, sx, w, b, off, i, df, pd, sd, dweight.data_ptr(), _ptr(dbias), _ptr(dinitial), pw, size,
+    capi._check(_fn("rec_history_conv_backward")(d, pg, sg, px, sx, w, b, off, i, df, pd, sd, dweight.data_ptr(), _ptr(dbias), _ptr(dinitial), pw, size,
                                                  _raw_stream(dev)))
     return ConvGradients(dx, dweight, dbias, dinitial)
 
@@ -223,9 +206,9 @@ def history_conv_step(x, weight, bias=None, *, state, slots, silu=True, out=None
     n = len(state)
     d, px, sx, dtype, dev, rows, ch, taps, w, b = _conv(x, weight, bias, n, silu, 0)
     ps = _whole(state, "state", (n, taps - 1, ch), dtype, dev)
-    y = x.new_empty((rows, ch)) if out is None else out
+    y = torch.empty_like(x) if out is None else out
     py, sy = _rows(y, "out", dtype, dev, rows, ch)
-    capi._check(_fn("rec_history_conv_step")(C.byref(d), px, sx, w, b, _whole(slots, "slots", (rows,), torch.int32, dev), ps, py, sy, _raw_stream(dev)))
+    capi._check(_fn("rec_history_conv_step")(d, px, sx, w, b, _whole(slots, "slots", (rows,), torch.int32, dev), ps, py, sy, _raw_stream(dev)))
     return y
 
 
@@ -233,7 +216,7 @@ def _scan(u, delta, A, B, Cm, D, z, delta_bias, n_seq, initial, softplus, zero_r
     kind, dtype, dev, rows, ch = _first(u, "u")
     pu, su = _rows(u, "u", dtype, dev, rows, ch)
     pd, sd = _rows(delta, "delta", dtype, dev, rows, ch)
-    pz, sz = _rows(z, "z", dtype, dev, rows, ch) if z is not None else (None, 0)
+    pz, sz = _rows(z, "z", dtype, dev, rows, ch) if z is not None else (0, 0)
     if not isinstance(A, torch.Tensor) or A.dim() != 2:
         _bad("A must have the shape [channels, states]")
     states = A.shape[1]
@@ -242,9 +225,9 @@ def _scan(u, delta, A, B, Cm, D, z, delta_bias, n_seq, initial, softplus, zero_r
     groups = B.shape[1]
     pB, sB = _groups(B, "B", dtype, dev, rows, groups, states)
     pC, sC = _groups(Cm, "C", dtype, dev, rows, groups, states)
-    d = _ScanDesc(dev, kind, rows, n_seq, ch, groups, states, 1 if softplus else 0, zero_rest)
-    i = _ScanInputs(pu, pd, pz, pB, pC, su, sd, sz, sB, sC, _whole(A, "A", (ch, states), F32, dev), _whole(D, "D", (ch,), F32, dev),
-                    _whole(delta_bias, "delta_bias", (ch,), F32, dev), _whole(initial, "initial", (n_seq, ch, states), F32, dev))
+    d = _scan_desc(dev, kind, rows, n_seq, ch, groups, states, 1 if softplus else 0, zero_rest)
+    i = _scan_inputs(pu, pd, pz, pB, pC, su, sd, sz, sB, sC, _whole(A, "A", (ch, states), F32, dev), _whole(D, "D", (ch,), F32, dev) or 0,
+                     _whole(delta_bias, "delta_bias", (ch,), F32, dev) or 0, _whole(initial, "initial", (n_seq, ch, states), F32, dev) or 0)
     return d, i, dtype, dev, rows, ch, states
 
 
@@ -253,13 +236,13 @@ def history_scan(u, delta, A, B, C_, D=None, z=None, delta_bias=None, *, seq_off
     D, delta_bias [channels], initial and final [histories, channels, states] float32.  The gradient takes the checkpoints."""
     off, n = _offsets(seq_off, u.get_device())
     d, i, dtype, dev, rows, ch, states = _scan(u, delta, A, B, C_, D, z, delta_bias, n, initial, softplus, 1 if out is None else 0)
-    y = u.new_empty((rows, ch)) if out is None else out
+    y = torch.empty_like(u) if out is None else out
     py, sy = _rows(y, "out", dtype, dev, rows, ch)
     final = u.new_empty((n, ch, states), dtype=F32) if want_final else None
     kept = u.new_empty((-(-rows // SCAN_CHECKPOINT), ch, states), dtype=F32) if want_checkpoints else None
-    size = _fn("rec_history_scan_workspace")(C.byref(d))
+    size = _fn("rec_history_scan_workspace")(d)
     ws, pw = _space(size, u)
-    capi._check(_fn("rec_history_scan")(C.byref(d), C.byref(i), off, py, sy, _ptr(final), _ptr(kept), pw, size, _raw_stream(dev)))
+    capi._check(_fn("rec_history_scan")(d, i, off, py, sy, _ptr(final), _ptr(kept), pw, size, _raw_stream(dev)))
     return y, final, kept
 
 
@@ -280,10 +263,10 @@ def history_scan_backward(dy, u, delta, A, B, C_, D=None, z=None, delta_bias=Non
     dD = torch.empty_like(D) if D is not None else None
     dbias = torch.empty_like(delta_bias) if delta_bias is not None else None
     dinitial = torch.empty_like(initial) if initial is not None else None
-    o = _ScanGradientPointers(du.data_ptr(), ddelta.data_ptr(), _ptr(dz), dB.data_ptr(), dC.data_ptr(), dA.data_ptr(), _ptr(dD), _ptr(dbias), _ptr(dinitial))
-    size = _fn("rec_history_scan_backward_workspace")(C.byref(d))
+    o = _scan_gradients(du.data_ptr(), ddelta.data_ptr(), _ptr(dz) or 0, dB.data_ptr(), dC.data_ptr(), dA.data_ptr(), _ptr(dD) or 0, _ptr(dbias) or 0, _ptr(dinitial) or 0)
+    size = _fn("rec_history_scan_backward_workspace")(d)
     ws, pw = _space(size, u)
-    capi._check(_fn("rec_history_scan_backward")(C.byref(d), pg, sg, C.byref(i), off, kept, df, C.byref(o), pw, size, _raw_stream(dev)))
+    capi._check(_fn("rec_history_scan_backward")(d, pg, sg, i, off, kept, df, o, pw, size, _raw_stream(dev)))
     return ScanGradients(du, ddelta, dA, dB, dC, dD, dz, dbias, dinitial)
 
 
@@ -292,9 +275,9 @@ def history_scan_step(u, delta, A, B, C_, D=None, z=None, delta_bias=None, *, st
     n = len(state)
     d, i, dtype, dev, rows, ch, states = _scan(u, delta, A, B, C_, D, z, delta_bias, n, None, softplus, 0)
     ps = _whole(state, "state", (n, ch, states), F32, dev)
-    y = u.new_empty((rows, ch)) if out is None else out
+    y = torch.empty_like(u) if out is None else out
     py, sy = _rows(y, "out", dtype, dev, rows, ch)
-    capi._check(_fn("rec_history_scan_step")(C.byref(d), C.byref(i), _whole(slots, "slots", (rows,), torch.int32, dev), ps, py, sy, _raw_stream(dev)))
+    capi._check(_fn("rec_history_scan_step")(d, i, _whole(slots, "slots", (rows,), torch.int32, dev), ps, py, sy, _raw_stream(dev)))
     return y
 
 
@@ -305,7 +288,7 @@ def _gradient(scores, grad_weight, n, out, dtype, dev, rows, width):
             _bad("out is the gradient's: it needs grad_weight")
         return None, None, None, 0
     w = _whole(grad_weight, "grad_weight", (n,), F32, dev)
-    ds = scores.new_empty((rows, width)) if out is None else out
+    ds = torch.empty_like(scores) if out is None else out
     return (w, ds, *_rows(ds, "out", dtype, dev, rows, width))
 
 
@@ -320,13 +303,13 @@ def preference_loss(scores, items, seq_off, ref_logp=None, *, beta=0.1, label_sm
     pairs = n // 2
     p, s = _rows(scores, "scores", dtype, dev, rows, width)
     w, ds, pd, sd = _gradient(scores, grad_weight, pairs, out, dtype, dev, rows, width)
-    d = _LossDesc(dev, kind, rows, width, scale, 1 if out is None else 0)
+    d = _loss_desc(dev, kind, rows, width, scale, 1 if out is None else 0)
     i, r = _whole(items, "items", (rows,), torch.int32, dev), _whole(ref_logp, "ref_logp", (rows,), F32, dev)
     logp = scores.new_empty(rows, dtype=F32) if out is None else scores.new_zeros(rows, dtype=F32)   # rows of no list: 0
     loss, margin = scores.new_empty((2, pairs), dtype=F32).unbind()
-    size = _fn("rec_preference_loss_workspace")(C.byref(d), pairs)
+    size = _fn("rec_preference_loss_workspace")(d, pairs)
     ws, pw = _space(size, scores)
-    capi._check(_fn("rec_preference_loss")(C.byref(d), p, s, i, off, pairs, r, beta, label_smoothing, w, loss.data_ptr(), margin.data_ptr(), logp.data_ptr(), pd, sd, pw, size,
+    capi._check(_fn("rec_preference_loss")(d, p, s, i, off, pairs, r, beta, label_smoothing, w, loss.data_ptr(), margin.data_ptr(), logp.data_ptr(), pd, sd, pw, size,
                                            _raw_stream(dev)))
     return PreferenceLoss(loss, margin, logp, ds)
 
@@ -338,7 +321,7 @@ def policy_loss(scores, items, old_logp, advantage, ref_logp=None, *, clip_low=0
     kind, dtype, dev, rows, width = _first(scores, "scores")
     p, s = _rows(scores, "scores", dtype, dev, rows, width)
     w, ds, pd, sd = _gradient(scores, grad_weight, rows, out, dtype, dev, rows, width)
-    d = _LossDesc(dev, kind, rows, width, scale, 0)
+    d = _loss_desc(dev, kind, rows, width, scale, 0)
     vec = (rows,)
     i = _whole(items, "items", vec, torch.int32, dev)
     old, adv, ref = _whole(old_logp, "old_logp", vec, F32, dev), _whole(advantage, "advantage", vec, F32, dev), _whole(ref_logp, "ref_logp", vec, F32, dev)
@@ -347,8 +330,8 @@ def policy_loss(scores, items, old_logp, advantage, ref_logp=None, *, clip_low=0
         kl = None
     else:
         loss, logp, kl = scores.new_empty((3, rows), dtype=F32).unbind()
-    size = _fn("rec_policy_loss_workspace")(C.byref(d))
+    size = _fn("rec_policy_loss_workspace")(d)
     ws, pw = _space(size, scores)
-    capi._check(_fn("rec_policy_loss")(C.byref(d), p, s, i, old, adv, ref, clip_low, clip_high, kl_coef, w, loss.data_ptr(), _ptr(kl), logp.data_ptr(), pd, sd, pw, size,
+    capi._check(_fn("rec_policy_loss")(d, p, s, i, old, adv, ref, clip_low, clip_high, kl_coef, w, loss.data_ptr(), _ptr(kl), logp.data_ptr(), pd, sd, pw, size,
                                        _raw_stream(dev)))
     return PolicyLoss(loss, kl, logp, ds)

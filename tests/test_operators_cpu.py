@@ -9,6 +9,33 @@ import recommendation_amd as ra
 from recommendation_amd import ops
 from tests import operators_ref as ref
 
+
+# the structs of include/recsys_engine.h
+class ConvDesc(C.Structure):
+    _fields_ = [("device", C.c_int32), ("type", C.c_int32), ("rows", C.c_int64), ("n_seq", C.c_int32), ("channels", C.c_int32),
+                ("taps", C.c_int32), ("silu", C.c_int32), ("zero_rest", C.c_int32)]
+
+
+class ScanDesc(C.Structure):
+    _fields_ = [("device", C.c_int32), ("type", C.c_int32), ("rows", C.c_int64), ("n_seq", C.c_int32), ("channels", C.c_int32),
+                ("groups", C.c_int32), ("states", C.c_int32), ("softplus", C.c_int32), ("zero_rest", C.c_int32)]
+
+
+class ScanInputs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("u", "delta", "z", "B", "C")] + \
+               [(n + "_stride", C.c_int64) for n in ("u", "delta", "z", "B", "C")] + \
+               [(n, C.c_void_p) for n in ("A", "D", "delta_bias", "initial")]
+
+
+class ScanGradientPointers(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("du", "ddelta", "dz", "dB", "dC", "dA", "dD", "ddelta_bias", "dinitial")]
+
+
+class LossDesc(C.Structure):
+    _fields_ = [("device", C.c_int32), ("type", C.c_int32), ("rows", C.c_int64), ("n_items", C.c_int64), ("scale", C.c_float),
+                ("zero_rest", C.c_int32)]
+
+
 BUF = (C.c_char * (1 << 16))()
 AT = (C.addressof(BUF) + 255) // 256 * 256     # host memory: a call that is not refused would be stopped by the missing device
 
@@ -19,7 +46,7 @@ def call(name, *args):
 
 
 def conv(entry="rec_history_conv", at=AT, out=AT + 8192, stride=8, ws=0, **kw):
-    d = ops._ConvDesc(**{**dict(device=0, type=0, rows=4, n_seq=1, channels=8, taps=4, silu=1, zero_rest=0), **kw})
+    d = ConvDesc(**{**dict(device=0, type=0, rows=4, n_seq=1, channels=8, taps=4, silu=1, zero_rest=0), **kw})
     if entry == "rec_history_conv":
         return call(entry, C.byref(d), at, stride, AT, None, AT, None, out, stride, None, None)
     if entry == "rec_history_conv_step":
@@ -27,27 +54,27 @@ def conv(entry="rec_history_conv", at=AT, out=AT + 8192, stride=8, ws=0, **kw):
     return call(entry, C.byref(d), AT + 4096, stride, at, stride, AT, None, AT, None, None, out, stride, AT + 30000 // 256 * 256, None, None, AT + 40960, ws, None)
 
 
-CONV_4X8 = ops._ConvDesc(device=0, type=0, rows=4, n_seq=1, channels=8, taps=4, silu=1, zero_rest=0)
+CONV_4X8 = ConvDesc(device=0, type=0, rows=4, n_seq=1, channels=8, taps=4, silu=1, zero_rest=0)
 
 
 def scan(entry="rec_history_scan", in_kw={}, out=AT + 8192, y_stride=8, ws=1 << 20, final=None, **kw):
-    d = ops._ScanDesc(**{**dict(device=0, type=0, rows=4, n_seq=1, channels=8, groups=2, states=4, softplus=1, zero_rest=0), **kw})
-    i = ops._ScanInputs(**{**dict(u=AT, delta=AT + 256, z=None, B=AT + 512, C=AT + 1024, u_stride=8, delta_stride=8, z_stride=0, B_stride=8, C_stride=8, A=AT), **in_kw})
+    d = ScanDesc(**{**dict(device=0, type=0, rows=4, n_seq=1, channels=8, groups=2, states=4, softplus=1, zero_rest=0), **kw})
+    i = ScanInputs(**{**dict(u=AT, delta=AT + 256, z=None, B=AT + 512, C=AT + 1024, u_stride=8, delta_stride=8, z_stride=0, B_stride=8, C_stride=8, A=AT), **in_kw})
     if entry == "rec_history_scan":
         return call(entry, C.byref(d), C.byref(i), AT, out, y_stride, final, None, AT, ws, None)
     if entry == "rec_history_scan_step":
         return call(entry, C.byref(d), C.byref(i), AT, AT + 16384, out, y_stride, None)
-    o = ops._ScanGradientPointers(du=out, ddelta=out + 1024, dB=out + 2048, dC=out + 3200, dA=out + 4096, dinitial=final)
+    o = ScanGradientPointers(du=out, ddelta=out + 1024, dB=out + 2048, dC=out + 3200, dA=out + 4096, dinitial=final)
     return call(entry, C.byref(d), AT + 2048, y_stride, C.byref(i), AT, AT, None, C.byref(o), AT + 32768, ws, None)
 
 
 def preference(out=None, weight=None, stride=16, ws=1 << 20, n_pairs=1, beta=0.1, smoothing=0.0, out_stride=16, **kw):
-    d = ops._LossDesc(**{**dict(device=0, type=0, rows=4, n_items=16, scale=1.0, zero_rest=0), **kw})
+    d = LossDesc(**{**dict(device=0, type=0, rows=4, n_items=16, scale=1.0, zero_rest=0), **kw})
     return call("rec_preference_loss", C.byref(d), AT, stride, AT, AT, n_pairs, None, beta, smoothing, weight, AT, AT, AT, out, out_stride, AT + 16384, ws, None)
 
 
 def policy(out=None, weight=None, clip=(0.2, 0.2), kl=0.0, refs=None, ws=1 << 20, stride=16, **kw):
-    d = ops._LossDesc(**{**dict(device=0, type=0, rows=4, n_items=16, scale=1.0, zero_rest=0), **kw})
+    d = LossDesc(**{**dict(device=0, type=0, rows=4, n_items=16, scale=1.0, zero_rest=0), **kw})
     return call("rec_policy_loss", C.byref(d), AT, stride, AT, AT, AT, refs, *clip, kl, weight, AT, None, AT, out, 16, AT + 16384, ws, None)
 
 
@@ -90,11 +117,21 @@ def test_refused_with_a_reason(case):
     assert rc == -1 and words in said, (rc, said)
 
 
+def test_packed_structs_are_those_of_the_header():
+    for pack, cls, few in ((ops._conv_desc, ConvDesc, (1, 2, 3 << 33, 4, 5, 6, 7, 8)), (ops._scan_desc, ScanDesc, (1, 2, 3 << 33, 4, 5, 6, 7, 8, 9)),
+                           (ops._scan_inputs, ScanInputs, tuple(k << 40 for k in range(1, 15))), (ops._scan_gradients, ScanGradientPointers, tuple(k << 40 for k in range(1, 10))),
+                           (ops._loss_desc, LossDesc, (1, 2, 3 << 33, 4 << 33, 0.5, 6))):
+        packed = pack(*few)
+        assert len(packed) == C.sizeof(cls)
+        back = cls.from_buffer_copy(packed)
+        assert tuple(getattr(back, f[0]) for f in cls._fields_) == few
+
+
 def test_workspace_queries_refuse_what_the_calls_refuse():
-    bad = ops._ScanDesc(device=0, type=0, rows=4, n_seq=1, channels=8, groups=3, states=4)
+    bad = ScanDesc(device=0, type=0, rows=4, n_seq=1, channels=8, groups=3, states=4)
     assert ops._fn("rec_history_scan_workspace")(C.byref(bad)) == -1 and ops._fn("rec_history_scan_backward_workspace")(C.byref(bad)) == -1
     assert ops._fn("rec_history_conv_backward_workspace")(None) == -1 and ops._fn("rec_policy_loss_workspace")(None) == -1
-    none = ops._ScanDesc(device=0, type=0, rows=0, n_seq=0, channels=8, groups=1, states=4)
+    none = ScanDesc(device=0, type=0, rows=0, n_seq=0, channels=8, groups=1, states=4)
     assert ops._fn("rec_history_scan_workspace")(C.byref(none)) == 0
 
 
@@ -166,7 +203,7 @@ def test_loss_reference_gradients_against_differences():
 
 def test_columns_of_one_array_do_not_overlap():
     """An output that is another column slice of the array its input is a slice of passes the check; one column further it does not."""
-    d = ops._ConvDesc(device=99, type=0, rows=4, n_seq=1, channels=8, taps=4, silu=1, zero_rest=0)
+    d = ConvDesc(device=99, type=0, rows=4, n_seq=1, channels=8, taps=4, silu=1, zero_rest=0)
     for shift, words in ((8 * 4, "no such HIP device"), (7 * 4, "overlaps"), (9 * 4, "overlaps"), (0, "overlaps")):
         rc, said = call("rec_history_conv", C.byref(d), AT, 16, AT + 4096, None, AT + 8192, None, AT + shift, 16, None, None)
         assert rc == -1 and words in said, (shift, said)
