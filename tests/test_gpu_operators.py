@@ -2,6 +2,8 @@
 
 Tolerances: the value's own rounding, half a step of its type, plus c * 2^-24 times what the absolute values of the terms add
 up to, c counting the roundings that a term goes through at most.  exp(v) counts |v| + 2 (its argument's rounding and its own)."""
+from concurrent.futures import ThreadPoolExecutor
+
 import numpy as np
 import pytest
 import torch
@@ -644,6 +646,48 @@ def test_nothing_to_do():
     assert float((r.loss - np.log(2)).abs().max()) < 1e-6 and not r.margin.any()
     with pytest.raises(ValueError, match="2 pairs"):
         ops.preference_loss(torch.zeros(4, 9, device=DEV), none, offsets([0, 0]))
+
+
+def test_rows_of_no_history_alone():
+    """No histories at all, though there are rows: zeros, and parameters that learn nothing from what the rows hold."""
+    off = offsets([17])
+    x = torch.full((40, 8), float("nan"), device=DEV)
+    w, A, B = torch.randn(8, 4, device=DEV), -torch.rand(8, 4, device=DEV), x[:, :4].reshape(40, 1, 4)
+    y, fin = ops.history_conv(x, w, w[:, 0].contiguous(), seq_off=off, want_final=True)
+    g = ops.history_conv_backward(x, x, w, w[:, 0].contiguous(), seq_off=off)
+    assert not y.any() and fin.shape == (0, 3, 8) and not g.dx.any() and not g.dweight.any() and not g.dbias.any()
+    y, fin, kept = ops.history_scan(x, x, A, B, B, A[:, 0].contiguous(), x, seq_off=off, want_final=True, want_checkpoints=True)
+    g = ops.history_scan_backward(x, x, x, A, B, B, A[:, 0].contiguous(), x, seq_off=off, checkpoints=kept)
+    assert not y.any() and fin.shape == (0, 8, 4)
+    for name in ("du", "ddelta", "dA", "dB", "dC", "dD", "dz"):
+        assert not getattr(g, name).any(), name
+    r = ops.preference_loss(x, torch.zeros(40, dtype=torch.int32, device=DEV), off, grad_weight=torch.zeros(0, device=DEV))
+    assert r.loss.shape == (0,) and not r.logp.any() and not r.dscores.any()
+
+
+def test_calls_of_two_threads():
+    """Each on a stream of its own, over the same inputs, with workspaces of their own."""
+    x, A = torch.randn(3000, 32, device=DEV), -torch.rand(32, 16, device=DEV)
+    B, off = torch.randn(3000, 1, 16, device=DEV), offsets([0, 1000, 1001, 3000])
+    s, item = torch.randn(6, 50000, device=DEV), torch.arange(6, dtype=torch.int32, device=DEV)
+    two, one = offsets([0, 2, 6]), torch.ones(1, device=DEV)
+
+    def work():
+        y, _, kept = ops.history_scan(x, x, A, B, B, seq_off=off, want_checkpoints=True)
+        g = ops.history_scan_backward(x, x, x, A, B, B, seq_off=off, checkpoints=kept)
+        return y, g.du, g.dA, g.dB, ops.preference_loss(s, item, two, grad_weight=one).dscores
+
+    want = work()
+    torch.cuda.synchronize()
+    with ThreadPoolExecutor(2) as pool:
+        def run(_):
+            with torch.cuda.stream(torch.cuda.Stream()):
+                out = [work() for _ in range(10)]
+                torch.cuda.current_stream().synchronize()
+            return out
+        for outs in pool.map(run, range(2)):
+            for got in outs:
+                assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 def test_element_offsets_beyond_32_bits():
