@@ -296,6 +296,20 @@ __global__ __launch_bounds__(256) void policy_kernel(LossArgs a)
     policy_row(a, row, logp, on, a.coef[row]);
 }
 
+// 16 bytes that are not needed again: the gradient, and the scores it is made of, leave the Infinity Cache to the rows that are
+// yet to be read a second time (2000 rows of 200 000 bf16 scores: 355 us without, 332 so; 1536 rows of preferences 365 and 321 us)
+typedef unsigned int Quad __attribute__((ext_vector_type(4)));
+template <class P> __device__ __forceinline__ P load_once(const P* p)
+{
+    static_assert(sizeof(P) == 16);
+    return __builtin_bit_cast(P, __builtin_nontemporal_load(reinterpret_cast<const Quad*>(p)));
+}
+template <class P> __device__ __forceinline__ void store_once(P* p, const P& v)
+{
+    static_assert(sizeof(P) == 16);
+    __builtin_nontemporal_store(__builtin_bit_cast(Quad, v), reinterpret_cast<Quad*>(p));
+}
+
 // The gradient's elements [j0, j1) of a row, from its end to its beginning: where the same block has just read the row, what it
 // read last is still in the cache.
 template <class T>
@@ -330,13 +344,13 @@ __device__ __forceinline__ void write_gradient(const LossArgs& a, int64_t row, i
         return o;
     };
     const int64_t whole = w.n / (N * step) * (N * step);
-    for (int64_t i = whole + tid; i < w.n; i += step) q[i] = vector_of(p[i], i);
+    for (int64_t i = whole + tid; i < w.n; i += step) store_once(q + i, vector_of(load_once(p + i), i));
     for (int64_t i = whole - N * step + tid; i >= 0; i -= N * step) {
         Pack<T, V> raw[N];
 #pragma unroll
-        for (int n = 0; n < N; n++) raw[n] = p[i + n * step];
+        for (int n = 0; n < N; n++) raw[n] = load_once(p + i + n * step);
 #pragma unroll
-        for (int n = 0; n < N; n++) q[i + n * step] = vector_of(raw[n], i + n * step);
+        for (int n = 0; n < N; n++) store_once(q + i + n * step, vector_of(raw[n], i + n * step));
     }
     for (int64_t j = j0 + tid; j < w.lead; j += step) out[j] = from_f32<T>(of(to_f32(in[j]), j));
     for (int64_t j = w.tail + tid; j < j1; j += step) out[j] = from_f32<T>(of(to_f32(in[j]), j));
@@ -357,7 +371,7 @@ __device__ __forceinline__ void write_zeros(const LossArgs& a, int64_t row, int6
 }
 
 // Rows in falling order: the last ones that the statistics read are the ones still in the Infinity Cache.  1536 rows of 200 000 bf16
-// scores: statistics 130 us, 4.7 TB/s; gradient 214 us, 5.7 TB/s of scores and gradient.
+// scores: statistics 107 us, 5.7 TB/s; gradient 208 us, 5.9 TB/s of scores and gradient.
 template <class T>
 __global__ __launch_bounds__(512) void gradient_kernel(LossArgs a)
 {
@@ -377,7 +391,7 @@ __global__ __launch_bounds__(512) void gradient_kernel(LossArgs a)
 
 // The policy loss where a block takes whole rows: it reads a row twice, but the second time from the cache (two blocks of a
 // compute unit hold 2 x 400 KB of bf16 rows of 200 000 items at a time, 200 MB over the chip, within the 256 MB of Infinity
-// Cache), and one launch does it all (2000 rows: 355 us, 4.5 TB/s of scores and gradient, counted once).
+// Cache), and one launch does it all (2000 rows: 332 us, 4.8 TB/s of scores and gradient, counted once).
 template <class T>
 __global__ __launch_bounds__(1024) void policy_fused_kernel(LossArgs a)
 {
@@ -486,6 +500,18 @@ int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 // one launch does it all, and nothing passes between launches
 bool small_preference(const rec_loss_desc* d) { return d->rows <= kSmallRows && d->rows * d->n_items <= 131072; }
 bool whole_policy(const rec_loss_desc* d) { return splits_of(d) == 1; }
+// Threads for a row that a block reads and then turns into its gradient.  Small blocks keep more rows in flight, and a row's loads
+// over the waits of another's sums; the rows in flight, 2048 threads' worth on each of 256 compute units, should stay within 210 MB
+// of the Infinity Cache.  Few rows take more, down to two or three 16-byte loads a thread, until a quarter of the lanes are
+// busy.  (bf16: 20 000 rows of 20 000 items 599 us with 1024 threads, 356, 350, 345 with 256, 128, 192; 4000 of 60 000 items 234, 198, 206
+// with 1024, 512, 256; 300 of 8000 items 12, 10, 7.6 with 64, 128, 512; f32, 50 000 of 4000 items 579, 311, 326 with 512, 128, 64.)
+int row_threads(const rec_loss_desc* d)
+{
+    const int64_t bytes = d->n_items * rec_type_size(d->type);
+    int threads = 64;
+    while (threads < 1024 && (threads * 400 < bytes || (d->rows * threads < 131072 && bytes / 16 >= 3 * threads))) threads *= 2;
+    return threads;
+}
 int64_t workspace_of(const rec_loss_desc* d) { return d->rows * splits_of(d) * 16 + round16(d->rows * 8) + round16(d->rows * 4); }
 
 int check_call(const rec_loss_desc* d, const void* scores, int64_t scores_stride, const float* grad_weight, int64_t weights, const void* dscores,
@@ -597,10 +623,7 @@ extern "C" int rec_policy_loss(const rec_loss_desc* d, const void* scores, int64
         HIP_TRY(scope.enter(d->device));
         hipStream_t st = (hipStream_t)stream;
         if (whole_policy(d)) {
-            // rows of few items take smaller blocks: two 16-byte loads for each thread at least
-            const int64_t vectors = d->n_items * rec_type_size(d->type) / 16 / 2;
-            const int threads = vectors >= 1024 ? 1024 : vectors < 64 ? 64 : (int)(vectors + 63) / 64 * 64;
-#define CALL(T) policy_fused_kernel<T><<<(unsigned)d->rows, threads, 0, st>>>(a)
+#define CALL(T) policy_fused_kernel<T><<<(unsigned)d->rows, row_threads(d), 0, st>>>(a)
             LOSS_DISPATCH(CALL)
 #undef CALL
             HIP_TRY(hipGetLastError());
