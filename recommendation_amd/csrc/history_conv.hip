@@ -394,10 +394,12 @@ __global__ __launch_bounds__(256) void conv_step_kernel(ConvArgs a, const int32_
 }
 
 // Rows of a strip: long strips read fewer rows twice (gradient above: 163, 142, 134 us at 32, 64, 128 rows), short ones give a small
-// call more threads (2048 x 128 f32 forward: 15 us at 32 rows, 5 at 4).  64k threads fill the chip.
+// call more threads (2048 x 128 f32 forward: 15 us at 32 rows, 5 at 4).  262 144 threads, half of what the chip holds, are enough
+// (100 000 x 128 bf16, forward and gradient: 25 and 56 us with strips for 65 536 threads, 19 and 40 for 131 072, 16 and 36 for 262 144,
+// 19 and 43 for 524 288).
 int strip_rows_of(int64_t rows, int64_t nvec, int longest)
 {
-    const int64_t s = rows * nvec / 65536 / 4 * 4;
+    const int64_t s = rows * nvec / 262144 / 4 * 4;
     return (int)(s < 4 ? 4 : s > longest ? longest : s);
 }
 constexpr int kForwardVec = 2, kBackwardVec = 2;
