@@ -499,7 +499,9 @@ int splits_of(const rec_loss_desc* d)
 int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 // one launch does it all, and nothing passes between launches
 bool small_preference(const rec_loss_desc* d) { return d->rows <= kSmallRows && d->rows * d->n_items <= 131072; }
-bool whole_policy(const rec_loss_desc* d) { return splits_of(d) == 1; }
+// (64, 256 and 900 rows of 20 000 bf16 items: calls of 13, 14 and 20 us, 20, 21 and 36 by three launches over parts of rows; 900 of
+// 200 000 items 158 and 194)
+bool whole_policy(const rec_loss_desc* d) { return splits_of(d) == 1 || d->rows >= 512 || d->n_items * rec_type_size(d->type) < 65536; }
 // Threads for a row that a block reads and then turns into its gradient.  Small blocks keep more rows in flight, and a row's loads
 // over the waits of another's sums; the rows in flight, 2048 threads' worth on each of 256 compute units, should stay within 210 MB
 // of the Infinity Cache.  Few rows take more, down to two or three 16-byte loads a thread, until a quarter of the lanes are
@@ -510,6 +512,15 @@ int row_threads(const rec_loss_desc* d)
     const int64_t bytes = d->n_items * rec_type_size(d->type);
     int threads = 64;
     while (threads < 1024 && (threads * 400 < bytes || (d->rows * threads < 131072 && bytes / 16 >= 3 * threads))) threads *= 2;
+    return threads;
+}
+// Threads for a row, or a part of one, where one launch reads the scores and another makes the gradient: four 16-byte loads each at
+// least (500 000 rows of 300 bf16 items 3734 us with 512 threads, 677 with 64; 8000 of 2000 items 70 and 37).
+int part_threads(const rec_loss_desc* d)
+{
+    const int64_t vectors = d->n_items * rec_type_size(d->type) / 16;
+    int threads = 64;
+    while (threads < kThreads && (splits_of(d) > 1 || vectors >= 8 * threads)) threads *= 2;
     return threads;
 }
 int64_t workspace_of(const rec_loss_desc* d) { return d->rows * splits_of(d) * 16 + round16(d->rows * 8) + round16(d->rows * 4); }
@@ -586,9 +597,9 @@ extern "C" int rec_preference_loss(const rec_loss_desc* d, const void* scores, i
         }
         const unsigned blocks = (unsigned)(d->rows * a.splits);
 #define CALL(T)                                                                                     \
-        if (blocks) row_statistics_kernel<T><<<blocks, kThreads, 0, st>>>(a);                       \
+        if (blocks) row_statistics_kernel<T><<<blocks, part_threads(d), 0, st>>>(a);                       \
         if (n_pairs) preference_kernel<T><<<(unsigned)n_pairs, 256, 0, st>>>(a);                    \
-        if (blocks && dscores) gradient_kernel<T><<<blocks, kThreads, 0, st>>>(a)
+        if (blocks && dscores) gradient_kernel<T><<<blocks, part_threads(d), 0, st>>>(a)
         LOSS_DISPATCH(CALL)
 #undef CALL
         if (d->zero_rest && !dscores && d->rows > 0) rest_kernel<<<(unsigned)((d->rows + 255) / 256), 256, 0, st>>>(a);
@@ -631,9 +642,9 @@ extern "C" int rec_policy_loss(const rec_loss_desc* d, const void* scores, int64
         }
         const unsigned blocks = (unsigned)(d->rows * a.splits);
 #define CALL(T)                                                                                     \
-        row_statistics_kernel<T><<<blocks, kThreads, 0, st>>>(a);                                   \
+        row_statistics_kernel<T><<<blocks, part_threads(d), 0, st>>>(a);                                   \
         policy_kernel<T><<<(unsigned)((d->rows + 3) / 4), 256, 0, st>>>(a);                         \
-        if (dscores) gradient_kernel<T><<<blocks, kThreads, 0, st>>>(a)
+        if (dscores) gradient_kernel<T><<<blocks, part_threads(d), 0, st>>>(a)
         LOSS_DISPATCH(CALL)
 #undef CALL
         HIP_TRY(hipGetLastError());
