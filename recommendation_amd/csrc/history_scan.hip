@@ -202,13 +202,15 @@ __global__ __launch_bounds__(256) void scan_local_kernel(ScanArgs a)
 
 // second pass: the state handed into chunk c + 1 is exp(A span) of what was handed into c (where c's history came from there), plus
 // what c adds.  Such steps compose, so 64 threads share the chunks of a channel's state: each composes a run of them, then
-// walks it again from what the runs in front of it lead to.
+// walks it again from what the runs in front of it lead to.  A run in which a history begins takes nothing over: `cut`, and not a
+// factor of 0, says so, for a factor that underflows still makes NaN of what is not finite, and NaN times 0 is not 0.
 // The gradient takes the same steps from the back.
 constexpr int LINK_COLS = 16, LINK_RUNS = 64;
 template <bool BACK>
 __global__ __launch_bounds__(LINK_COLS * LINK_RUNS) void scan_link_kernel(ScanArgs a)
 {
     __shared__ float sP[LINK_RUNS][LINK_COLS], sH[LINK_RUNS][LINK_COLS];
+    __shared__ bool s_cut[LINK_RUNS][LINK_COLS];
     const int col = threadIdx.x % LINK_COLS, run = threadIdx.x / LINK_COLS;
     const int64_t i = (int64_t)blockIdx.x * LINK_COLS + col, n = (int64_t)a.channels * a.states;
     const bool on = i < n;
@@ -238,19 +240,23 @@ __global__ __launch_bounds__(LINK_COLS * LINK_RUNS) void scan_link_kernel(ScanAr
         }
     };
     float P = 1.0f, H = 0.0f;
+    bool cut = false;
     if (on)
         walk([&](int, int kind, float own, float f) {
-            P = kind == 2 ? P * f : 0.0f;
+            cut |= kind != 2;
+            P *= f;
             H = kind == 2 ? fmaf(f, H, own) : kind == 1 ? own : 0.0f;
         });
     // what the runs up to each one lead to, by doubling
     for (int o = 1; o < LINK_RUNS; o *= 2) {
         sP[run][col] = P;
         sH[run][col] = H;
+        s_cut[run][col] = cut;
         __syncthreads();
-        if (run >= o) {
-            if (P != 0.0f) H = fmaf(P, sH[run - o][col], H);   // (a run that takes nothing over ignores what is in front of it, infinite or not)
+        if (run >= o && !cut) {
+            H = fmaf(P, sH[run - o][col], H);
             P *= sP[run - o][col];
+            cut = s_cut[run - o][col];
         }
         __syncthreads();
     }

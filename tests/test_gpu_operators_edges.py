@@ -1,0 +1,86 @@
+"""The device operators where a call is cut, linked or looped over: values that are not finite and states that grow across the chunks
+of a long history, launches whose blocks go around, counts near their limits, and writes beside the outputs.  Needs an MI355X.
+
+Tolerances as in test_gpu_operators: half a step of the value's type, plus a count of roundings times 2^-24 of the terms' size."""
+
+import pytest
+import torch
+
+from recommendation_amd import capi, ops
+from tests import operators_ref as ref
+from tests.test_gpu_operators import DEV, LEAST, TYPES, U, Source, close, offsets
+
+pytestmark = pytest.mark.gpu
+
+
+def close_on_gpu(got, want, slack, what):
+    """`close` for arrays of a gigabyte, all finite."""
+    allowed = (want.abs() + slack).mul_(torch.finfo(got.dtype).eps / 2).add_(slack).add_(LEAST[got.dtype])
+    off = float(got.double().sub_(want).abs_().sub_(allowed).max())
+    assert off <= 0, (what, off, float(allowed.max()))
+
+
+def scan_arrays(rows, ch, N, histories, seed=1, decay=None):
+    src = Source(seed, torch.float32)
+    u, delta, dy = (src(rows, ch)[0] for _ in range(3))
+    B, Cm = src(rows, 1, N)[0], src(rows, 1, N)[0]
+    A = torch.full((ch, N), decay, device=DEV) if decay is not None else -torch.rand(ch, N, generator=src.gen).to(DEV) - 0.05
+    return u, delta, dy, B, Cm, A, src(histories, ch, N)[0], src(histories, ch, N)[0]
+
+
+def same(a, b):
+    return int((a.cpu() != b).sum()) == 0
+
+
+# ------------------------------------------------------------------ values that are not finite, over many chunks
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("states", [True, False])
+def test_what_is_not_finite_reaches_the_end_of_a_long_history(value, states):
+    """A decay of 8 forgets a finite state within a chunk - its factor is 0 in f32 - but 0 times what is not finite is not 0."""
+    rows, ch, N, off = 7000, 16, 8, [0, 500, 6500, 7000]
+    u, delta, dy, B, Cm, A, init, dfin = scan_arrays(rows, ch, N, 3, decay=-8.0)
+    kw = dict(seq_off=offsets(off), initial=init if states else None)
+    bad = u.clone()
+    bad[600, 3] = value
+    y, fin, _ = ops.history_scan(bad, delta, A, B, Cm, want_final=True, **kw)
+    other = [d for d in range(ch) if d != 3]
+    assert torch.isfinite(y[:, other]).all() and torch.isfinite(fin[:, other]).all()
+    inside = torch.zeros(rows, dtype=torch.bool)
+    inside[600:6500] = True
+    assert same(~torch.isfinite(y[:, 3]), inside)
+    assert not torch.isfinite(fin[1, 3]).any() and torch.isfinite(fin[[0, 2], 3]).all()
+    # the gradient, from a row near the end to the history's beginning
+    _, _, kept = ops.history_scan(u, delta, A, B, Cm, want_checkpoints=True, **kw)
+    dy[6400, 3] = value
+    g = ops.history_scan_backward(dy, u, delta, A, B, Cm, checkpoints=kept, dfinal=dfin if states else None, **kw)
+    inside[:] = False
+    inside[500:6401] = True
+    for name in ("du", "ddelta"):
+        t = getattr(g, name)
+        assert torch.isfinite(t[:, other]).all(), name
+        assert same(~torch.isfinite(t[:, 3]), inside), name
+    assert same(~torch.isfinite(g.dB[:, 0]).all(1), inside)
+    if states:
+        assert not torch.isfinite(g.dinitial[1, 3]).any() and torch.isfinite(g.dinitial[[0, 2], 3]).all() and torch.isfinite(g.dinitial[:, other]).all()
+
+
+@pytest.mark.parametrize("states", [True, False])
+def test_a_decay_that_is_not_finite_stays_in_its_history(states):
+    """Chunks of 16 rows; a delta of NaN makes the decay of a whole chunk NaN, the next history begins in the chunk behind it (for the
+    gradient: ends in the one in front) and runs over fifty more."""
+    rows, ch, N, off = 1000, 16, 8, [0, 100, 900, 1000]
+    u, delta, dy, B, Cm, A, init, dfin = scan_arrays(rows, ch, N, 3)
+    delta[80:96, 3] = delta[912:928, 3] = float("nan")
+    kw = dict(seq_off=offsets(off), initial=init if states else None)
+    y, fin, kept = ops.history_scan(u, delta, A, B, Cm, want_final=True, want_checkpoints=True, **kw)
+    bad = torch.zeros(rows, dtype=torch.bool)
+    bad[80:100] = bad[912:1000] = True
+    assert same(torch.isnan(y[:, 3]), bad)
+    assert torch.isnan(fin[[0, 2], 3]).all() and torch.isfinite(fin[1]).all()
+    g = ops.history_scan_backward(dy, u, delta, A, B, Cm, checkpoints=kept, dfinal=dfin if states else None, **kw)
+    for name in ("du", "ddelta"):
+        assert torch.isfinite(getattr(g, name)[100:900]).all(), name
+        assert torch.isnan(getattr(g, name)[900:928, 3]).all(), name
+    assert torch.isfinite(g.dB[100:900]).all() and torch.isfinite(g.dC[100:900]).all()
+    if states:
+        assert torch.isfinite(g.dinitial[1]).all() and torch.isnan(g.dinitial[[0, 2], 3]).all()
