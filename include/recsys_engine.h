@@ -391,6 +391,8 @@ typedef struct {
 
 /* Selective state space scan over each history, h[channels][states] starting at its initial state:
  *     h = exp(delta_t A) h + delta_t u_t B_t        y_t = (sum_n C_t[n] h[n] + D u_t) * (z_t / (1 + exp(-z_t)))
+ * A in (-2^127, 2^127).  States may grow (delta A > 0) as far as f32 holds them, however the rows are cut; a NaN or an infinity
+ * stays in its history's channel up to the history's end, and so it does backwards in the gradient.
  * final_state (optional): [n_seq][channels][states] f32, initial of an empty history.  checkpoints (optional): the states in
  * front of every REC_SCAN_CHECKPOINT-th packed row, [ceil(rows / REC_SCAN_CHECKPOINT)][channels][states] f32, which the
  * gradient starts its recomputation from. */

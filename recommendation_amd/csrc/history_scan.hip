@@ -12,7 +12,7 @@
 // walks again from the linked states and writes y.  With one chunk the first two are not launched.
 //
 // Bound by vector instructions: per row and state one exp and three multiply-adds forwards, one exp and some ten backwards, and
-// the sums over states and channels.  100 000 rows of 128 bf16 channels with 16 states (1000 histories): 45 + 16 + 80 us for
+// the sums over states and channels.  100 000 rows of 128 bf16 channels with 16 states (1000 histories): 45 + 17 + 80 us for
 // the three passes, 48 + 21 + 243 and 12 + 9 for sums backwards, where the arrays alone would take 45 us in all at the rate of a copy.
 #include "operators.h"
 #include <type_traits>
@@ -200,22 +200,31 @@ __global__ __launch_bounds__(256) void scan_local_kernel(ScanArgs a)
     if (p.on && p.lane_n == 0) a.span[(int64_t)p.chunk * a.channels + p.d] = span;
 }
 
-// second pass: the state handed into chunk c + 1 is exp(A span) of what was handed into c (where c's history came from there), plus
+// The state behind rows whose decays multiply to 2^(2 x), and what those rows add to it.  The factor may be beyond f32 where the
+// state is not - nothing is there to grow yet, or it is far from the end of the range - so its root is taken twice.  It is cut at
+// 2^254, which leaves nothing of f32's normal range but infinity, so that 0 stays 0.
+__device__ __forceinline__ float carried(float h, float x, float own)
+{
+    const float e = fast_exp2(x), root = x > 127.0f ? 0x1p127f : e;
+    return fmaf(h * root, root, own);
+}
+
+// second pass: the state handed into chunk c + 1 is exp(A span) times what was handed into c (where c's history came from there), plus
 // what c adds.  Such steps compose, so 64 threads share the chunks of a channel's state: each composes a run of them, then
-// walks it again from what the runs in front of it lead to.  A run in which a history begins takes nothing over: `cut`, and not a
-// factor of 0, says so, for a factor that underflows still makes NaN of what is not finite, and NaN times 0 is not 0.
+// walks it again from what the runs in front of it lead to.  The exponents are added, not the factors multiplied.  A run in which
+// a history begins takes nothing over: `cut`, and not a factor of 0, says so, for a factor that underflows still makes NaN of NaN.
 // The gradient takes the same steps from the back.
 constexpr int LINK_COLS = 16, LINK_RUNS = 64;
 template <bool BACK>
 __global__ __launch_bounds__(LINK_COLS * LINK_RUNS) void scan_link_kernel(ScanArgs a)
 {
-    __shared__ float sP[LINK_RUNS][LINK_COLS], sH[LINK_RUNS][LINK_COLS];
+    __shared__ float sX[LINK_RUNS][LINK_COLS], sH[LINK_RUNS][LINK_COLS];
     __shared__ bool s_cut[LINK_RUNS][LINK_COLS];
     const int col = threadIdx.x % LINK_COLS, run = threadIdx.x / LINK_COLS;
     const int64_t i = (int64_t)blockIdx.x * LINK_COLS + col, n = (int64_t)a.channels * a.states;
     const bool on = i < n;
     const int d = on ? (int)(i / a.states) : 0;
-    const float A2 = on ? a.A[i] * REC_LOG2E : 0.0f;
+    const float A2 = on ? a.A[i] * (0.5f * REC_LOG2E) : 0.0f;   // halves of the exponents, as carried() wants them
     const int steps = a.chunks - 1, per = (steps + LINK_RUNS - 1) / LINK_RUNS;
     const int k0 = min(run * per, steps), k1 = min(k0 + per, steps);
     // step k: forwards from chunk k, whose state goes to slot k + 1; backwards from chunk `steps - k`, whose gradient is in its own slot
@@ -236,26 +245,26 @@ __global__ __launch_bounds__(LINK_COLS * LINK_RUNS) void scan_link_kernel(ScanAr
             }
 #pragma unroll
             for (int e = 0; e < AHEAD; e++)
-                if (k + e < k1) step(k + e, kind[e], own[e], fast_exp2(A2 * span[e]));
+                if (k + e < k1) step(k + e, kind[e], own[e], A2 * span[e]);
         }
     };
-    float P = 1.0f, H = 0.0f;
+    float X = 0.0f, H = 0.0f;
     bool cut = false;
     if (on)
-        walk([&](int, int kind, float own, float f) {
+        walk([&](int, int kind, float own, float x) {
             cut |= kind != 2;
-            P *= f;
-            H = kind == 2 ? fmaf(f, H, own) : kind == 1 ? own : 0.0f;
+            X += x;
+            H = kind == 2 ? carried(H, x, own) : kind == 1 ? own : 0.0f;
         });
     // what the runs up to each one lead to, by doubling
     for (int o = 1; o < LINK_RUNS; o *= 2) {
-        sP[run][col] = P;
+        sX[run][col] = X;
         sH[run][col] = H;
         s_cut[run][col] = cut;
         __syncthreads();
         if (run >= o && !cut) {
-            H = fmaf(P, sH[run - o][col], H);
-            P *= sP[run - o][col];
+            H = carried(sH[run - o][col], X, H);
+            X += sX[run - o][col];
             cut = s_cut[run - o][col];
         }
         __syncthreads();
@@ -264,8 +273,8 @@ __global__ __launch_bounds__(LINK_COLS * LINK_RUNS) void scan_link_kernel(ScanAr
     __syncthreads();
     float h = run > 0 ? sH[run - 1][col] : 0.0f;
     if (!on) return;
-    walk([&](int k, int kind, float own, float f) {
-        h = kind == 2 ? fmaf(f, h, own) : kind == 1 ? own : 0.0f;
+    walk([&](int k, int kind, float own, float x) {
+        h = kind == 2 ? carried(h, x, own) : kind == 1 ? own : 0.0f;
         a.link[slot_of(k)] = h;
     });
 }

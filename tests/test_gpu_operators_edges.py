@@ -84,3 +84,37 @@ def test_a_decay_that_is_not_finite_stays_in_its_history(states):
     assert torch.isfinite(g.dB[100:900]).all() and torch.isfinite(g.dC[100:900]).all()
     if states:
         assert torch.isfinite(g.dinitial[1]).all() and torch.isnan(g.dinitial[[0, 2], 3]).all()
+
+
+# ------------------------------------------------------------------ states that grow
+@pytest.mark.parametrize("late", [True, False])
+def test_states_that_grow_over_many_chunks(late):
+    """exp(delta A) > 1.  late: the factor over the history is e^450, beyond f32, but nothing is there to grow until 100 rows are left; else
+    2^-120 grows by e^90, 2^129.8, to some hundreds.  Both are far from the end of f32 in every row."""
+    rows, ch, N, off = 2000, 8, 4, [0, 1800, 2000]
+    u, _, dy, B, Cm, _, init, dfin = scan_arrays(rows, ch, N, 2, seed=7)
+    step = 0.25 if late else 0.05
+    A = -torch.ones(ch, N, device=DEV)
+    delta = torch.full((rows, ch), -step, device=DEV)
+    if late:
+        u[:1700], u[1900:] = 0, 0
+        init.zero_(), dfin.zero_()
+        dy[100:1800], dy[1850:] = 0, 0
+    else:
+        u.zero_(), dy.zero_()
+        init, dfin = init.sign() * 2.0 ** -120, dfin.sign() * 2.0 ** -120
+    six = dict(u=u.double(), delta=delta.double(), A=A.double(), B=B.double(), C=Cm.double(), D=None, z=None, bias=None, initial=init.double(), off=off, use_softplus=False)
+    y6, fin6 = ref.scan(**six)
+    ya, fina = ref.scan(**six, absolute=True)
+    kw = dict(seq_off=offsets(off), initial=init, softplus=False)
+    y, fin, kept = ops.history_scan(u, delta, A, B, Cm, want_final=True, want_checkpoints=True, **kw)
+    # a step's roundings as everywhere, and an exponent of up to 650 (base 2) that some ten additions have made
+    c = U * (1800 * (12 * step + 6) + 24 + 10 * 650)
+    assert float(fin6.abs().max()) > 1 and float(fin6.abs().max()) < 2.0 ** 100
+    close(y, y6.cpu(), (c * ya).cpu(), "y")
+    close(fin, fin6.cpu(), (c * fina).cpu(), "final")
+    g = ops.history_scan_backward(dy, u, delta, A, B, Cm, checkpoints=kept, dfinal=dfin, **kw)
+    want = ref.scan_gradient(dy.double(), **six, dfinal=dfin.double())
+    size = ref.scan_gradient(dy.double(), **six, dfinal=dfin.double(), absolute=True)
+    for name, got in (("u", g.du), ("initial", g.dinitial)):
+        close(got, want[name].cpu(), (2 * c * size[name]).cpu(), name)
