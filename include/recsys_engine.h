@@ -341,7 +341,7 @@ enum rec_type { REC_TYPE_F32 = 0, REC_TYPE_F16 = 1, REC_TYPE_BF16 = 2 };
 typedef struct {
     int32_t device, type;     /* HIP device ordinal, enum rec_type */
     int64_t rows;             /* packed rows (steps: clicks), at most 2^31 - 1 */
-    int32_t n_seq;            /* sequences (steps: slots of the state) */
+    int32_t n_seq;            /* sequences (steps: slots of the state), at most 2^31 - 2 */
     int32_t channels;
     int32_t taps;             /* 2 .. 8 */
     int32_t silu;             /* 1: y = v / (1 + exp(-v)) of the sum v below, 0: y = v */
@@ -373,7 +373,7 @@ int rec_history_conv_step(const rec_conv_desc* d, const void* x, int64_t x_strid
 typedef struct {
     int32_t device, type;
     int64_t rows;             /* packed rows (steps: clicks), at most 2^31 - 1 */
-    int32_t n_seq;            /* sequences (steps: slots of the state) */
+    int32_t n_seq;            /* sequences (steps: slots of the state), at most 2^31 - 2 */
     int32_t channels, groups; /* channel d takes B and C of group d / (channels / groups); groups divides channels */
     int32_t states;           /* 1 .. 64 per channel */
     int32_t softplus;         /* 1: delta = log(1 + exp(v)), 0: delta = v, of v = raw delta + delta_bias */

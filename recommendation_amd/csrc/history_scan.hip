@@ -864,7 +864,7 @@ int check_desc(const rec_scan_desc* d)
     REC_REFUSE(!d, "null argument");
     REC_REFUSE(d->type < REC_TYPE_F32 || d->type > REC_TYPE_BF16, "unknown type");
     REC_REFUSE(d->rows < 0 || d->rows > INT32_MAX, "rows must be in 0..2^31-1");
-    REC_REFUSE(d->n_seq < 0, "n_seq must not be negative");
+    REC_REFUSE(d->n_seq < 0 || d->n_seq == INT32_MAX, "n_seq must be in 0..2^31-2");
     REC_REFUSE(d->channels < 1 || d->channels > 1 << 20, "channels must be in 1..2^20");
     REC_REFUSE(d->groups < 1 || d->channels % d->groups, "groups must divide the channels");
     REC_REFUSE(d->states < 1 || d->states > 64, "states must be in 1..64");

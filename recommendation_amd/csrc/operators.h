@@ -69,9 +69,9 @@ template <class T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
 // Only compares what it reads: offsets that are out of order lead to some s in [-1, n_seq], never out of the arrays.
 __device__ __forceinline__ int sequence_of(const int64_t* __restrict__ off, int n_seq, int64_t row)
 {
-    int lo = 0, hi = n_seq + 1;   // first index whose offset is beyond the row
+    int lo = 0, hi = n_seq + 1;   // first index whose offset is beyond the row (n_seq < 2^31 - 1; lo + hi may be more than an int)
     while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
+        const int mid = lo + ((hi - lo) >> 1);
         if (off[mid] <= row) lo = mid + 1; else hi = mid;
     }
     return lo - 1;

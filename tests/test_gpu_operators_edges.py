@@ -118,3 +118,26 @@ def test_states_that_grow_over_many_chunks(late):
     size = ref.scan_gradient(dy.double(), **six, dfinal=dfin.double(), absolute=True)
     for name, got in (("u", g.du), ("initial", g.dinitial)):
         close(got, want[name].cpu(), (2 * c * size[name]).cpu(), name)
+
+
+def test_more_than_a_billion_histories():
+    """Histories whose numbers are beyond 2^30: the middle of two of them is beyond an int before it is halved."""
+    n = (1 << 30) + 21
+    full, at = [0, 40, 120, 200], [3, (1 << 30) + 4, n - 1]
+    off = torch.zeros(n + 1, dtype=torch.int64, device=DEV)
+    off[at[0] + 1:] = 40
+    off[at[1] + 1:] = 120
+    off[n:] = 200
+    few = offsets(full)
+    x, dy, w, B = torch.randn(200, 8, device=DEV), torch.randn(200, 8, device=DEV), torch.randn(8, 4, device=DEV), torch.randn(200, 1, 4, device=DEV)
+    A = -torch.rand(8, 4, device=DEV)
+    out = []
+    for o in (off, few):
+        y, _ = ops.history_conv(x, w, seq_off=o)
+        g = ops.history_conv_backward(dy, x, w, seq_off=o)
+        ys, _, kept = ops.history_scan(x, x, A, B, B, seq_off=o, want_checkpoints=True)
+        gs = ops.history_scan_backward(dy, x, x, A, B, B, seq_off=o, checkpoints=kept)
+        out.append([y, g.dx, g.dweight, ys, kept, gs.du, gs.ddelta, gs.dA, gs.dB, gs.dC])
+    assert all(torch.equal(a, b) for a, b in zip(*out))
+    del off
+    torch.cuda.empty_cache()
