@@ -335,7 +335,7 @@ int rec_kernel_stats(rec_engine* e, int which, double* total_ms, int64_t* launch
  * nothing, wait for nothing and can be captured into a HIP graph.  A workspace needs no initial contents and holds nothing
  * between calls; calls that may overlap in time, replays of two captured graphs among them, need one each.  The outputs of a
  * call must not overlap its inputs or each other, except where an entry says so.  Results do not depend on timing: equal inputs
- * give equal bits.  Entry points that need a workspace of rec_..._workspace() bytes take NULL where that is 0. */
+ * give equal bits.  A call that would take a launch of 2^32 threads or more is refused as a whole.  Entry points that need a workspace of rec_..._workspace() bytes take NULL where that is 0. */
 enum rec_type { REC_TYPE_F32 = 0, REC_TYPE_F16 = 1, REC_TYPE_BF16 = 2 };
 
 typedef struct {

@@ -950,6 +950,9 @@ int check_blocks(int64_t blocks)
     return 0;
 }
 
+// a launch for n columns, `cols` to a block, `times` threads a column: as many blocks of 256 threads as that would be
+int64_t in_blocks(int64_t n, int64_t cols, int64_t times) { return (n + cols - 1) / cols * (cols * times / 256); }
+
 int check_workspace(const void* p, int64_t has, int64_t needs)
 {
     REC_REFUSE(has < needs, "the workspace is too small");
@@ -991,10 +994,11 @@ extern "C" int rec_history_scan(const rec_scan_desc* d, const rec_scan_inputs* i
         REC_REFUSE(rec_overlap(in->initial, state_bytes(d), final_state, state_bytes(d)), "final_state overlaps initial");
         const Cut c = cut_of(d, kForwardBlocks, pass_lanes(d));
         if (int rc = check_workspace(workspace, workspace_bytes, link_bytes(d, c))) return rc;
-        if (int rc = rec_check_device(d->device)) return rc;
         const int64_t blocks = (int64_t)c.chunks * c.tiles, n = (int64_t)d->channels * d->states;
         const int64_t empty_blocks = final_state ? (n * d->n_seq + 255) / 256 : 0;
         if (int rc = check_blocks(blocks + empty_blocks)) return rc;
+        if (int rc = check_blocks(c.chunks > 1 ? in_blocks(n, LINK_COLS, LINK_RUNS) : 0)) return rc;
+        if (int rc = rec_check_device(d->device)) return rc;
         ScanArgs a = {};
         fill(a, d, in, c);
         a.off = seq_off; a.y = y; a.y_stride = y_stride; a.final_state = final_state; a.checkpoints = checkpoints;
@@ -1051,13 +1055,14 @@ extern "C" int rec_history_scan_backward(const rec_scan_desc* d, const void* dy,
         REC_REFUSE(rec_overlap(in->initial, state_bytes(d), out->dinitial, state_bytes(d)) || rec_overlap(dfinal, state_bytes(d), out->dinitial, state_bytes(d)),
                    "dinitial overlaps initial or dfinal");
         if (int rc = check_workspace(workspace, workspace_bytes, rec_history_scan_backward_workspace(d))) return rc;
-        if (int rc = rec_check_device(d->device)) return rc;
         const Cut c = cut_of(d, kBackwardBlocks, pass_lanes(d));
         const int64_t blocks = (int64_t)c.chunks * c.tiles, n = (int64_t)d->channels * d->states;
         const int64_t empty_blocks = out->dinitial ? (n * d->n_seq + 255) / 256 : 0;
         const int64_t sum_blocks = c.tiles_per_group > 1 ? (d->rows + SUM_ROWS - 1) / SUM_ROWS : 0;
-        if (int rc = check_blocks(blocks + empty_blocks > sum_blocks ? blocks + empty_blocks : sum_blocks)) return rc;
         const bool params = out->dA || out->dD || out->ddelta_bias;
+        for (int64_t launch : {blocks + empty_blocks, sum_blocks, c.chunks > 1 ? in_blocks(n, LINK_COLS, LINK_RUNS) : 0, params ? sum_partials_blocks(n + 2 * d->channels) : 0})
+            if (int rc = check_blocks(launch)) return rc;
+        if (int rc = rec_check_device(d->device)) return rc;
         ScanArgs a = {};
         fill(a, d, in, c);
         a.off = seq_off; a.dy = dy; a.dy_stride = dy_stride; a.checkpoints_in = checkpoints; a.dfinal = dfinal;

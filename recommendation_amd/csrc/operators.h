@@ -57,6 +57,8 @@ inline bool rec_aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1
 // sums over the rows of a partial matrix [n_rows][n_cols], in row order, in 64 bits: columns [0, n0) to out0, [n0, n0 + n1) to
 // out1, the rest to out2 (each may be null)
 int launch_sum_partials(const float* part, int64_t n_rows, int64_t n_cols, float* out0, int64_t n0, float* out1, int64_t n1, float* out2, hipStream_t st);
+// the launch's size, in blocks of 256 threads
+int64_t sum_partials_blocks(int64_t n_cols);
 
 #ifdef __HIPCC__
 // ---- device side

@@ -33,6 +33,8 @@ __global__ __launch_bounds__(1024) void sum_partials_kernel(const float* __restr
 
 }  // namespace
 
+int64_t sum_partials_blocks(int64_t n_cols) { return (n_cols + SUM_COLS - 1) / SUM_COLS * (SUM_COLS * SUM_ROWS / 256); }
+
 int launch_sum_partials(const float* part, int64_t n_rows, int64_t n_cols, float* out0, int64_t n0, float* out1, int64_t n1, float* out2, hipStream_t st)
 {
     sum_partials_kernel<<<(unsigned)((n_cols + SUM_COLS - 1) / SUM_COLS), SUM_COLS * SUM_ROWS, 0, st>>>(part, n_rows, n_cols, out0, n0, out1, n1, out2);

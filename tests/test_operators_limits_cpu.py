@@ -1,9 +1,29 @@
 """More refusals of the device operators (no GPU needed): counts at the ends of their ranges."""
+import ctypes as C
+
 import pytest
 
-from tests.test_operators_cpu import conv, scan
+from tests.test_operators_cpu import AT, ScanDesc, ScanGradientPointers, ScanInputs, call, conv, scan
+
+FAR = 1 << 40
+WIDE = dict(channels=1 << 20, groups=1, y_stride=1 << 20, ws=1 << 60, out=AT + FAR)   # as wide as a call may be
+IN = dict(u_stride=1 << 20, delta_stride=1 << 20, B_stride=64, C_stride=64, B=AT + 2 * FAR, C=AT + 2 * FAR)
+
+
+def wide_gradient(rows, states, device=0, dA=True):
+    """rec_history_scan_backward of 2^20 channels, its arrays far from each other."""
+    d = ScanDesc(device=device, type=0, rows=rows, n_seq=1, channels=1 << 20, groups=1, states=states, softplus=1, zero_rest=0)
+    i = ScanInputs(u=AT, delta=AT, B=AT + FAR, C=AT + FAR, u_stride=1 << 20, delta_stride=1 << 20, B_stride=states, C_stride=states, A=AT)
+    o = ScanGradientPointers(du=AT + 2 * FAR, ddelta=AT + 3 * FAR, dB=AT + 4 * FAR, dC=AT + 5 * FAR, dA=AT if dA else None)
+    return call("rec_history_scan_backward", C.byref(d), AT + 6 * FAR, 1 << 20, C.byref(i), AT, AT, None, C.byref(o), AT, 1 << 60, None)
+
 
 REFUSED = [
+    # launches of 2^32 threads: the link of 2^26 states, the sums over 2^26 parameters and more
+    (lambda: scan(rows=1024, states=64, in_kw=IN, **WIDE), "too many"), (lambda: scan(rows=1024, states=63, in_kw=IN, device=99, **WIDE), "no such HIP device"),
+    (lambda: scan(rows=16, states=64, in_kw=IN, device=99, **WIDE), "no such HIP device"),
+    (lambda: wide_gradient(16, 62), "too many"), (lambda: wide_gradient(16, 61, device=99), "no such HIP device"), (lambda: wide_gradient(16, 62, device=99, dA=False), "no such HIP device"),
+    (lambda: wide_gradient(1024, 64, dA=False), "too many"),
     (lambda: conv(n_seq=(1 << 31) - 1), "n_seq must be"), (lambda: conv("rec_history_conv_backward", n_seq=(1 << 31) - 1), "n_seq must be"),
     (lambda: scan(n_seq=(1 << 31) - 1), "n_seq must be"), (lambda: scan("rec_history_scan_step", n_seq=(1 << 31) - 1), "n_seq must be"),
     (lambda: conv(n_seq=(1 << 31) - 2, device=99), "no such HIP device"), (lambda: scan(n_seq=(1 << 31) - 2, device=99), "no such HIP device"),
