@@ -73,10 +73,8 @@ __device__ __forceinline__ void load_window(const ConvArgs& a, int s, int64_t st
 // The windows that histories leave behind: item q of sequence s is its row end - (W-1) + q, or item q + length of its initial
 // window where the history is shorter than that.  One thread per (sequence, item, V channels), in blocks behind the strips'.
 template <class T, int W, int V>
-__device__ __forceinline__ void final_windows(const ConvArgs& a, int64_t i)
+__device__ __forceinline__ void final_window(const ConvArgs& a, int64_t i)
 {
-    const int64_t n = (int64_t)a.n_seq * (W - 1) * a.nvec;
-    if (i >= n) return;
     const int d = (int)(i % a.nvec) * V, q = (int)(i / a.nvec % (W - 1));
     const int s = (int)(i / a.nvec / (W - 1));
     const int64_t b = a.off[s], e = a.off[s + 1], at = e - (W - 1) + q, iq = at - b + (W - 1);
@@ -89,6 +87,25 @@ __device__ __forceinline__ void final_windows(const ConvArgs& a, int64_t i)
         load_row<T, V>(a.initial, ((int64_t)s * (W - 1) + iq) * a.channels + d, v);
     }
     store_row<T, V>(a.final_window, ((int64_t)s * (W - 1) + q) * a.channels + d, v);
+}
+// dinitial of empty histories: their window passes through
+template <class T, int W, int V>
+__device__ __forceinline__ void empty_dinitial(const ConvArgs& a, int64_t i)
+{
+    const int64_t s = i / a.nvec / (W - 1);
+    if (a.off[s + 1] > a.off[s]) return;
+    const int64_t at = i / a.nvec * a.channels + i % a.nvec * V;
+    float v[V];
+#pragma unroll
+    for (int k = 0; k < V; k++) v[k] = 0.0f;
+    if (a.dfinal) load_row<T, V>(a.dfinal, at, v);
+    store_row<T, V>(a.dinitial, at, v);
+}
+// what the blocks behind the strips' do: f(i) for every place i of the windows
+template <int W, class F> __device__ __forceinline__ void every_window_place(const ConvArgs& a, F&& f)
+{
+    const int64_t n = (int64_t)a.n_seq * (W - 1) * a.nvec, step = (int64_t)(gridDim.x - a.main_blocks) * 256;
+    for (int64_t i = (int64_t)(blockIdx.x - a.main_blocks) * 256 + threadIdx.x; i < n; i += step) f(i);
 }
 
 constexpr int kForwardGroup = 4, kBackwardGroup = 2;
@@ -128,7 +145,7 @@ template <class T, int W, int V, bool ONE>
 __global__ __launch_bounds__(256) void conv_forward_kernel(ConvArgs a)
 {
     if ((int)blockIdx.x >= a.main_blocks) {
-        final_windows<T, W, V>(a, (int64_t)(blockIdx.x - a.main_blocks) * 256 + threadIdx.x);
+        every_window_place<W>(a, [&](int64_t i) { final_window<T, W, V>(a, i); });
         return;
     }
     constexpr int GROUP = kForwardGroup;
@@ -195,17 +212,8 @@ __global__ __launch_bounds__(256) void conv_forward_kernel(ConvArgs a)
 template <class T, int W, int V, bool ONE>
 __global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs a)
 {
-    if ((int)blockIdx.x >= a.main_blocks) {   // dinitial of empty histories: their window passes through
-        const int64_t i = (int64_t)(blockIdx.x - a.main_blocks) * 256 + threadIdx.x;
-        if (i >= (int64_t)a.n_seq * (W - 1) * a.nvec) return;
-        const int64_t s = i / a.nvec / (W - 1);
-        if (a.off[s + 1] > a.off[s]) return;
-        const int64_t at = i / a.nvec * a.channels + i % a.nvec * V;
-        float v[V];
-#pragma unroll
-        for (int k = 0; k < V; k++) v[k] = 0.0f;
-        if (a.dfinal) load_row<T, V>(a.dfinal, at, v);
-        store_row<T, V>(a.dinitial, at, v);
+    if ((int)blockIdx.x >= a.main_blocks) {
+        every_window_place<W>(a, [&](int64_t i) { empty_dinitial<T, W, V>(a, i); });
         return;
     }
     constexpr int GROUP = kBackwardGroup;
@@ -505,7 +513,7 @@ extern "C" int rec_history_conv(const rec_conv_desc* d, const void* x, int64_t x
         a.silu = d->silu; a.zero_rest = d->zero_rest; a.strip_rows = g.strip_rows; a.strips = g.strips;
         a.ct = g.ct; a.tiles = g.tiles;
         const int64_t main_blocks = (int64_t)g.blocks_r * g.tiles;
-        const int64_t more = final_window ? ((int64_t)d->n_seq * (d->taps - 1) * l.nvec + 255) / 256 : 0;
+        const int64_t more = final_window ? rec_side_blocks((int64_t)d->n_seq * (d->taps - 1) * l.nvec) : 0;
         if (int rc = check_blocks(main_blocks + more)) return rc;
         if (main_blocks + more == 0) return 0;
         a.main_blocks = (int)main_blocks;
@@ -556,7 +564,7 @@ extern "C" int rec_history_conv_backward(const rec_conv_desc* d, const void* dy,
         a.strips = g.strips; a.ct = g.ct; a.tiles = g.tiles;
         a.partial = sums ? (float*)workspace : nullptr;
         const int64_t main_blocks = (int64_t)g.blocks_r * g.tiles;
-        const int64_t more = dinitial ? ((int64_t)d->n_seq * (d->taps - 1) * l.nvec + 255) / 256 : 0;
+        const int64_t more = dinitial ? rec_side_blocks((int64_t)d->n_seq * (d->taps - 1) * l.nvec) : 0;
         if (int rc = check_blocks(main_blocks + more)) return rc;
         a.main_blocks = (int)main_blocks;
         DeviceScope scope;

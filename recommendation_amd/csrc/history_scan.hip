@@ -297,10 +297,11 @@ template <int LN, int GR> __device__ __forceinline__ void write_sums(float (*to)
 // the walk's take them, a value per thread.
 __device__ __forceinline__ void pass_empty(const ScanArgs& a, const float* from, float* to)
 {
-    const int64_t i = (int64_t)(blockIdx.x - a.main_blocks) * 256 + threadIdx.x, n = (int64_t)a.channels * a.states;
-    if (i >= n * a.n_seq) return;
-    const int64_t s = i / n;
-    if (a.off[s + 1] <= a.off[s]) to[i] = from ? from[i] : 0.0f;
+    const int64_t n = (int64_t)a.channels * a.states, step = (int64_t)(gridDim.x - a.main_blocks) * 256;
+    for (int64_t i = (int64_t)(blockIdx.x - a.main_blocks) * 256 + threadIdx.x; i < n * a.n_seq; i += step) {
+        const int64_t s = i / n;
+        if (a.off[s + 1] <= a.off[s]) to[i] = from ? from[i] : 0.0f;
+    }
 }
 
 // third pass: y, the states that histories end with, and the checkpoints
@@ -995,7 +996,7 @@ extern "C" int rec_history_scan(const rec_scan_desc* d, const rec_scan_inputs* i
         const Cut c = cut_of(d, kForwardBlocks, pass_lanes(d));
         if (int rc = check_workspace(workspace, workspace_bytes, link_bytes(d, c))) return rc;
         const int64_t blocks = (int64_t)c.chunks * c.tiles, n = (int64_t)d->channels * d->states;
-        const int64_t empty_blocks = final_state ? (n * d->n_seq + 255) / 256 : 0;
+        const int64_t empty_blocks = final_state ? rec_side_blocks(n * d->n_seq) : 0;
         if (int rc = check_blocks(blocks + empty_blocks)) return rc;
         if (int rc = check_blocks(c.chunks > 1 ? in_blocks(n, LINK_COLS, LINK_RUNS) : 0)) return rc;
         if (int rc = rec_check_device(d->device)) return rc;
@@ -1057,7 +1058,7 @@ extern "C" int rec_history_scan_backward(const rec_scan_desc* d, const void* dy,
         if (int rc = check_workspace(workspace, workspace_bytes, rec_history_scan_backward_workspace(d))) return rc;
         const Cut c = cut_of(d, kBackwardBlocks, pass_lanes(d));
         const int64_t blocks = (int64_t)c.chunks * c.tiles, n = (int64_t)d->channels * d->states;
-        const int64_t empty_blocks = out->dinitial ? (n * d->n_seq + 255) / 256 : 0;
+        const int64_t empty_blocks = out->dinitial ? rec_side_blocks(n * d->n_seq) : 0;
         const int64_t sum_blocks = c.tiles_per_group > 1 ? (d->rows + SUM_ROWS - 1) / SUM_ROWS : 0;
         const bool params = out->dA || out->dD || out->ddelta_bias;
         for (int64_t launch : {blocks + empty_blocks, sum_blocks, c.chunks > 1 ? in_blocks(n, LINK_COLS, LINK_RUNS) : 0, params ? sum_partials_blocks(n + 2 * d->channels) : 0})

@@ -141,3 +141,36 @@ def test_more_than_a_billion_histories():
     assert all(torch.equal(a, b) for a, b in zip(*out))
     del off
     torch.cuda.empty_cache()
+
+
+def test_final_states_of_a_million_histories():
+    """More than 2^32 values of state, and 2^28 places in windows (two channels each); all but three histories are empty and hand on zeros, or the state they were handed."""
+    n, ch, N = 1050000, 256, 16
+    at = [5, 700000, n - 1]
+    off = torch.zeros(n + 1, dtype=torch.int64, device=DEV)
+    for s in at:
+        off[s + 1:] += 3
+    x, A, B = torch.randn(9, ch, device=DEV), -torch.rand(ch, N, device=DEV), torch.randn(9, 1, N, device=DEV)
+    _, want, kept = ops.history_scan(x, x, A, B, B, seq_off=offsets([0, 3, 6, 9]), want_final=True, want_checkpoints=True)
+    _, fin, _ = ops.history_scan(x, x, A, B, B, seq_off=off, want_final=True)
+    assert fin.shape == (n, ch, N) and torch.equal(fin[at], want)
+    fin[at] = 0
+    assert int(torch.count_nonzero(fin.view(-1, 4096 * 25).abs().amax(1))) == 0
+    fin.fill_(2.0)
+    g = ops.history_scan_backward(x, x, x, A, B, B, seq_off=off, checkpoints=kept, initial=fin, dfinal=fin)
+    assert g.dinitial.shape == fin.shape
+    g.dinitial[at] = 2
+    assert float(g.dinitial.min()) == 2 and float(g.dinitial.max()) == 2
+    del fin, g
+    w = torch.randn(ch, 4, device=DEV)
+    _, want = ops.history_conv(x, w, seq_off=offsets([0, 3, 6, 9]), want_final=True)
+    _, fin = ops.history_conv(x, w, seq_off=off, want_final=True)
+    assert torch.equal(fin[at], want)
+    fin[at] = 0
+    assert float(fin.abs().max()) == 0
+    fin.fill_(3.0)
+    g = ops.history_conv_backward(x, x, w, seq_off=off, initial=fin, dfinal=fin)
+    g.dinitial[at] = 3
+    assert float(g.dinitial.min()) == 3 and float(g.dinitial.max()) == 3
+    del fin, g
+    torch.cuda.empty_cache()
