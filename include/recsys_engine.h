@@ -425,7 +425,7 @@ typedef struct {
     int32_t device, type;
     int64_t rows;             /* at most 2^22 - 1 */
     int64_t n_items;          /* 1 .. 2^31 - 1 */
-    float scale;              /* > 0 (an inverse temperature) */
+    float scale;              /* > 0 (an inverse temperature), at most 2.35e38 */
     int32_t zero_rest;
 } rec_loss_desc;
 

@@ -482,7 +482,7 @@ int check_desc(const rec_loss_desc* d)
     REC_REFUSE(d->type < REC_TYPE_F32 || d->type > REC_TYPE_BF16, "unknown type");
     REC_REFUSE(d->rows < 0 || d->rows > (1 << 22) - 1, "rows must be in 0..2^22-1");   // a launch holds fewer than 2^32 threads
     REC_REFUSE(d->n_items < 1 || d->n_items > INT32_MAX, "n_items must be in 1..2^31-1");
-    REC_REFUSE(!(d->scale > 0.0f) || !isfinite(d->scale), "scale must be positive and finite");
+    REC_REFUSE(!(d->scale > 0.0f) || !isfinite((float)(d->scale * 1.4426950408889634)), "scale must be positive, and scale * log2(e) finite");
     return 0;
 }
 

@@ -3,7 +3,7 @@ import ctypes as C
 
 import pytest
 
-from tests.test_operators_cpu import AT, ScanDesc, ScanGradientPointers, ScanInputs, call, conv, scan
+from tests.test_operators_cpu import AT, ScanDesc, ScanGradientPointers, ScanInputs, call, conv, policy, preference, scan
 
 FAR = 1 << 40
 WIDE = dict(channels=1 << 20, groups=1, y_stride=1 << 20, ws=1 << 60, out=AT + FAR)   # as wide as a call may be
@@ -26,6 +26,8 @@ REFUSED = [
     (lambda: wide_gradient(1024, 64, dA=False), "too many"),
     (lambda: conv(n_seq=(1 << 31) - 1), "n_seq must be"), (lambda: conv("rec_history_conv_backward", n_seq=(1 << 31) - 1), "n_seq must be"),
     (lambda: scan(n_seq=(1 << 31) - 1), "n_seq must be"), (lambda: scan("rec_history_scan_step", n_seq=(1 << 31) - 1), "n_seq must be"),
+    # the exponent's factor, scale * log2(e), is an f32 as well
+    (lambda: preference(scale=2.4e38), "scale must be"), (lambda: policy(scale=3.4e38), "scale must be"), (lambda: policy(scale=2.3e38, device=99), "no such HIP device"),
     (lambda: conv(n_seq=(1 << 31) - 2, device=99), "no such HIP device"), (lambda: scan(n_seq=(1 << 31) - 2, device=99), "no such HIP device"),
 ]
 
