@@ -261,9 +261,9 @@ __device__ __forceinline__ void policy_row(const LossArgs& a, int64_t row, doubl
         const double adv = a.advantage[row], r = exp(logp - (double)a.old_logp[row]);
         // an advantage of 0 asks for nothing, however far the ratio went
         const double open = adv == 0.0 ? 0.0 : r * adv, held = adv == 0.0 ? 0.0 : fmin(fmax(r, 1.0 - a.clip_low), 1.0 + a.clip_high) * adv;
-        const bool nan = r != r || adv != adv;
-        loss = nan ? r * adv : -fmin(open, held);
-        c = nan ? r * adv : open <= held ? -open : 0.0;
+        const bool nan = r != r || open != open || held != held;   // (0 times infinity too; fmin would take the other term)
+        loss = nan ? (double)NAN : -fmin(open, held);
+        c = nan ? (double)NAN : open <= held ? -open : 0.0;
         if (a.ref_logp) {
             const double x = (double)a.ref_logp[row] - logp, e = expm1(x);
             kl = x == (double)INFINITY ? x : e - x;

@@ -174,3 +174,15 @@ def test_final_states_of_a_million_histories():
     assert float(g.dinitial.min()) == 3 and float(g.dinitial.max()) == 3
     del fin, g
     torch.cuda.empty_cache()
+
+
+def test_an_advantage_without_an_end():
+    """0 times infinity is not a number, whichever of the two terms of the minimum it stands in."""
+    inf = float("inf")
+    s = torch.tensor([[0.0, -inf, 1.0]] * 4, device=DEV)
+    item = torch.tensor([1, 1, 0, 0], dtype=torch.int32, device=DEV)       # the masked item has probability 0
+    adv = torch.tensor([inf, -inf, inf, 1.0], device=DEV)
+    zero, one = torch.zeros(4, device=DEV), torch.ones(4, device=DEV)
+    r = ops.policy_loss(s, item, zero, adv, grad_weight=one)
+    assert torch.isnan(r.loss[:2]).all() and float(r.loss[2]) == -inf and torch.isfinite(r.loss[3])
+    assert torch.isnan(r.dscores[:2]).any(1).all() and torch.isfinite(r.dscores[3]).all()
