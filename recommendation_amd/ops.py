@@ -69,6 +69,25 @@ def _bad(what):
     raise ValueError("recsys operators: " + what)
 
 
+def _desc(pack, *fields):
+    try:
+        return pack(*fields)
+    except struct.error as e:
+        _bad(f"a count or the scale is none that the call takes ({e})")
+
+
+def _gpu_of(t, name):
+    if not isinstance(t, torch.Tensor):
+        _bad(f"{name} must be a tensor on the GPU")
+    return t.get_device()
+
+
+def _slots(state):
+    if not isinstance(state, torch.Tensor) or state.dim() != 3:
+        _bad("state must be a tensor of three dimensions, the slots first")
+    return state.shape[0]
+
+
 # A call of a few microseconds spends most of them here, so the checks take one pass over plain attributes; what is wrong is
 # found out in the functions that say so.
 def _first(t, name):
@@ -164,13 +183,13 @@ def _conv(x, weight, bias, n_seq, silu, zero_rest):
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
         _bad("weight must have the shape [channels, taps]")
     taps = weight.shape[1]
-    d = _conv_desc(dev, kind, rows, n_seq, ch, taps, 1 if silu else 0, zero_rest)
+    d = _desc(_conv_desc, dev, kind, rows, n_seq, ch, taps, 1 if silu else 0, zero_rest)
     return d, px, sx, dtype, dev, rows, ch, taps, _whole(weight, "weight", (ch, taps), F32, dev), _whole(bias, "bias", (ch,), F32, dev)
 
 
 def history_conv(x, weight, bias=None, *, seq_off, initial=None, silu=True, want_final=False, out=None):
     """(y, final window or None): x [rows, channels], weight [channels, taps], initial and final [histories, taps - 1, channels]."""
-    off, n = _offsets(seq_off, x.get_device())
+    off, n = _offsets(seq_off, _gpu_of(x, "x"))
     d, px, sx, dtype, dev, rows, ch, taps, w, b = _conv(x, weight, bias, n, silu, 1 if out is None else 0)
     window = (n, max(0, taps - 1), ch)
     i = _whole(initial, "initial", window, dtype, dev)
@@ -183,7 +202,7 @@ def history_conv(x, weight, bias=None, *, seq_off, initial=None, silu=True, want
 
 def history_conv_backward(dy, x, weight, bias=None, *, seq_off, initial=None, silu=True, dfinal=None, out=None):
     """ConvGradients for dy [rows, channels] and dfinal (the final window's gradient); dbias and dinitial are None without bias / initial."""
-    off, n = _offsets(seq_off, x.get_device())
+    off, n = _offsets(seq_off, _gpu_of(x, "x"))
     d, px, sx, dtype, dev, rows, ch, taps, w, b = _conv(x, weight, bias, n, silu, 1 if out is None else 0)
     pg, sg = _rows(dy, "dy", dtype, dev, rows, ch)
     window = (n, max(0, taps - 1), ch)
@@ -203,7 +222,7 @@ def history_conv_backward(dy, x, weight, bias=None, *, seq_off, initial=None, si
 def history_conv_step(x, weight, bias=None, *, state, slots, silu=True, out=None):
     """y [rows, channels] of one click per row; state [slots, taps - 1, channels] (windows, of x's type) is updated in place at
     slots [rows] (int32)."""
-    n = len(state)
+    n = _slots(state)
     d, px, sx, dtype, dev, rows, ch, taps, w, b = _conv(x, weight, bias, n, silu, 0)
     ps = _whole(state, "state", (n, taps - 1, ch), dtype, dev)
     y = torch.empty_like(x) if out is None else out
@@ -225,7 +244,7 @@ def _scan(u, delta, A, B, Cm, D, z, delta_bias, n_seq, initial, softplus, zero_r
     groups = B.shape[1]
     pB, sB = _groups(B, "B", dtype, dev, rows, groups, states)
     pC, sC = _groups(Cm, "C", dtype, dev, rows, groups, states)
-    d = _scan_desc(dev, kind, rows, n_seq, ch, groups, states, 1 if softplus else 0, zero_rest)
+    d = _desc(_scan_desc, dev, kind, rows, n_seq, ch, groups, states, 1 if softplus else 0, zero_rest)
     i = _scan_inputs(pu, pd, pz, pB, pC, su, sd, sz, sB, sC, _whole(A, "A", (ch, states), F32, dev), _whole(D, "D", (ch,), F32, dev) or 0,
                      _whole(delta_bias, "delta_bias", (ch,), F32, dev) or 0, _whole(initial, "initial", (n_seq, ch, states), F32, dev) or 0)
     return d, i, dtype, dev, rows, ch, states
@@ -234,7 +253,7 @@ def _scan(u, delta, A, B, Cm, D, z, delta_bias, n_seq, initial, softplus, zero_r
 def history_scan(u, delta, A, B, C_, D=None, z=None, delta_bias=None, *, seq_off, initial=None, softplus=True, want_final=False, want_checkpoints=False, out=None):
     """(y, final state or None, checkpoints or None): u, delta, z [rows, channels], A [channels, states], B, C [rows, groups, states],
     D, delta_bias [channels], initial and final [histories, channels, states] float32.  The gradient takes the checkpoints."""
-    off, n = _offsets(seq_off, u.get_device())
+    off, n = _offsets(seq_off, _gpu_of(u, "u"))
     d, i, dtype, dev, rows, ch, states = _scan(u, delta, A, B, C_, D, z, delta_bias, n, initial, softplus, 1 if out is None else 0)
     y = torch.empty_like(u) if out is None else out
     py, sy = _rows(y, "out", dtype, dev, rows, ch)
@@ -249,7 +268,7 @@ def history_scan(u, delta, A, B, C_, D=None, z=None, delta_bias=None, *, seq_off
 def history_scan_backward(dy, u, delta, A, B, C_, D=None, z=None, delta_bias=None, *, seq_off, checkpoints, initial=None, softplus=True, dfinal=None):
     """ScanGradients for dy [rows, channels] and dfinal (the final state's gradient); dD, dz, ddelta_bias and dinitial are None
     where the call has no D, z, delta_bias or initial."""
-    off, n = _offsets(seq_off, u.get_device())
+    off, n = _offsets(seq_off, _gpu_of(u, "u"))
     d, i, dtype, dev, rows, ch, states = _scan(u, delta, A, B, C_, D, z, delta_bias, n, initial, softplus, 1)
     pg, sg = _rows(dy, "dy", dtype, dev, rows, ch)
     if checkpoints is None:
@@ -272,7 +291,7 @@ def history_scan_backward(dy, u, delta, A, B, C_, D=None, z=None, delta_bias=Non
 
 def history_scan_step(u, delta, A, B, C_, D=None, z=None, delta_bias=None, *, state, slots, softplus=True, out=None):
     """y [rows, channels] of one click per row; state [slots, channels, states] float32 is updated in place at slots [rows] (int32)."""
-    n = len(state)
+    n = _slots(state)
     d, i, dtype, dev, rows, ch, states = _scan(u, delta, A, B, C_, D, z, delta_bias, n, None, softplus, 0)
     ps = _whole(state, "state", (n, ch, states), F32, dev)
     y = torch.empty_like(u) if out is None else out
@@ -303,7 +322,7 @@ def preference_loss(scores, items, seq_off, ref_logp=None, *, beta=0.1, label_sm
     pairs = n // 2
     p, s = _rows(scores, "scores", dtype, dev, rows, width)
     w, ds, pd, sd = _gradient(scores, grad_weight, pairs, out, dtype, dev, rows, width)
-    d = _loss_desc(dev, kind, rows, width, scale, 1 if out is None else 0)
+    d = _desc(_loss_desc, dev, kind, rows, width, scale, 1 if out is None else 0)
     i, r = _whole(items, "items", (rows,), torch.int32, dev), _whole(ref_logp, "ref_logp", (rows,), F32, dev)
     logp = scores.new_empty(rows, dtype=F32) if out is None else scores.new_zeros(rows, dtype=F32)   # rows of no list: 0
     loss, margin = scores.new_empty((2, pairs), dtype=F32).unbind()
@@ -321,7 +340,7 @@ def policy_loss(scores, items, old_logp, advantage, ref_logp=None, *, clip_low=0
     kind, dtype, dev, rows, width = _first(scores, "scores")
     p, s = _rows(scores, "scores", dtype, dev, rows, width)
     w, ds, pd, sd = _gradient(scores, grad_weight, rows, out, dtype, dev, rows, width)
-    d = _loss_desc(dev, kind, rows, width, scale, 0)
+    d = _desc(_loss_desc, dev, kind, rows, width, scale, 0)
     vec = (rows,)
     i = _whole(items, "items", vec, torch.int32, dev)
     old, adv, ref = _whole(old_logp, "old_logp", vec, F32, dev), _whole(advantage, "advantage", vec, F32, dev), _whole(ref_logp, "ref_logp", vec, F32, dev)

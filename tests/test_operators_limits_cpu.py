@@ -1,7 +1,11 @@
 """More refusals of the device operators (no GPU needed): counts at the ends of their ranges."""
 import ctypes as C
 
+import numpy as np
 import pytest
+import torch
+
+from recommendation_amd import ops
 
 from tests.test_operators_cpu import AT, ScanDesc, ScanGradientPointers, ScanInputs, call, conv, policy, preference, scan
 
@@ -37,3 +41,26 @@ def test_refused_with_a_reason(case):
     f, words = REFUSED[case]
     rc, said = f()
     assert rc == -1 and words in said, (rc, said)
+
+
+def test_what_is_no_tensor_is_refused_as_one():
+    """ValueError, as for a tensor of the wrong kind."""
+    t, a, off = torch.zeros(4, 8), np.zeros((4, 8), np.float32), torch.tensor([0, 4])
+    slots, B = torch.zeros(4, dtype=torch.int32), torch.zeros(4, 1, 2)
+    for bad in (None, a, 3.0):
+        for f, words in [
+            (lambda: ops.history_conv(bad, t, seq_off=off), "x must be"), (lambda: ops.history_conv_backward(t, bad, t, seq_off=off), "x must be"),
+            (lambda: ops.history_scan(bad, t, t, B, B, seq_off=off), "u must be"), (lambda: ops.history_scan_backward(t, bad, t, t, B, B, seq_off=off, checkpoints=t), "u must be"),
+            (lambda: ops.history_conv(t, t, seq_off=bad), "seq_off must be"), (lambda: ops.history_conv_step(bad, t, state=B, slots=slots), "x must be"),
+            (lambda: ops.history_conv_step(t, t, state=bad, slots=slots), "state must be"), (lambda: ops.history_scan_step(t, t, t, B, B, state=bad, slots=slots), "state must be"),
+            (lambda: ops.preference_loss(bad, slots, off), "scores must be"), (lambda: ops.policy_loss(bad, slots, t[0], t[0]), "scores must be"),
+        ]:
+            with pytest.raises(ValueError, match=words):
+                f()
+
+
+def test_numbers_that_no_field_holds_are_refused():
+    with pytest.raises(ValueError, match="a count or the scale"):
+        ops._desc(ops._conv_desc, 0, 0, 4, 1 << 31, 8, 4, 1, 0)
+    with pytest.raises(ValueError, match="a count or the scale"):
+        ops._desc(ops._loss_desc, 0, 0, 4, 16, "1", 0)
