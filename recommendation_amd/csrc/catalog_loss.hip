@@ -564,9 +564,11 @@ void fill(LossArgs& a, const rec_loss_desc* d, const void* scores, int64_t score
 
 extern "C" int64_t rec_preference_loss_workspace(const rec_loss_desc* d, int32_t n_pairs)
 {
-    if (check_desc(d)) return -1;
-    if (n_pairs < 0 || n_pairs > (1 << 22) - 1) { rec_set_error("n_pairs must be in 0..2^22-1"); return -1; }
-    return small_preference(d) ? 0 : workspace_of(d);
+    return rec_guarded([&]() -> int64_t {
+        if (check_desc(d)) return -1;
+        REC_REFUSE(n_pairs < 0 || n_pairs > (1 << 22) - 1, "n_pairs must be in 0..2^22-1");
+        return small_preference(d) ? 0 : workspace_of(d);
+    });
 }
 
 extern "C" int rec_preference_loss(const rec_loss_desc* d, const void* scores, int64_t scores_stride, const int32_t* item,
@@ -610,8 +612,10 @@ extern "C" int rec_preference_loss(const rec_loss_desc* d, const void* scores, i
 
 extern "C" int64_t rec_policy_loss_workspace(const rec_loss_desc* d)
 {
-    if (check_desc(d)) return -1;
-    return whole_policy(d) ? 0 : workspace_of(d);
+    return rec_guarded([&]() -> int64_t {
+        if (check_desc(d)) return -1;
+        return whole_policy(d) ? 0 : workspace_of(d);
+    });
 }
 
 extern "C" int rec_policy_loss(const rec_loss_desc* d, const void* scores, int64_t scores_stride, const int32_t* item,

@@ -529,11 +529,13 @@ extern "C" int rec_history_conv(const rec_conv_desc* d, const void* x, int64_t x
 
 extern "C" int64_t rec_history_conv_backward_workspace(const rec_conv_desc* d)
 {
-    if (check_desc(d)) return -1;
-    // as much as the layout that takes the most blocks needs, whatever the alignment of the arrays turns out to be
-    const int narrow = grid_of(d, d->channels, kBackwardStrip, kBackwardBlocks).blocks_r;
-    const int wide = d->channels % kBackwardVec == 0 ? grid_of(d, d->channels / kBackwardVec, kBackwardStrip, kBackwardBlocks).blocks_r : 0;
-    return (int64_t)(narrow > wide ? narrow : wide) * d->channels * (d->taps + 1) * 4;
+    return rec_guarded([&]() -> int64_t {
+        if (check_desc(d)) return -1;
+        // as much as the layout that takes the most blocks needs, whatever the alignment of the arrays turns out to be
+        const int narrow = grid_of(d, d->channels, kBackwardStrip, kBackwardBlocks).blocks_r;
+        const int wide = d->channels % kBackwardVec == 0 ? grid_of(d, d->channels / kBackwardVec, kBackwardStrip, kBackwardBlocks).blocks_r : 0;
+        return (int64_t)(narrow > wide ? narrow : wide) * d->channels * (d->taps + 1) * 4;
+    });
 }
 
 extern "C" int rec_history_conv_backward(const rec_conv_desc* d, const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,

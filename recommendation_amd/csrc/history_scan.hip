@@ -979,8 +979,10 @@ int check_workspace(const void* p, int64_t has, int64_t needs)
 
 extern "C" int64_t rec_history_scan_workspace(const rec_scan_desc* d)
 {
-    if (check_desc(d)) return -1;
-    return link_bytes(d, cut_of(d, kForwardBlocks, pass_lanes(d)));
+    return rec_guarded([&]() -> int64_t {
+        if (check_desc(d)) return -1;
+        return link_bytes(d, cut_of(d, kForwardBlocks, pass_lanes(d)));
+    });
 }
 
 extern "C" int rec_history_scan(const rec_scan_desc* d, const rec_scan_inputs* in, const int64_t* seq_off, void* y, int64_t y_stride,
@@ -1032,9 +1034,11 @@ static int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 
 extern "C" int64_t rec_history_scan_backward_workspace(const rec_scan_desc* d)
 {
-    if (check_desc(d)) return -1;
-    const Cut c = cut_of(d, kBackwardBlocks, pass_lanes(d));
-    return round16(link_bytes(d, c)) + round16(backward_part_a(d, c)) + backward_part_bc(d, c);
+    return rec_guarded([&]() -> int64_t {
+        if (check_desc(d)) return -1;
+        const Cut c = cut_of(d, kBackwardBlocks, pass_lanes(d));
+        return round16(link_bytes(d, c)) + round16(backward_part_a(d, c)) + backward_part_bc(d, c);
+    });
 }
 
 extern "C" int rec_history_scan_backward(const rec_scan_desc* d, const void* dy, int64_t dy_stride, const rec_scan_inputs* in,

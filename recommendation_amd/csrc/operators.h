@@ -22,7 +22,7 @@ struct DeviceScope {
         if (cond) { rec_set_error(msg); return -1; } \
     } while (0)
 
-template <class F> int rec_guarded(F&& f)
+template <class F> auto rec_guarded(F&& f) -> decltype(f())
 {
     try { return f(); } catch (...) { return -3; }   // only the message's own allocation can throw
 }
