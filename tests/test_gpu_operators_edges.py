@@ -2,7 +2,6 @@
 of a long history, launches whose blocks go around, counts near their limits, and writes beside the outputs.  Needs an MI355X.
 
 Tolerances as in test_gpu_operators: half a step of the value's type, plus a count of roundings times 2^-24 of the terms' size."""
-
 import pytest
 import torch
 
@@ -120,6 +119,48 @@ def test_states_that_grow_over_many_chunks(late):
         close(got, want[name].cpu(), (2 * c * size[name]).cpu(), name)
 
 
+# ------------------------------------------------------------------ launches that go around, and strips of the longest kind
+@pytest.mark.parametrize("tn,rows,ch,W,longest", [
+    ("f32", 60000, 33, 3, 4),          # 15 000 strips of 4 rows, 3750 blocks: two rounds of 1875
+    ("bf16", 1100001, 128, 4, 128),    # 8594 strips of 128 rows, 2149 blocks: two rounds of 1075
+    ("f16", 34000001, 1, 2, 128),      # one channel: 265 626 strips of 128 rows, 256 a block, one round
+])
+def test_conv_gradient_over_more_strips_than_blocks(tn, rows, ch, W, longest):
+    src = Source(ch, TYPES[tn])
+    n = max(4, rows // 100)
+    gpu = torch.Generator(device=DEV).manual_seed(ch)
+    off = torch.cat([torch.zeros(1, dtype=torch.int64), torch.randint(0, rows + 1, (n - 1,), generator=src.gen).sort().values, torch.tensor([rows])]).to(DEV)
+    x, dy = (torch.randn(rows, ch, generator=gpu, device=DEV).to(TYPES[tn]) for _ in range(2))
+    w, b = src.f32(ch, W, scale=0.5)[0], src.f32(ch)[0]
+    t = torch.arange(rows, device=DEV)
+    seq = torch.searchsorted(off, t, right=True) - 1
+    at, left = (t - off[seq])[:, None], (off[seq + 1] - 1 - t)[:, None]
+    x6, dy6, w6 = x.double(), dy.double(), w.double()
+    v, M = b.double().expand(rows, ch), b.double().abs().expand(rows, ch)
+    for j in range(W):
+        k = W - 1 - j
+        term = torch.where(at >= k, torch.roll(x6, k, 0), 0.0) * w6[:, j]
+        v, M = v + term, M + term.abs()
+    g = torch.sigmoid(v)
+    top = float(M.max())
+    y, _ = ops.history_conv(x, w, b, seq_off=off)
+    close_on_gpu(y, v * g, U * (1.1 * (W + 2) * M + (v * g).abs() * (M + 5)), "y")
+    d, D = dy6 * g * (1 + v * (1 - g)), dy6.abs() * (1.1 + 0.5 * M)
+    del v, M, g, y
+    got = ops.history_conv_backward(dy, x, w, b, seq_off=off)
+    c = U * (2 * W + 16 + top)
+    want = sum(w6[:, W - 1 - k] * torch.where(left >= k, torch.roll(d, -k, 0), 0.0) for k in range(W))
+    size = sum(w6[:, W - 1 - k].abs() * torch.where(left >= k, torch.roll(D, -k, 0), 0.0) for k in range(W))
+    close_on_gpu(got.dx, want, c * size, "dx")
+    # a thread adds up two strips one after the other at most, a block its 256 threads at most; blocks are added in 64 bits
+    few = c + U * (2 * longest + 256)
+    for j in range(W):
+        k = W - 1 - j
+        behind = torch.where(at >= k, torch.roll(x6, k, 0), 0.0)
+        close_on_gpu(got.dweight[:, j], (d * behind).sum(0), few * (D * behind.abs()).sum(0), "dweight")
+    close_on_gpu(got.dbias, d.sum(0), few * D.sum(0), "dbias")
+
+
 def test_more_than_a_billion_histories():
     """Histories whose numbers are beyond 2^30: the middle of two of them is beyond an int before it is halved."""
     n = (1 << 30) + 21
@@ -186,3 +227,66 @@ def test_an_advantage_without_an_end():
     r = ops.policy_loss(s, item, zero, adv, grad_weight=one)
     assert torch.isnan(r.loss[:2]).all() and float(r.loss[2]) == -inf and torch.isfinite(r.loss[3])
     assert torch.isnan(r.dscores[:2]).any(1).all() and torch.isfinite(r.dscores[3]).all()
+
+
+# ------------------------------------------------------------------ writes beside the outputs
+class Carved:
+    """Outputs and workspace of a call, cut from one buffer of a known pattern with 64 KiB between them."""
+    MARGIN, FILL = 1 << 16, 0xA5
+
+    def __init__(self, size=1 << 24):
+        self.buf = torch.full((size,), self.FILL, dtype=torch.uint8, device=DEV)
+        self.mine = torch.zeros(size, dtype=torch.bool, device=DEV)
+        self.at = 0
+
+    def __call__(self, nbytes, rows=1, gap=0):
+        """`rows` pieces of nbytes, `gap` bytes of margin behind each."""
+        start = self.at + self.MARGIN
+        for r in range(rows):
+            self.mine[start + r * (nbytes + gap):start + r * (nbytes + gap) + nbytes] = True
+        self.at = (start + rows * (nbytes + gap) + 255) // 256 * 256
+        assert self.at + self.MARGIN <= self.buf.numel()
+        return self.buf.data_ptr() + start
+
+    def check(self):
+        torch.cuda.synchronize()
+        assert bool((self.buf[~self.mine] == self.FILL).all())
+
+
+@pytest.mark.parametrize("off", [[0, 50, 20, 64, 10], [-9, 3, 1 << 40, 64, 64], [70, 80, 90, 1 << 60, -(1 << 60)], [400, 300, 200, 100, 0], [0, 130, 130, 350, 400]],
+                         ids=["out of order", "beyond", "far", "falling", "in order"])
+def test_offsets_that_break_the_rules_write_nothing_beside_the_outputs(off):
+    rows, ch, W, N, items = 400, 20, 4, 8, 32
+    o = offsets(off)
+    x, dy, B = torch.randn(rows, ch, device=DEV), torch.randn(rows, ch, device=DEV), torch.randn(rows, 1, N, device=DEV)
+    w, A = torch.randn(ch, W, device=DEV), -torch.rand(ch, N, device=DEV)
+    i, df = torch.randn(4, W - 1, ch, device=DEV), torch.randn(4, W - 1, ch, device=DEV)
+    h, dh = torch.randn(4, ch, N, device=DEV), torch.randn(4, ch, N, device=DEV)
+    kept = torch.randn(-(-rows // 16), ch, N, device=DEV)
+    s, item, gw = torch.randn(rows, items, device=DEV), torch.randint(0, items, (rows,), device=DEV).int(), torch.ones(2, device=DEV)
+    stream = torch.cuda.current_stream().cuda_stream
+    p = lambda t: t.data_ptr()  # noqa: E731
+    call = lambda name, *a: capi._check(ops._fn(name)(*a))  # noqa: E731
+    for zero_rest in (0, 1):
+        c = Carved()
+        d = ops._conv_desc(0, 0, rows, 4, ch, W, 1, zero_rest)
+        call("rec_history_conv", d, p(x), ch, p(w), None, p(o), p(i), c(4 * ch, rows, 16), ch + 4, c(4 * i.numel()), stream)
+        size = ops._fn("rec_history_conv_backward_workspace")(d)
+        call("rec_history_conv_backward", d, p(dy), ch, p(x), ch, p(w), None, p(o), p(i), p(df), c(4 * ch, rows, 16), ch + 4, c(4 * w.numel()), c(4 * ch), c(4 * i.numel()),
+             c(size), size, stream)
+        d = ops._scan_desc(0, 0, rows, 4, ch, 1, N, 1, zero_rest)
+        for state in (h, None):
+            inputs = ops._scan_inputs(p(x), p(x), 0, p(B), p(B), ch, ch, 0, N, N, p(A), 0, 0, p(state) if state is not None else 0)
+            size = ops._fn("rec_history_scan_workspace")(d)
+            assert size > 0    # several chunks
+            call("rec_history_scan", d, inputs, p(o), c(4 * ch, rows, 16), ch + 4, c(4 * h.numel()), c(4 * kept.numel()), c(size), size, stream)
+            size = ops._fn("rec_history_scan_backward_workspace")(d)
+            g = ops._scan_gradients(c(4 * rows * ch), c(4 * rows * ch), 0, c(4 * rows * N), c(4 * rows * N), c(4 * A.numel()), c(4 * ch), c(4 * ch), c(4 * h.numel()) if state is not None else 0)
+            call("rec_history_scan_backward", d, p(dy), ch, inputs, p(o), p(kept), p(dh) if state is not None else None, g, c(size), size, stream)
+        for n in (rows, 40):   # three launches, and one
+            d = ops._loss_desc(0, 0, n, items, 1.0, zero_rest)
+            size = ops._fn("rec_preference_loss_workspace")(d, 2)
+            assert (size > 0) == (n > 64)
+            call("rec_preference_loss", d, p(s), items, p(item), p(o), 2, None, 0.1, 0.0, p(gw), c(8), c(8), c(4 * n), c(4 * items, n, 12), items + 3, c(size) if size else None, size, stream)
+            call("rec_preference_loss", d, p(s), items, p(item), p(o), 2, None, 0.1, 0.0, None, c(8), c(8), c(4 * n), None, 0, c(size) if size else None, size, stream)
+        c.check()
