@@ -497,8 +497,17 @@ int splits_of(const rec_loss_desc* d)
 }
 
 int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
-// one launch does it all, and nothing passes between launches
-bool small_preference(const rec_loss_desc* d) { return d->rows <= kSmallRows && d->rows * d->n_items <= 131072; }
+// One launch does it all, and nothing passes between launches: a wavefront reads a row by itself, a pair's block 16 at a time, so rows
+// are short, and few to a pair (how they are spread over the pairs the host does not know).  One launch against three, us in a graph:
+// 2 rows of 4000, 8000, 16 000, 65 536 f32 items 9.5 / 12.5, 13.0 / 12.7, 19 / 13, 60 / 12; 6 of 4000 and 8000 11 / 13, 15 / 13; 16 of
+// 2000 and 4000 11 / 13, 15 / 13; a second round pays below 25 rows: 24 of 300 and 1000 9.0 / 11.0, 11.6 / 11.7; 32 of 500 11.4 / 10.9; 64
+// of 2000 34 / 13 in one pair, 12 / 13 in four, 8 / 13 in 32.
+bool small_preference(const rec_loss_desc* d, int n_pairs)
+{
+    if (d->rows > kSmallRows || d->rows * d->n_items > 131072) return false;
+    if (d->rows > 16 * (int64_t)n_pairs) return d->rows <= 24 * (int64_t)n_pairs && d->n_items <= 1000;
+    return d->n_items <= 8000 && d->rows * d->n_items <= 32768 * (int64_t)n_pairs;
+}
 // (64, 256 and 900 rows of 20 000 bf16 items: calls of 13, 14 and 20 us, 20, 21 and 36 by three launches over parts of rows; 900 of
 // 200 000 items 158 and 194)
 bool whole_policy(const rec_loss_desc* d) { return splits_of(d) == 1 || d->rows >= 512 || d->n_items * rec_type_size(d->type) < 65536; }
@@ -567,7 +576,7 @@ extern "C" int64_t rec_preference_loss_workspace(const rec_loss_desc* d, int32_t
     return rec_guarded([&]() -> int64_t {
         if (check_desc(d)) return -1;
         REC_REFUSE(n_pairs < 0 || n_pairs > (1 << 22) - 1, "n_pairs must be in 0..2^22-1");
-        return small_preference(d) ? 0 : workspace_of(d);
+        return small_preference(d, n_pairs) ? 0 : workspace_of(d);
     });
 }
 
@@ -582,15 +591,15 @@ extern "C" int rec_preference_loss(const rec_loss_desc* d, const void* scores, i
         REC_REFUSE(!seq_off || (d->rows > 0 && (!scores || !item || !logp)) || (n_pairs > 0 && (!loss || !margin)), "null argument");
         REC_REFUSE(!isfinite(beta), "beta must be finite");
         REC_REFUSE(!(smoothing >= 0.0f && smoothing <= 1.0f), "smoothing must be in 0..1");
-        if (int rc = check_call(d, scores, scores_stride, grad_weight, n_pairs, dscores, dscores_stride, workspace, workspace_bytes, small_preference(d) ? 0 : workspace_of(d))) return rc;
+        if (int rc = check_call(d, scores, scores_stride, grad_weight, n_pairs, dscores, dscores_stride, workspace, workspace_bytes, small_preference(d, n_pairs) ? 0 : workspace_of(d))) return rc;
         LossArgs a = {};
         fill(a, d, scores, scores_stride, item, ref_logp, grad_weight, loss, logp, dscores, dscores_stride, workspace);
         a.off = seq_off; a.n_seq = 2 * n_pairs; a.margin = margin; a.beta = beta; a.smoothing = smoothing;
         DeviceScope scope;
         HIP_TRY(scope.enter(d->device));
         hipStream_t st = (hipStream_t)stream;
-        // (one pair of 6 x 2848 f32: 9.5 us, three launches of 4.8, 4.0 and 3.4 us otherwise; 16 rows at a time pay up to some thousand items)
-        if (d->rows > 0 && small_preference(d)) {
+        // (one pair of 6 x 2848 f32: 9.5 us, three launches of 4.8, 4.0 and 3.4 us otherwise)
+        if (d->rows > 0 && small_preference(d, n_pairs)) {
 #define CALL(T) preference_small_kernel<T><<<n_pairs ? (unsigned)n_pairs : 1u, 1024, 0, st>>>(a)
             LOSS_DISPATCH(CALL)
 #undef CALL

@@ -7,6 +7,7 @@ import torch
 
 from recommendation_amd import capi, ops
 from tests import operators_ref as ref
+from tests import test_gpu_operators as base
 from tests.test_gpu_operators import DEV, LEAST, TYPES, U, Source, close, offsets
 
 pytestmark = pytest.mark.gpu
@@ -290,3 +291,16 @@ def test_offsets_that_break_the_rules_write_nothing_beside_the_outputs(off):
             call("rec_preference_loss", d, p(s), items, p(item), p(o), 2, None, 0.1, 0.0, p(gw), c(8), c(8), c(4 * n), c(4 * items, n, 12), items + 3, c(size) if size else None, size, stream)
             call("rec_preference_loss", d, p(s), items, p(item), p(o), 2, None, 0.1, 0.0, None, c(8), c(8), c(4 * n), None, 0, c(size) if size else None, size, stream)
         c.check()
+
+
+# ------------------------------------------------------------------ preferences on both sides of the one launch's bounds
+@pytest.mark.parametrize("case", [
+    ("f32", 24, 999, [0, 20, 24], 1.0, 0.1, 0.1, True),                  # one launch, two rounds of a block's wavefronts
+    ("bf16", 25, 999, [0, 20, 25], 1.0, 0.1, 0.1, True),                 # three launches
+    ("f16", 3, 8000, [1, 2, 3], 1.0, 0.0, 0.1, False), ("f16", 3, 8001, [1, 2, 3], 1.0, 0.0, 0.1, False),
+    ("bf16", 64, 700, [0, 1, 30, 31, 60, 60, 64], 1.0, 0.0, 0.1, True),  # one launch for rows that are nearly all one pair's
+    ("f32", 64, 40, [64], 1.0, 0.0, 0.1, True),                          # no pairs
+], ids=lambda c: f"{c[0]}-{c[1]}x{c[2]}")
+@pytest.mark.parametrize("layout", ["packed", "strided", "in place"])
+def test_preferences_in_one_launch_and_in_three(case, layout):
+    base.test_preference_loss(case, layout)

@@ -7,7 +7,7 @@ import torch
 
 from recommendation_amd import ops
 
-from tests.test_operators_cpu import AT, ScanDesc, ScanGradientPointers, ScanInputs, call, conv, policy, preference, scan
+from tests.test_operators_cpu import AT, LossDesc, ScanDesc, ScanGradientPointers, ScanInputs, call, conv, policy, preference, scan
 
 FAR = 1 << 40
 WIDE = dict(channels=1 << 20, groups=1, y_stride=1 << 20, ws=1 << 60, out=AT + FAR)   # as wide as a call may be
@@ -64,3 +64,11 @@ def test_numbers_that_no_field_holds_are_refused():
         ops._desc(ops._conv_desc, 0, 0, 4, 1 << 31, 8, 4, 1, 0)
     with pytest.raises(ValueError, match="a count or the scale"):
         ops._desc(ops._loss_desc, 0, 0, 4, 16, "1", 0)
+
+
+@pytest.mark.parametrize("rows,items,pairs,one", [(6, 2848, 1, True), (2, 65536, 1, False), (2, 4000, 1, True), (16, 8000, 1, False), (16, 2000, 1, True), (64, 500, 1, False), (64, 500, 32, True),
+                                                  (24, 1000, 1, True), (24, 2000, 1, False), (64, 2000, 8, True), (65, 16, 30, False), (4, 33, 0, False)])
+def test_long_rows_and_long_lists_are_not_one_block_s(rows, items, pairs, one):
+    """A preference call of one launch needs no workspace."""
+    d = LossDesc(device=0, type=0, rows=rows, n_items=items, scale=1.0)
+    assert (ops._fn("rec_preference_loss_workspace")(C.byref(d), pairs) == 0) == one
