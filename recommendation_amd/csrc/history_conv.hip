@@ -101,7 +101,13 @@ __device__ __forceinline__ void empty_dinitial(const ConvArgs& a, int64_t i)
     if (a.dfinal) load_row<T, V>(a.dfinal, at, v);
     store_row<T, V>(a.dinitial, at, v);
 }
-// what the blocks behind the strips' do: f(i) for every place i of the windows
+// what the blocks behind the strips' do: f(i) for every place i of the windows, one per thread up to 2^28 of them, several where there
+// are more, for these alone must not make a launch too large
+int64_t window_blocks(const rec_conv_desc* d, int64_t nvec)
+{
+    const int64_t n = (int64_t)d->n_seq * (d->taps - 1) * nvec;
+    return n < (1ll << 28) ? (n + 255) / 256 : 1ll << 20;
+}
 template <int W, class F> __device__ __forceinline__ void every_window_place(const ConvArgs& a, F&& f)
 {
     const int64_t n = (int64_t)a.n_seq * (W - 1) * a.nvec, step = (int64_t)(gridDim.x - a.main_blocks) * 256;
@@ -513,7 +519,7 @@ extern "C" int rec_history_conv(const rec_conv_desc* d, const void* x, int64_t x
         a.silu = d->silu; a.zero_rest = d->zero_rest; a.strip_rows = g.strip_rows; a.strips = g.strips;
         a.ct = g.ct; a.tiles = g.tiles;
         const int64_t main_blocks = (int64_t)g.blocks_r * g.tiles;
-        const int64_t more = final_window ? rec_side_blocks((int64_t)d->n_seq * (d->taps - 1) * l.nvec) : 0;
+        const int64_t more = final_window ? window_blocks(d, l.nvec) : 0;
         if (int rc = check_blocks(main_blocks + more)) return rc;
         if (main_blocks + more == 0) return 0;
         a.main_blocks = (int)main_blocks;
@@ -566,7 +572,7 @@ extern "C" int rec_history_conv_backward(const rec_conv_desc* d, const void* dy,
         a.strips = g.strips; a.ct = g.ct; a.tiles = g.tiles;
         a.partial = sums ? (float*)workspace : nullptr;
         const int64_t main_blocks = (int64_t)g.blocks_r * g.tiles;
-        const int64_t more = dinitial ? rec_side_blocks((int64_t)d->n_seq * (d->taps - 1) * l.nvec) : 0;
+        const int64_t more = dinitial ? window_blocks(d, l.nvec) : 0;
         if (int rc = check_blocks(main_blocks + more)) return rc;
         a.main_blocks = (int)main_blocks;
         DeviceScope scope;

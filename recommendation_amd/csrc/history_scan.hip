@@ -294,15 +294,24 @@ template <int LN, int GR> __device__ __forceinline__ void write_sums(float (*to)
 }
 
 // Empty histories: their state passes through (forwards initial -> final_state, backwards dfinal -> dinitial).  Blocks behind
-// the walk's take them, a value per thread.
+// the walk's take them, a value per thread; so many that they alone would make a launch too large have one of their own, whose
+// threads go around (a loop in the walk's kernels costs the gradient 3 % where it goes around once).
+__device__ __forceinline__ void pass_value(const ScanArgs& a, const float* from, float* to, int64_t i)
+{
+    const int64_t s = i / ((int64_t)a.channels * a.states);
+    if (a.off[s + 1] <= a.off[s]) to[i] = from ? from[i] : 0.0f;
+}
 __device__ __forceinline__ void pass_empty(const ScanArgs& a, const float* from, float* to)
 {
-    const int64_t n = (int64_t)a.channels * a.states, step = (int64_t)(gridDim.x - a.main_blocks) * 256;
-    for (int64_t i = (int64_t)(blockIdx.x - a.main_blocks) * 256 + threadIdx.x; i < n * a.n_seq; i += step) {
-        const int64_t s = i / n;
-        if (a.off[s + 1] <= a.off[s]) to[i] = from ? from[i] : 0.0f;
-    }
+    const int64_t i = (int64_t)(blockIdx.x - a.main_blocks) * 256 + threadIdx.x;
+    if (i < (int64_t)a.channels * a.states * a.n_seq) pass_value(a, from, to, i);
 }
+__global__ __launch_bounds__(256) void scan_pass_empty_kernel(ScanArgs a, const float* from, float* to)
+{
+    const int64_t n = (int64_t)a.channels * a.states * a.n_seq;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) pass_value(a, from, to, i);
+}
+constexpr int64_t kManyStates = 1 << 28;
 
 // third pass: y, the states that histories end with, and the checkpoints
 template <class T, int LN>
@@ -998,7 +1007,8 @@ extern "C" int rec_history_scan(const rec_scan_desc* d, const rec_scan_inputs* i
         const Cut c = cut_of(d, kForwardBlocks, pass_lanes(d));
         if (int rc = check_workspace(workspace, workspace_bytes, link_bytes(d, c))) return rc;
         const int64_t blocks = (int64_t)c.chunks * c.tiles, n = (int64_t)d->channels * d->states;
-        const int64_t empty_blocks = final_state ? rec_side_blocks(n * d->n_seq) : 0;
+        const bool many_states = final_state && n * d->n_seq >= kManyStates;
+        const int64_t empty_blocks = final_state && !many_states ? (n * d->n_seq + 255) / 256 : 0;
         if (int rc = check_blocks(blocks + empty_blocks)) return rc;
         if (int rc = check_blocks(c.chunks > 1 ? in_blocks(n, LINK_COLS, LINK_RUNS) : 0)) return rc;
         if (int rc = rec_check_device(d->device)) return rc;
@@ -1023,6 +1033,7 @@ extern "C" int rec_history_scan(const rec_scan_desc* d, const rec_scan_inputs* i
             SCAN_TYPES(SCAN_PASS_LANES, CALL)
 #undef CALL
         }
+        if (many_states) scan_pass_empty_kernel<<<kManyStates / 256, 256, 0, st>>>(a, a.initial, a.final_state);
         HIP_TRY(hipGetLastError());
         return 0;
     });
@@ -1062,7 +1073,8 @@ extern "C" int rec_history_scan_backward(const rec_scan_desc* d, const void* dy,
         if (int rc = check_workspace(workspace, workspace_bytes, rec_history_scan_backward_workspace(d))) return rc;
         const Cut c = cut_of(d, kBackwardBlocks, pass_lanes(d));
         const int64_t blocks = (int64_t)c.chunks * c.tiles, n = (int64_t)d->channels * d->states;
-        const int64_t empty_blocks = out->dinitial ? rec_side_blocks(n * d->n_seq) : 0;
+        const bool many_states = out->dinitial && n * d->n_seq >= kManyStates;
+        const int64_t empty_blocks = out->dinitial && !many_states ? (n * d->n_seq + 255) / 256 : 0;
         const int64_t sum_blocks = c.tiles_per_group > 1 ? (d->rows + SUM_ROWS - 1) / SUM_ROWS : 0;
         const bool params = out->dA || out->dD || out->ddelta_bias;
         for (int64_t launch : {blocks + empty_blocks, sum_blocks, c.chunks > 1 ? in_blocks(n, LINK_COLS, LINK_RUNS) : 0, params ? sum_partials_blocks(n + 2 * d->channels) : 0})
@@ -1101,6 +1113,7 @@ extern "C" int rec_history_scan_backward(const rec_scan_desc* d, const void* dy,
 #undef CALL
             }
         }
+        if (many_states) scan_pass_empty_kernel<<<kManyStates / 256, 256, 0, st>>>(a, a.dfinal, a.dinitial);
         if (sum_blocks > 0) {
             if (d->type == REC_TYPE_F32) scan_sum_groups_kernel<float><<<(unsigned)sum_blocks, 256, 0, st>>>(a);
             else if (d->type == REC_TYPE_F16) scan_sum_groups_kernel<_Float16><<<(unsigned)sum_blocks, 256, 0, st>>>(a);

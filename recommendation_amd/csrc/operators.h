@@ -51,10 +51,6 @@ inline bool rec_overlap(const RowsOf& a, const RowsOf& b)
     return ahead < a.width || a.stride - ahead < b.width;
 }
 
-// Blocks of 256 threads for n values that a launch takes on the side (states and windows of empty histories), one per thread up to
-// 2^28 of them, several where there are more: these alone must not make a launch too large.
-inline int64_t rec_side_blocks(int64_t n) { return n < (1ll << 28) ? (n + 255) / 256 : 1ll << 20; }
-
 inline int rec_type_size(int type) { return type == REC_TYPE_F32 ? 4 : 2; }
 inline bool rec_aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
