@@ -514,8 +514,9 @@ bool whole_policy(const rec_loss_desc* d) { return splits_of(d) == 1 || d->rows 
 // Threads for a row that a block reads and then turns into its gradient.  Small blocks keep more rows in flight, and a row's loads
 // over the waits of another's sums; the rows in flight, 2048 threads' worth on each of 256 compute units, should stay within 210 MB
 // of the Infinity Cache.  Few rows take more, down to two or three 16-byte loads a thread, until a quarter of the lanes are
-// busy.  (bf16: 20 000 rows of 20 000 items 599 us with 1024 threads, 356, 350, 345 with 256, 128, 192; 4000 of 60 000 items 234, 198, 206
-// with 1024, 512, 256; 300 of 8000 items 12, 10, 7.6 with 64, 128, 512; f32, 50 000 of 4000 items 579, 311, 326 with 512, 128, 64.)
+// busy.  (bf16: 20 000 rows of 20 000 items 599 us with 1024 threads, 356 with 256, 350 with the rule's 128; 4000 of 60 000 items 234, 206
+// with 1024, 256, 198 with the rule's 512; 300 of 8000 items 12, 10 with 64, 128, 7.6 with the rule's 512; f32, 50 000 of 4000 items 579,
+// 311 with 512, 128, 326 with the rule's 64.)
 int row_threads(const rec_loss_desc* d)
 {
     const int64_t bytes = d->n_items * rec_type_size(d->type);
