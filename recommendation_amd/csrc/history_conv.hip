@@ -3,12 +3,13 @@
 //   v[t][d] = bias[d] + sum_{j < W} weight[d][j] x[t - (W-1) + j][d],   y = silu(v) or v
 //
 // About 2 W flop per element read and written, four times that in the gradient: bound by memory, the gradient by its vector
-// instructions as much (issued in 68 % of its cycles, while it moves 3.4 TB/s).  A thread owns V neighbouring channels and walks a strip of consecutive rows with the window in
-// registers, so a row is read once plus W-1 rows of halo per strip (these come from the cache), its loads a few rows ahead.
-// Where a history begins inside the strip, the window is replaced by that history's own.  A wavefront has one strip where the
-// channels allow: what it knows of the histories is scalar then, and the registers hold windows (gradient over 598 655 x 128
-// bf16, W = 4: 88 registers and 134 us against 138 and 165 with a strip per thread).  V = 2: with V = 4 the gradient takes 205 us, with 8 375,
-// their registers leaving one or two wavefronts per SIMD.  The forward call over the same rows takes 69 us, 4.4 TB/s.
+// instructions as much (issued in 68 % of its cycles, while it moves 3.4 TB/s).  A thread owns V neighbouring channels and walks a
+// strip of consecutive rows with the window in registers, so a row is read once plus W-1 rows of halo per strip (these come from
+// the cache), its loads a few rows ahead.  Where a history begins inside the strip, the window is replaced by that history's own.  A
+// wavefront has one strip where the channels allow: what it knows of the histories is scalar then, and the registers hold windows
+// (gradient over 598 655 x 128 bf16, W = 4: 88 registers and 134 us against 138 and 165 with a strip per thread).  V = 2: with V = 4
+// the gradient takes 205 us, with 8 375, their registers leaving one or two wavefronts per SIMD.  The forward call over the same rows
+// takes 69 us, 4.4 TB/s.
 #include "operators.h"
 
 namespace {
